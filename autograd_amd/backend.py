@@ -31,7 +31,7 @@ import numpy as np
 
 from .op import (AddLayerNormOp, AddOp, AddRMSNormOp, BiasGELUOp, ContiguousOp, CrossEntropyLossOp, EmbeddingSumOp, ExpOp,
                  GatherOp, GELUOp, LayerNormOp, LogOp, MulOp, PermuteOp, ReLUSquaredOp, ReshapeOp, RMSNormOp, RopeOp,
-                 RsqrtOp, SoftmaxOp, SwiGLUOp, TransposeOp, ViewOp)
+                 RsqrtOp, SoftmaxOp, SwiGLUOp, TokenLogprobsOp, TopKDistillOp, TransposeOp, ViewOp)
 from .scratch import equal_slots, single_slot
 from .utils import (bf16_bits, bf16_bits_to_f32_array, contiguous_strides, f32_array_to_bf16_bits, f32_bits,
                     is_bf16, mul_bcast_kind, storage_dtype, xavier_uniform)
@@ -159,6 +159,8 @@ class HipBackend(Backend):
             AddRMSNormOp: self.hip_add_norm_forward,
             RopeOp: self.hip_rope_forward,
             CrossEntropyLossOp: self.hip_cross_entropy_forward,
+            TokenLogprobsOp: self.hip_token_logprobs_forward,
+            TopKDistillOp: self.hip_distill_forward,
             MulOp: self.hip_mul_forward,
             ExpOp: self.hip_unary_forward,
             LogOp: self.hip_unary_forward,
@@ -184,6 +186,8 @@ class HipBackend(Backend):
             AddRMSNormOp: self.hip_add_norm_backward,
             RopeOp: self.hip_rope_backward,
             CrossEntropyLossOp: self.hip_cross_entropy_backward,
+            TokenLogprobsOp: self.hip_token_logprobs_backward,
+            TopKDistillOp: self.hip_distill_backward,
             MulOp: self.hip_mul_backward,
             ExpOp: self.hip_unary_backward,
             LogOp: self.hip_unary_backward,
@@ -884,6 +888,55 @@ class HipBackend(Backend):
         self._launch("cross_entropy_backward", [logits, labels, loss.grad, lse, logits.grad],
                      [_dt(logits)] + _lo_hi(rows) + [V, self._grad_flag(loss.op, logits),
                                                     _mask(logits, labels, loss.grad, lse, logits.grad)])
+
+    # -- token log probabilities, distillation from a teacher's top logits ------------------------
+    # These have typed methods on the context instead of kernel names: the name table is the reference's.
+    @staticmethod
+    def _rows_classes(logits):
+        return prod(logits.shape[:-1]), logits.shape[-1]
+
+    def hip_token_logprobs_forward(self, inputs, outputs, scratch=None):
+        logits, tokens = inputs
+        op = outputs[0].op.op
+        logp, lse, entropy, top_ids, top_logp = op.split(outputs)
+        rows, V = self._rows_classes(logits)
+        self.ctx.token_logprobs_forward(_dt(logits), *_ids(logits, tokens, logp, entropy, lse, top_ids, top_logp),
+                                        rows, V, V, op.top, op.scale)
+
+    def hip_token_logprobs_backward(self, inputs, outputs, scratch=None):
+        logits, tokens = inputs
+        op = outputs[0].op.op
+        logp, lse, entropy, _, _ = op.split(outputs)
+        if not logits.requires_grad or logits.grad is None:
+            return
+        flag = self._grad_flag(logp.op, logits)
+        dentropy = entropy.grad if entropy is not None else None
+        if logp.grad is None and dentropy is None:
+            if not flag:                # the first writer, with nothing to write but zeros
+                self.fill(logits.grad, 0)
+            return
+        rows, V = self._rows_classes(logits)
+        self.ctx.token_logprobs_backward(_dt(logits), *_ids(logits, tokens, lse, entropy, logp.grad, dentropy, logits.grad),
+                                         rows, V, V, op.scale, flag)
+
+    def hip_distill_forward(self, inputs, outputs, scratch=None):
+        logits, teacher_ids, teacher_values = inputs
+        loss, stats = outputs
+        op = loss.op.op
+        rows, V = self._rows_classes(logits)
+        self.ctx.topk_distill_forward(_dt(logits), *_ids(logits, teacher_ids, teacher_values, loss, stats),
+                                      rows, V, V, teacher_ids.shape[-1], op.scale, op.teacher_scale, int(op.tail))
+
+    def hip_distill_backward(self, inputs, outputs, scratch=None):
+        logits, teacher_ids, teacher_values = inputs
+        loss, stats = outputs
+        if loss.grad is None or not logits.requires_grad or logits.grad is None:
+            return
+        op = loss.op.op
+        rows, V = self._rows_classes(logits)
+        self.ctx.topk_distill_backward(_dt(logits), *_ids(logits, teacher_ids, teacher_values, loss.grad, stats, logits.grad),
+                                       rows, V, V, teacher_ids.shape[-1], op.scale, op.teacher_scale, int(op.tail),
+                                       self._grad_flag(loss.op, logits))
 
     # -- fills and copies (backend.py:5069-5113) ---------------------------------------
     def fill_storage(self, storage, value):

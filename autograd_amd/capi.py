@@ -20,6 +20,8 @@ NORM_LAYER, NORM_RMS = 0, 1
 ACC_INPUT_GRAD, ACC_PARAM_GRAD, ACC_INPUT_GRAD2, ACC_PARAM_GRAD2, PARAM_GRAD_BF16, DEFER_PARAM_GRAD = 1, 2, 4, 8, 16, 32
 UNARY_EXP, UNARY_LOG, UNARY_RSQRT = 0, 1, 2
 MUL_SAME, MUL_ROW, MUL_COL, MUL_SCALAR = 0, 1, 2, 3
+DISTILL_RENORM, DISTILL_TAIL = 0, 1
+MAX_TOP = 128
 OK, EINVAL, EHIP, ENOKERNEL, EINDEX, EWORKSPACE = 0, -1, -2, -3, -4, -5
 NOALLOC_SCRATCH_BYTES = 32 << 20
 
@@ -117,6 +119,12 @@ SIGNATURES = {
     "agrad_cross_entropy_forward": (_int, [_ctx, _int, _ptr, _ptr, _ptr, _ptr, _u64, _u32]),
     "agrad_cross_entropy_backward": (_int, [_ctx, _int, _ptr, _ptr, _ptr, _ptr, _ptr, _u64, _u32, _u32]),
     "agrad_cross_entropy_fused": (_int, [_ctx, _int, _ptr, _ptr, _ptr, _ptr, _ptr, _u64, _u32, _u64, _f32, _u32]),
+    "agrad_buffer_address": (_int, [_ctx, _u64, _u64, _u64, C.POINTER(_ptr)]),
+    "agrad_token_logprobs_forward": (_int, [_ctx, _int, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _u64, _u32, _u64, _u32, _f32]),
+    "agrad_token_logprobs_backward": (_int, [_ctx, _int, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _u64, _u32, _u64, _f32, _u32]),
+    "agrad_topk_distill_forward": (_int, [_ctx, _int, _ptr, _ptr, _ptr, _ptr, _ptr, _u64, _u32, _u64, _u32, _f32, _f32, _int]),
+    "agrad_topk_distill_backward": (_int, [_ctx, _int, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _u64, _u32, _u64, _u32, _f32, _f32, _int, _u32]),
+    "agrad_topk_distill_fused": (_int, [_ctx, _int, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _u64, _u32, _u64, _u32, _f32, _f32, _f32, _int]),
     "agrad_adamw8bit_step": (_int, [_ctx, _int, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr, _u64, _u64,
                                     _f32, _f32, _f32, _f32, _f32, _f32, _f32, _int]),
     "agrad_adamw_step": (_int, [_ctx, _int, _ptr, _ptr, _ptr, _ptr, _u64, _u64] + [_f32] * 9),

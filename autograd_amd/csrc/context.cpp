@@ -747,6 +747,13 @@ int agrad_stream(agrad_ctx* ctx, void** stream) {
     return AGRAD_OK;
 }
 
+int agrad_buffer_address(agrad_ctx* ctx, uint64_t buffer_id, uint64_t offset, uint64_t nbytes, void** address) {
+    CTX_OR_FAIL(ctx)
+    if (address == nullptr) return set_error(AGRAD_EINVAL, "null out pointer");
+    *address = nullptr;
+    return resolve(ctx, buffer_id, offset, nbytes, "buffer address", address);
+}
+
 int agrad_timer_start(agrad_ctx* ctx) {
     CTX_OR_FAIL(ctx)
     if (int rc = no_capture(ctx, "timer")) return rc;
@@ -1137,6 +1144,43 @@ int agrad_cross_entropy_backward(agrad_ctx* ctx, int dtype, const void* logits, 
                                  uint64_t rows, uint32_t V, uint32_t flags) {
     CTX_OR_FAIL(ctx)
     return launch_ce_bwd(ctx->stream, dtype, logits, labels, dloss, lse, dlogits, rows, V, flags, ctx->err_flag);
+}
+
+int agrad_token_logprobs_forward(agrad_ctx* ctx, int dtype, const void* logits, const int32_t* tokens, float* logp,
+                                 float* entropy, float* lse, int32_t* top_ids, float* top_logp, uint64_t rows, uint32_t V,
+                                 uint64_t ld, uint32_t top, float scale) {
+    CTX_OR_FAIL(ctx)
+    return launch_logprobs_fwd(ctx->stream, dtype, logits, tokens, logp, entropy, lse, top_ids, top_logp, rows, V, ld, top, scale,
+                               ctx->err_flag);
+}
+int agrad_token_logprobs_backward(agrad_ctx* ctx, int dtype, const void* logits, const int32_t* tokens, const float* lse,
+                                  const float* entropy, const float* dlogp, const float* dentropy, void* dlogits,
+                                  uint64_t rows, uint32_t V, uint64_t ld, float scale, uint32_t flags) {
+    CTX_OR_FAIL(ctx)
+    return launch_logprobs_bwd(ctx->stream, dtype, logits, tokens, lse, entropy, dlogp, dentropy, dlogits, rows, V, ld, scale, flags,
+                               ctx->err_flag);
+}
+int agrad_topk_distill_forward(agrad_ctx* ctx, int dtype, const void* logits, const int32_t* teacher_ids,
+                               const float* teacher_values, float* loss, float* stats, uint64_t rows, uint32_t V, uint64_t ld,
+                               uint32_t top, float scale, float teacher_scale, int mode) {
+    CTX_OR_FAIL(ctx)
+    return launch_distill_fwd(ctx->stream, dtype, logits, teacher_ids, teacher_values, loss, stats, rows, V, ld, top, scale,
+                              teacher_scale, mode, ctx->err_flag);
+}
+int agrad_topk_distill_backward(agrad_ctx* ctx, int dtype, const void* logits, const int32_t* teacher_ids,
+                                const float* teacher_values, const float* dloss, const float* stats, void* dlogits,
+                                uint64_t rows, uint32_t V, uint64_t ld, uint32_t top, float scale, float teacher_scale, int mode,
+                                uint32_t flags) {
+    CTX_OR_FAIL(ctx)
+    return launch_distill_bwd(ctx->stream, dtype, logits, teacher_ids, teacher_values, dloss, stats, dlogits, rows, V, ld, top, scale,
+                              teacher_scale, mode, flags, ctx->err_flag);
+}
+int agrad_topk_distill_fused(agrad_ctx* ctx, int dtype, const void* logits, const int32_t* teacher_ids,
+                             const float* teacher_values, float* loss, const float* row_scale, void* dlogits, uint64_t rows,
+                             uint32_t V, uint64_t ld, uint32_t top, float scale, float teacher_scale, float grad_scale, int mode) {
+    CTX_OR_FAIL(ctx)
+    return launch_distill_fused(ctx->stream, dtype, logits, teacher_ids, teacher_values, loss, row_scale, dlogits, rows, V, ld, top,
+                                scale, teacher_scale, grad_scale, mode, ctx->err_flag);
 }
 
 int agrad_adamw8bit_step(agrad_ctx* ctx, int grad_dtype, float* p, const void* g, uint8_t* qm, uint8_t* qv,

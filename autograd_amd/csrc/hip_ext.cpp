@@ -150,6 +150,74 @@ public:
         return out;
     }
 
+    // ---- the operators over logits: (buffer id, byte offset) lists in the order of the C ABI's operands, id 0 for an
+    // operand that is not given; every range is checked against the context's allocations first
+    void token_logprobs_forward(int dtype, const std::vector<uint64_t>& ids, const std::vector<uint64_t>& offs,
+                                uint64_t rows, uint32_t V, uint64_t ld, uint32_t top, float scale) {
+        Operands o(*this, "token_logprobs_forward", ids, offs, 7);
+        const uint64_t list = items(rows, top) * 4;
+        void* x = o.at(0, matrix_bytes(dtype, rows, V, ld));
+        const auto* tokens = static_cast<const int32_t*>(o.at(1, rows * 4));
+        auto* logp = static_cast<float*>(o.at(2, rows * 4));
+        auto* entropy = static_cast<float*>(o.at(3, rows * 4));
+        auto* lse = static_cast<float*>(o.at(4, rows * 4));
+        auto* top_ids = static_cast<int32_t*>(o.at(5, list));
+        auto* top_logp = static_cast<float*>(o.at(6, list));
+        raise_for(agrad_token_logprobs_forward(ctx_, dtype, x, tokens, logp, entropy, lse, top_ids, top_logp, rows, V, ld, top, scale));
+    }
+    void token_logprobs_backward(int dtype, const std::vector<uint64_t>& ids, const std::vector<uint64_t>& offs,
+                                 uint64_t rows, uint32_t V, uint64_t ld, float scale, uint32_t flags) {
+        Operands o(*this, "token_logprobs_backward", ids, offs, 7);
+        const uint64_t matrix = matrix_bytes(dtype, rows, V, ld);
+        void* x = o.at(0, matrix);
+        const auto* tokens = static_cast<const int32_t*>(o.at(1, rows * 4));
+        const auto* lse = static_cast<const float*>(o.at(2, rows * 4));
+        const auto* entropy = static_cast<const float*>(o.at(3, rows * 4));
+        const auto* dlogp = static_cast<const float*>(o.at(4, rows * 4));
+        const auto* dentropy = static_cast<const float*>(o.at(5, rows * 4));
+        void* dx = o.at(6, matrix);
+        raise_for(agrad_token_logprobs_backward(ctx_, dtype, x, tokens, lse, entropy, dlogp, dentropy, dx, rows, V, ld, scale, flags));
+    }
+    void topk_distill_forward(int dtype, const std::vector<uint64_t>& ids, const std::vector<uint64_t>& offs,
+                              uint64_t rows, uint32_t V, uint64_t ld, uint32_t top, float scale, float teacher_scale, int mode) {
+        Operands o(*this, "topk_distill_forward", ids, offs, 5);
+        const uint64_t list = items(rows, top) * 4;
+        void* x = o.at(0, matrix_bytes(dtype, rows, V, ld));
+        const auto* tids = static_cast<const int32_t*>(o.at(1, list));
+        const auto* values = static_cast<const float*>(o.at(2, list));
+        auto* loss = static_cast<float*>(o.at(3, rows * 4));
+        auto* stats = static_cast<float*>(o.at(4, rows * 16));
+        raise_for(agrad_topk_distill_forward(ctx_, dtype, x, tids, values, loss, stats, rows, V, ld, top, scale, teacher_scale, mode));
+    }
+    void topk_distill_backward(int dtype, const std::vector<uint64_t>& ids, const std::vector<uint64_t>& offs,
+                               uint64_t rows, uint32_t V, uint64_t ld, uint32_t top, float scale, float teacher_scale, int mode,
+                               uint32_t flags) {
+        Operands o(*this, "topk_distill_backward", ids, offs, 6);
+        const uint64_t list = items(rows, top) * 4, matrix = matrix_bytes(dtype, rows, V, ld);
+        void* x = o.at(0, matrix);
+        const auto* tids = static_cast<const int32_t*>(o.at(1, list));
+        const auto* values = static_cast<const float*>(o.at(2, list));
+        const auto* dloss = static_cast<const float*>(o.at(3, rows * 4));
+        const auto* stats = static_cast<const float*>(o.at(4, rows * 16));
+        void* dx = o.at(5, matrix);
+        raise_for(agrad_topk_distill_backward(ctx_, dtype, x, tids, values, dloss, stats, dx, rows, V, ld, top, scale, teacher_scale,
+                                              mode, flags));
+    }
+    void topk_distill_fused(int dtype, const std::vector<uint64_t>& ids, const std::vector<uint64_t>& offs,
+                            uint64_t rows, uint32_t V, uint64_t ld, uint32_t top, float scale, float teacher_scale,
+                            float grad_scale, int mode) {
+        Operands o(*this, "topk_distill_fused", ids, offs, 6);
+        const uint64_t list = items(rows, top) * 4, matrix = matrix_bytes(dtype, rows, V, ld);
+        void* x = o.at(0, matrix);
+        const auto* tids = static_cast<const int32_t*>(o.at(1, list));
+        const auto* values = static_cast<const float*>(o.at(2, list));
+        auto* loss = static_cast<float*>(o.at(3, rows * 4));
+        const auto* row_scale = static_cast<const float*>(o.at(4, rows * 4));
+        void* dx = o.at(5, matrix);
+        raise_for(agrad_topk_distill_fused(ctx_, dtype, x, tids, values, loss, row_scale, dx, rows, V, ld, top, scale, teacher_scale,
+                                           grad_scale, mode));
+    }
+
     uint64_t norm_backward_workspace_bytes(uint64_t rows, uint32_t C, int dtype) {
         return agrad_norm_backward_workspace_bytes(rows, C, dtype);
     }
@@ -185,6 +253,32 @@ public:
     uint64_t handle() { return reinterpret_cast<uint64_t>(ctx_); }
 
 private:
+    // a call's operands by (buffer id, offset)
+    struct Operands {
+        HipContext& c;
+        const std::vector<uint64_t>&ids, &offs;
+        Operands(HipContext& ctx, const char* what, const std::vector<uint64_t>& i, const std::vector<uint64_t>& f, size_t n)
+            : c(ctx), ids(i), offs(f) {
+            if (ids.size() != n || offs.size() != n)
+                throw py::value_error(std::string(what) + " expects " + std::to_string(n) + " buffer ids and offsets");
+        }
+        void* at(size_t i, uint64_t nbytes) const {
+            if (ids[i] == 0) return nullptr;
+            void* p = nullptr;
+            raise_for(agrad_buffer_address(c.ctx_, ids[i], offs[i], nbytes, &p));
+            return p;
+        }
+    };
+    static uint64_t items(uint64_t rows, uint64_t each) {
+        if (each != 0 && rows > (1ull << 48) / each) throw py::value_error("operand too large");
+        return rows * each;
+    }
+    // bytes from the first to the last element of [rows, V] with a row stride of ld
+    static uint64_t matrix_bytes(int dtype, uint64_t rows, uint64_t V, uint64_t ld) {
+        if (rows == 0 || V == 0) return 0;
+        return (items(rows - 1, ld) + V) * (dtype == AGRAD_BF16 ? 2 : 4);
+    }
+
     agrad_ctx* ctx_ = nullptr;
 };
 
@@ -226,6 +320,11 @@ PYBIND11_MODULE(hip_ext, m) {
         .def("copy_from_host", &HipContext::copy_from_host)
         .def("copy_to_host", &HipContext::copy_to_host, py::arg("buffer_id"), py::arg("offset"),
              py::arg("shape"), py::arg("dtype") = "float32")
+        .def("token_logprobs_forward", &HipContext::token_logprobs_forward)
+        .def("token_logprobs_backward", &HipContext::token_logprobs_backward)
+        .def("topk_distill_forward", &HipContext::topk_distill_forward)
+        .def("topk_distill_backward", &HipContext::topk_distill_backward)
+        .def("topk_distill_fused", &HipContext::topk_distill_fused)
         .def("norm_backward_workspace_bytes", &HipContext::norm_backward_workspace_bytes)
         .def("embedding_backward_workspace_bytes", &HipContext::embedding_backward_workspace_bytes)
         .def("broadcast_grad_workspace_bytes", &HipContext::broadcast_grad_workspace_bytes)

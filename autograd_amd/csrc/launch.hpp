@@ -181,4 +181,22 @@ int launch_ce_fused(hipStream_t s, int dtype, void* logits, const int32_t* targe
 // bytes of team_scratch: arrival counters and (max, sum) pairs of the workgroup teams that share long rows
 uint64_t ce_fused_scratch_bytes();
 
+// logprobs.hip: log probabilities of given tokens, entropy, alternatives (any output but one may be null)
+int logits_check(const char* what, int dtype, const void* x, const void* dx, uint64_t rows, uint32_t V, uint64_t ld, float scale);
+int launch_logprobs_fwd(hipStream_t s, int dtype, const void* logits, const int32_t* tokens, float* logp, float* entropy,
+                        float* lse, int32_t* top_ids, float* top_logp, uint64_t rows, uint32_t V, uint64_t ld, uint32_t top,
+                        float scale, int* err_flag);
+int launch_logprobs_bwd(hipStream_t s, int dtype, const void* logits, const int32_t* tokens, const float* lse,
+                        const float* entropy, const float* dlogp, const float* dentropy, void* dlogits, uint64_t rows,
+                        uint32_t V, uint64_t ld, float scale, uint32_t flags, int* err_flag);
+// distill.hip: the divergence from a teacher's top logits; stats [rows, 4] carries what the backward call needs
+int launch_distill_fwd(hipStream_t s, int dtype, const void* logits, const int32_t* ids, const float* values, float* loss, float* stats,
+                       uint64_t rows, uint32_t V, uint64_t ld, uint32_t top, float scale, float teacher_scale, int mode, int* err_flag);
+int launch_distill_bwd(hipStream_t s, int dtype, const void* logits, const int32_t* ids, const float* values, const float* dloss,
+                       const float* stats, void* dlogits, uint64_t rows, uint32_t V, uint64_t ld, uint32_t top, float scale,
+                       float teacher_scale, int mode, uint32_t flags, int* err_flag);
+int launch_distill_fused(hipStream_t s, int dtype, const void* logits, const int32_t* ids, const float* values, float* loss,
+                         const float* row_scale, void* dlogits, uint64_t rows, uint32_t V, uint64_t ld, uint32_t top, float scale,
+                         float teacher_scale, float grad_scale, int mode, int* err_flag);
+
 }  // namespace agrad

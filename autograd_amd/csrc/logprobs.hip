@@ -1,0 +1,328 @@
+// Log probabilities of given tokens, with the entropy of each row's distribution and its most likely classes.
+//
+//   z = scale * x,  lse = log sum exp(z),  p = exp(z - lse)
+//   forward   logp[r] = z[r, token] - lse,  entropy[r] = -sum p log p,  the `top` classes of largest x (equal logits: the
+//             lower index first) with their log probabilities
+//   backward  dx[v] (+)= scale * (g [v == token] - p[v] (g + h (log p[v] + entropy))),  g = dlogp, h = dentropy
+//
+// Both are streams over [rows, V]: the forward pass reads the logits once, the backward pass reads them once and
+// writes the gradient once; HBM bounds both.
+#include "launch.hpp"
+#include "row_softmax.hpp"
+
+#include <cmath>
+
+namespace agrad {
+
+namespace {
+
+constexpr int kLpBlock = 256;
+constexpr int kLpUnroll = 4;         // vectors a thread keeps in flight
+constexpr int kCandidates = 1024;    // candidates of a row's alternatives that LDS holds
+
+struct LpArgs {
+    const int32_t* tokens; float* logp; float* entropy; float* lse; int32_t* top_ids; float* top_logp;
+    uint64_t ld; uint32_t V, top; float scale, c;
+    int* err_flag;
+};
+
+// ---- alternatives ------------------------------------------------------------------------------------
+// A class is a 64-bit key: the logit as an integer of the same order above, the complement of the index below; keys
+// are distinct and descend in the order in which alternatives are given.  0 is no class.
+__device__ __forceinline__ uint64_t class_key(float x, uint32_t index) {
+    const uint32_t u = __float_as_uint(x + 0.0f);                   // (-0 ties with 0)
+    const uint32_t ordered = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    return x > -INFINITY ? ((uint64_t)ordered << 32) | (0xffffffffu - index) : 0ull;       // -inf and NaN: no alternative
+}
+__device__ __forceinline__ float key_logit(uint64_t key) {
+    const uint32_t o = (uint32_t)(key >> 32);
+    return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+}
+__device__ __forceinline__ uint32_t key_index(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
+
+struct Candidates {
+    uint64_t key[kCandidates];
+    uint32_t count;
+};
+
+// Appends the keys of the lanes that have one.  The places depend on the order in which waves arrive, the set does not.
+__device__ __forceinline__ void append(Candidates& q, bool has, uint64_t key) {
+    const uint64_t lanes = __ballot(has);
+    if (lanes == 0) return;
+    const uint32_t lane = threadIdx.x % kWave, first = (uint32_t)__builtin_ctzll(lanes);
+    uint32_t at = 0;
+    if (lane == first) at = atomicAdd(&q.count, (uint32_t)__popcll(lanes));
+    at = (uint32_t)__shfl((int)at, (int)first) + (uint32_t)__popcll(lanes & ((1ull << lane) - 1));
+    if (has && at < (uint32_t)kCandidates) q.key[at] = key;
+}
+
+// Keeps the largest `top` of the candidates, in descending order at the front: a key's place is the number of larger
+// keys, counted.  All threads of the workgroup call it after a barrier; it ends with one.
+template <int BLOCK>
+__device__ __forceinline__ void prune(Candidates& q, uint32_t top) {
+    constexpr int EACH = kCandidates / BLOCK;
+    const uint32_t n = q.count < (uint32_t)kCandidates ? q.count : (uint32_t)kCandidates;
+    uint64_t mine[EACH];
+    uint32_t larger[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const uint32_t at = threadIdx.x + (uint32_t)i * BLOCK;
+        mine[i] = at < n ? q.key[at] : 0ull;
+        larger[i] = 0;
+    }
+    for (uint32_t j = 0; j < n; ++j) {
+        const uint64_t other = q.key[j];
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) larger[i] += other > mine[i] ? 1u : 0u;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+        if (mine[i] != 0ull && larger[i] < top) q.key[larger[i]] = mine[i];
+    if (threadIdx.x == 0) q.count = n < top ? n : top;
+    __syncthreads();
+}
+
+// the alternatives of a whole row, one element a thread and step
+template <typename T, int BLOCK>
+__device__ __forceinline__ void row_top(const T* base, uint32_t V, uint32_t top, Candidates& q) {
+    if (threadIdx.x == 0) q.count = 0;
+    __syncthreads();
+    uint64_t floor_key = 0;
+    for (uint32_t e0 = 0; e0 < V; e0 += BLOCK) {
+        const uint32_t e = e0 + threadIdx.x;
+        float x[1];
+        VecIO<T, 1>::load(base + (e < V ? e : 0u), x);
+        const uint64_t key = class_key(x[0], e);
+        append(q, e < V && key > floor_key, key);
+        __syncthreads();
+        const bool full = q.count > (uint32_t)(kCandidates - BLOCK);
+        __syncthreads();
+        if (full) {
+            prune<BLOCK>(q, top);
+            floor_key = q.count == top ? q.key[top - 1] : 0ull;
+            __syncthreads();
+        }
+    }
+    prune<BLOCK>(q, top);
+}
+
+// ---- forward -----------------------------------------------------------------------------------------
+template <typename T, int VEC, bool ENT>
+__device__ __forceinline__ RowStat row_stat(const T* base, uint32_t V, float c, RowStat* lds) {
+    const RowParts<T, VEC> parts(base, V);
+    RowStat a = empty_stat();
+    if (threadIdx.x < parts.extra) {
+        float x[1];
+        VecIO<T, 1>::load(base + parts.extra_at(threadIdx.x), x);
+        absorb_stat<ENT, 1>(a, x, c);
+    }
+    const T* body = base + parts.head;
+    for (uint32_t i0 = threadIdx.x; i0 < parts.nvec; i0 += kLpBlock * kLpUnroll) {
+        float v[kLpUnroll][VEC];
+#pragma unroll
+        for (int u = 0; u < kLpUnroll; ++u) {
+            const uint32_t i = i0 + u * kLpBlock;
+            if (i < parts.nvec) VecIO<T, VEC>::load(body + (uint64_t)i * VEC, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < kLpUnroll; ++u)
+            if (i0 + u * kLpBlock < parts.nvec) absorb_stat<ENT, VEC>(a, v[u], c);
+    }
+    return block_stat<kLpBlock, ENT>(a, c, lds);
+}
+
+template <typename T, int VEC, bool ENT>
+__global__ void __launch_bounds__(kLpBlock)
+logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
+    __shared__ RowStat lds[kLpBlock / kWave];
+    __shared__ Candidates found;
+    const uint64_t row = blockIdx.x;
+    const T* base = x + row * a.ld;
+    const RowStat t = row_stat<T, VEC, ENT>(base, a.V, a.c, lds);
+    const bool empty = t.m == -INFINITY && t.s == 0.0f;
+    const float log_s = logf(t.s);                                // -inf for an empty row
+    if (threadIdx.x == 0) {
+        if (a.lse != nullptr) a.lse[row] = empty ? -INFINITY : t.m * a.scale + log_s;
+        if (ENT) a.entropy[row] = empty ? 0.0f : log_s - kLn2 * (t.d / t.s);
+        if (a.tokens != nullptr) {
+            const int32_t token = a.tokens[row];
+            float lp = 0.0f;
+            if (token >= 0 && (uint32_t)token < a.V) {
+                float at[1];
+                VecIO<T, 1>::load(base + token, at);
+                if (!empty) lp = (at[0] - t.m) * a.scale - log_s;
+            } else if (token != -1) {
+                *a.err_flag = 1;
+            }
+            a.logp[row] = lp;
+        }
+    }
+    if (a.top != 0) {
+        row_top<T, kLpBlock>(base, a.V, a.top, found);
+        if (threadIdx.x < a.top) {
+            const bool there = threadIdx.x < found.count;
+            const uint64_t key = there ? found.key[threadIdx.x] : 0ull;
+            const uint64_t to = row * a.top + threadIdx.x;
+            a.top_ids[to] = there ? (int32_t)key_index(key) : -1;
+            a.top_logp[to] = there ? (key_logit(key) - t.m) * a.scale - log_s : -INFINITY;
+        }
+    }
+}
+
+// ---- backward ----------------------------------------------------------------------------------------
+// One vector a thread, a workgroup a chunk of a row (the most independent waves: a stream of one read and one write runs
+// best that way here).  With l = log p:  dx = scale * (g [v == token] - p (g + h entropy + h l)).
+struct LpBwdArgs {
+    const int32_t* tokens; const float* lse; const float* entropy; const float* dlogp; const float* dentropy;
+    uint64_t ld; uint32_t V; float scale; uint32_t accumulate;
+    int* err_flag;
+};
+
+struct LpRow {
+    float scale, lse, a, h, g;          // a = scale * (g + h * entropy), h, g already multiplied by scale
+    uint32_t token;
+};
+
+__device__ __forceinline__ float lp_grad(float x, const LpRow& r, uint32_t e) {
+    const float l = x * r.scale - r.lse;
+    const float p = __builtin_amdgcn_exp2f(l * kLog2eHi);
+    float d = -p * __builtin_fmaf(r.h, fmaxf(l, -200.0f), r.a);
+    if (e == r.token) d = d + r.g;
+    return d;
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ void lp_store(T* to, float (&d)[VEC], uint32_t accumulate) {
+    if (accumulate) {
+        float old[VEC];
+        VecIO<T, VEC>::load(to, old);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) d[k] = old[k] + d[k];
+    }
+    VecIO<T, VEC>::store(to, d);
+}
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kLpBlock)
+logprobs_bwd_kernel(const T* x, T* dx, const LpBwdArgs a, const FastDiv32 chunks) {
+    const uint32_t row = chunks.div(blockIdx.x), chunk = blockIdx.x - row * chunks.d;
+    const T* base = x + (uint64_t)row * a.ld;
+    T* out = dx + (uint64_t)row * a.ld;
+    LpRow r;
+    const int32_t token = a.tokens != nullptr ? a.tokens[row] : -1;
+    const bool asked = token >= 0 && (uint32_t)token < a.V;
+    if (!asked && token != -1 && chunk == 0 && threadIdx.x == 0) *a.err_flag = 1;
+    r.scale = a.scale;
+    r.lse = a.lse[row];
+    const bool empty = r.lse == -INFINITY;
+    r.token = asked && !empty ? (uint32_t)token : 0xffffffffu;
+    r.g = asked && a.dlogp != nullptr ? a.scale * a.dlogp[row] : 0.0f;
+    r.h = a.dentropy != nullptr ? a.scale * a.dentropy[row] : 0.0f;
+    r.a = a.dentropy != nullptr ? __builtin_fmaf(r.h, a.entropy[row], r.g) : r.g;
+    if (empty) { r.lse = INFINITY; r.a = r.h = r.g = 0.0f; }
+    const RowParts<T, VEC> parts(base, a.V);
+    if (chunk == 0 && threadIdx.x < parts.extra) {
+        const uint32_t e = parts.extra_at(threadIdx.x);
+        float v[1];
+        VecIO<T, 1>::load(base + e, v);
+        v[0] = lp_grad(v[0], r, e);
+        lp_store<T, 1>(out + e, v, a.accumulate);
+    }
+    const uint32_t i = chunk * kLpBlock + threadIdx.x;
+    if (i >= parts.nvec) return;
+    const uint32_t first = parts.head + i * VEC;
+    float v[VEC];
+    VecIO<T, VEC>::load(base + first, v);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) v[k] = lp_grad(v[k], r, first + k);
+    lp_store<T, VEC>(out + first, v, a.accumulate);
+}
+
+template <typename T>
+int lp_fwd_typed(hipStream_t s, const T* x, const LpArgs& a, uint64_t rows) {
+    constexpr int WIDE = WideVec<T>::value;
+    const bool wide = a.V >= 4 * WIDE;
+    const dim3 grid((uint32_t)rows), block(kLpBlock);
+    if (wide && a.entropy) hipLaunchKernelGGL((logprobs_fwd_kernel<T, WIDE, true>), grid, block, 0, s, x, a);
+    else if (wide) hipLaunchKernelGGL((logprobs_fwd_kernel<T, WIDE, false>), grid, block, 0, s, x, a);
+    else if (a.entropy) hipLaunchKernelGGL((logprobs_fwd_kernel<T, 1, true>), grid, block, 0, s, x, a);
+    else hipLaunchKernelGGL((logprobs_fwd_kernel<T, 1, false>), grid, block, 0, s, x, a);
+    return check_hip(hipGetLastError(), "token log probabilities launch");
+}
+
+template <typename T>
+int lp_bwd_typed(hipStream_t s, const T* x, T* dx, LpBwdArgs a, uint64_t rows) {
+    constexpr int WIDE = WideVec<T>::value;
+    // rows are realigned by their first elements, which needs both tensors at one offset within 16 bytes
+    const bool wide = a.V >= 4 * WIDE && ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15u) == 0;
+    const uint32_t vec = wide ? WIDE : 1;
+    const uint32_t chunks = (a.V / vec + kLpBlock - 1) / kLpBlock;
+    uint64_t max_rows = 0x00ffffffull / chunks;                  // workgroups of a launch: 2^32 threads
+    if (max_rows == 0) max_rows = 1;
+    for (uint64_t r0 = 0; r0 < rows; r0 += max_rows) {
+        const uint64_t n = rows - r0 < max_rows ? rows - r0 : max_rows;
+        LpBwdArgs b = a;
+        if (b.tokens) b.tokens += r0;
+        b.lse += r0;
+        if (b.entropy) b.entropy += r0;
+        if (b.dlogp) b.dlogp += r0;
+        if (b.dentropy) b.dentropy += r0;
+        const dim3 grid((uint32_t)(n * chunks)), block(kLpBlock);
+        if (wide) hipLaunchKernelGGL((logprobs_bwd_kernel<T, WIDE>), grid, block, 0, s, x + r0 * a.ld, dx + r0 * a.ld, b, FastDiv32(chunks));
+        else hipLaunchKernelGGL((logprobs_bwd_kernel<T, 1>), grid, block, 0, s, x + r0 * a.ld, dx + r0 * a.ld, b, FastDiv32(chunks));
+    }
+    return check_hip(hipGetLastError(), "token log probabilities backward launch");
+}
+
+}  // namespace
+
+int logits_check(const char* what, int dtype, const void* x, const void* dx, uint64_t rows, uint32_t V, uint64_t ld, float scale) {
+    if (dtype != AGRAD_F32 && dtype != AGRAD_BF16) return set_error(AGRAD_EINVAL, "%s: unknown dtype %d", what, dtype);
+    if (V == 0 || V >= 0x7fffffffu) return set_error(AGRAD_EINVAL, "%s: %u classes", what, V);
+    if (ld < V || ld > 0xffffffffull) return set_error(AGRAD_EINVAL, "%s: row stride %llu for %u classes", what, (unsigned long long)ld, V);
+    // (a launch has fewer than 2^32 threads; the largest workgroup here has 1024)
+    if (rows >= 0x00400000ull) return set_error(AGRAD_EINVAL, "%s: at most %u rows a call", what, 0x003fffffu);
+    if (!(scale > 0.0f) || !std::isfinite(scale)) return set_error(AGRAD_EINVAL, "%s: the scale must be positive and finite", what);
+    const uintptr_t es = dtype_size(dtype);
+    if (reinterpret_cast<uintptr_t>(x) % es || reinterpret_cast<uintptr_t>(dx) % es)
+        return set_error(AGRAD_EINVAL, "%s: logits or gradient not aligned to their elements", what);
+    return AGRAD_OK;
+}
+
+int launch_logprobs_fwd(hipStream_t s, int dtype, const void* logits, const int32_t* tokens, float* logp, float* entropy,
+                        float* lse, int32_t* top_ids, float* top_logp, uint64_t rows, uint32_t V, uint64_t ld, uint32_t top,
+                        float scale, int* err_flag) {
+    const char* what = "token log probabilities";
+    if (int rc = logits_check(what, dtype, logits, nullptr, rows, V, ld, scale)) return rc;
+    if (top > AGRAD_MAX_TOP) return set_error(AGRAD_EINVAL, "%s: at most %u alternatives, got %u", what, AGRAD_MAX_TOP, top);
+    if (rows == 0) return AGRAD_OK;
+    if (logits == nullptr) return set_error(AGRAD_EINVAL, "%s: null logits", what);
+    if ((tokens != nullptr) != (logp != nullptr)) return set_error(AGRAD_EINVAL, "%s: tokens and logp go together", what);
+    if ((top != 0) != (top_ids != nullptr) || (top != 0) != (top_logp != nullptr))
+        return set_error(AGRAD_EINVAL, "%s: top_ids and top_logp are given exactly when top > 0", what);
+    if (logp == nullptr && entropy == nullptr && lse == nullptr && top == 0) return set_error(AGRAD_EINVAL, "%s: nothing to compute", what);
+    const float c = (float)((double)scale * 1.4426950408889634);
+    const LpArgs a{tokens, logp, entropy, lse, top_ids, top_logp, ld, V, top, scale, c, err_flag};
+    if (dtype == AGRAD_F32) return lp_fwd_typed<float>(s, (const float*)logits, a, rows);
+    return lp_fwd_typed<bf16_t>(s, (const bf16_t*)logits, a, rows);
+}
+
+int launch_logprobs_bwd(hipStream_t s, int dtype, const void* logits, const int32_t* tokens, const float* lse,
+                        const float* entropy, const float* dlogp, const float* dentropy, void* dlogits, uint64_t rows,
+                        uint32_t V, uint64_t ld, float scale, uint32_t flags, int* err_flag) {
+    const char* what = "token log probabilities backward";
+    if (int rc = logits_check(what, dtype, logits, dlogits, rows, V, ld, scale)) return rc;
+    if (flags & ~(uint32_t)AGRAD_ACC_INPUT_GRAD) return set_error(AGRAD_EINVAL, "%s: unknown flag bits 0x%x", what, flags);
+    if (rows == 0) return AGRAD_OK;
+    if (logits == nullptr || dlogits == nullptr || lse == nullptr) return set_error(AGRAD_EINVAL, "%s: null operand", what);
+    if (dlogp == nullptr && dentropy == nullptr) return set_error(AGRAD_EINVAL, "%s: neither dlogp nor dentropy", what);
+    if (dlogp != nullptr && tokens == nullptr) return set_error(AGRAD_EINVAL, "%s: dlogp without tokens", what);
+    if (dentropy != nullptr && entropy == nullptr) return set_error(AGRAD_EINVAL, "%s: dentropy without the entropy", what);
+    const LpBwdArgs a{dlogp != nullptr ? tokens : nullptr, lse, entropy, dlogp, dentropy, ld, V, scale,
+                      (flags & AGRAD_ACC_INPUT_GRAD) ? 1u : 0u, err_flag};
+    if (dtype == AGRAD_F32) return lp_bwd_typed<float>(s, (const float*)logits, (float*)dlogits, a, rows);
+    return lp_bwd_typed<bf16_t>(s, (const bf16_t*)logits, (bf16_t*)dlogits, a, rows);
+}
+
+}  // namespace agrad

@@ -14,11 +14,12 @@ new.
 from __future__ import annotations
 
 from abc import ABC, abstractmethod
+from typing import NamedTuple
 
 import numpy as np
 
 from .tensor import Tensor
-from .utils import broadcast_shape, mul_bcast_kind
+from .utils import broadcast_shape, is_bf16, mul_bcast_kind
 
 
 class OpNode:
@@ -515,6 +516,132 @@ class CrossEntropyLossOp(Op):
         node = OpNode(op=self, inputs=(logits, labels), outputs=(loss, lse))
         loss.op = node
         lse.op = node
+        return loss
+
+    def save_for_backward(self, inputs, outputs):
+        return list(inputs) + [outputs[1]]
+
+    def fully_written_inputs(self, inputs, outputs):
+        return [0]
+
+
+def _inverse_temperature(value, what):
+    value = float(value)
+    if not (0.0 < value < float("inf")):
+        raise ValueError(f"{what} must be positive and finite, got {value}")
+    return value
+
+
+MAX_TOP = 128     # classes a row that the operators below take or give (AGRAD_MAX_TOP)
+
+
+class TokenLogprobs(NamedTuple):
+    """what TokenLogprobsOp returns; None for what was not asked for"""
+    logp: Tensor
+    entropy: Tensor | None
+    top_ids: Tensor | None
+    top_logp: Tensor | None
+
+
+class TokenLogprobsOp(Op):
+    """Log probabilities of given tokens: logp[b, t] = log softmax(scale * logits[b, t, :])[tokens[b, t]], fp32 like
+    the entropy of the row's distribution and the `top` most likely classes (int32 ids, equal logits by ascending
+    id) with their log probabilities.  Token -1 is a position without a token: logp 0, no gradient of it.  logp and
+    entropy carry gradients, the alternatives do not.  Masked classes (-inf) are no alternatives: a slot that finds
+    no class holds id -1 and -inf.
+
+    The node keeps the row's log-sum-exp as a further output for the backward kernel.  An output lives in the arena
+    as any activation does: read one back after a forward pass whose last node this is."""
+    op_name = "TokenLogprobs"
+
+    def __init__(self, top=0, entropy=False, scale=1.0):
+        if not 0 <= int(top) <= MAX_TOP:
+            raise ValueError(f"TokenLogprobs gives up to {MAX_TOP} alternatives, asked for {top}")
+        self.top = int(top)
+        self.entropy = bool(entropy)
+        self.scale = _inverse_temperature(scale, "TokenLogprobs: scale")
+
+    def infer_shape(self, logits, tokens):
+        if logits.ndim < 1 or logits.shape[:-1] != tokens.shape:
+            raise ValueError(f"TokenLogprobs: logits {logits.shape} and tokens {tokens.shape}")
+        if is_bf16(tokens.dtype) or np.dtype(tokens.dtype) not in INT_DTYPES:
+            raise ValueError(f"TokenLogprobs: tokens are int32, got {tokens.dtype}")
+        return tokens.shape
+
+    def __call__(self, logits, tokens):
+        self.require_contiguous((logits, tokens))
+        shape = self.infer_shape(logits, tokens)
+
+        def out(shape, dtype, grad):
+            return Tensor(shape=shape, dtype=dtype, requires_grad=grad, device=logits.device)
+
+        logp, lse = out(shape, np.float32, logits.requires_grad), out(shape, np.float32, False)
+        entropy = out(shape, np.float32, logits.requires_grad) if self.entropy else None
+        top_ids = out(shape + (self.top,), np.int32, False) if self.top else None
+        top_logp = out(shape + (self.top,), np.float32, False) if self.top else None
+        outputs = tuple(t for t in (logp, lse, entropy, top_ids, top_logp) if t is not None)
+        node = OpNode(op=self, inputs=(logits, tokens), outputs=outputs)
+        for t in outputs:
+            t.op = node
+        return TokenLogprobs(logp, entropy, top_ids, top_logp)
+
+    def split(self, outputs):
+        """(logp, lse, entropy, top_ids, top_logp) of a node's outputs, None for what it does not have"""
+        rest = list(outputs[2:])
+        entropy = rest.pop(0) if self.entropy else None
+        top_ids, top_logp = rest if self.top else (None, None)
+        return outputs[0], outputs[1], entropy, top_ids, top_logp
+
+    def save_for_backward(self, inputs, outputs):
+        return list(inputs) + list(outputs[1:3 if self.entropy else 2])
+
+    def fully_written_inputs(self, inputs, outputs):
+        return [0]
+
+
+class TopKDistillOp(Op):
+    """loss[b, t] = KL(q || softmax(scale * logits[b, t, :])), fp32, of a teacher's q that is known by its top classes:
+    teacher_ids [..., K] int32 (-1: an unused slot) and teacher_values [..., K] fp32.
+
+      tail=False   q = softmax(teacher_scale * teacher_values) over the row's used slots
+      tail=True    the values are log probabilities (TokenLogprobs.top_logp); what they leave belongs to all other
+                   classes together
+
+    A row without used slots has loss 0 and a zero gradient.  The teacher's side carries no gradient.  The node's second
+    output holds what the backward kernel needs of each row."""
+    op_name = "TopKDistill"
+
+    def __init__(self, tail=False, scale=1.0, teacher_scale=1.0):
+        self.tail = bool(tail)
+        self.scale = _inverse_temperature(scale, "TopKDistill: scale")
+        self.teacher_scale = _inverse_temperature(teacher_scale, "TopKDistill: teacher_scale")
+        if self.tail and self.teacher_scale != 1.0:
+            raise ValueError("TopKDistill: log probabilities with a tail are taken as they are (teacher_scale 1)")
+
+    def infer_shape(self, logits, teacher_ids, teacher_values):
+        if (logits.ndim < 1 or teacher_ids.shape != teacher_values.shape or teacher_ids.ndim != logits.ndim
+                or teacher_ids.shape[:-1] != logits.shape[:-1]):
+            raise ValueError(f"TopKDistill: logits {logits.shape}, teacher ids {teacher_ids.shape} and values "
+                             f"{teacher_values.shape}")
+        if not 1 <= teacher_ids.shape[-1] <= MAX_TOP:
+            raise ValueError(f"TopKDistill takes 1 to {MAX_TOP} classes a row, got {teacher_ids.shape[-1]}")
+        if is_bf16(teacher_ids.dtype) or np.dtype(teacher_ids.dtype) not in INT_DTYPES:
+            raise ValueError(f"TopKDistill: teacher ids are int32, got {teacher_ids.dtype}")
+        if is_bf16(teacher_values.dtype) or np.dtype(teacher_values.dtype) != np.dtype(np.float32):
+            raise ValueError(f"TopKDistill: teacher values are fp32, got {teacher_values.dtype}")
+        if teacher_values.requires_grad:
+            raise ValueError("TopKDistill: the teacher's values carry no gradient (requires_grad=False)")
+        return logits.shape[:-1]
+
+    def __call__(self, logits, teacher_ids, teacher_values):
+        inputs = (logits, teacher_ids, teacher_values)
+        self.require_contiguous(inputs)
+        shape = self.infer_shape(*inputs)
+        loss = Tensor(shape=shape, dtype=np.float32, requires_grad=logits.requires_grad, device=logits.device)
+        stats = Tensor(shape=shape + (4,), dtype=np.float32, requires_grad=False, device=logits.device)
+        node = OpNode(op=self, inputs=inputs, outputs=(loss, stats))
+        loss.op = node
+        stats.op = node
         return loss
 
     def save_for_backward(self, inputs, outputs):

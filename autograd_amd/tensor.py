@@ -115,6 +115,17 @@ class Tensor:
         from .op import CrossEntropyLossOp
         return CrossEntropyLossOp(dim)(self, labels)
 
+    # -- what logits say about given tokens, and learning from another model's top logits ----
+    def token_logprobs(self, tokens, top=0, entropy=False, scale=1.0):
+        """TokenLogprobs(logp, entropy, top_ids, top_logp) of softmax(scale * self) over the last axis"""
+        from .op import TokenLogprobsOp
+        return TokenLogprobsOp(top=top, entropy=entropy, scale=scale)(self, tokens)
+
+    def distill_topk(self, teacher_ids, teacher_values, tail=False, scale=1.0, teacher_scale=1.0):
+        """KL divergence of softmax(scale * self) from a teacher's top classes, per row"""
+        from .op import TopKDistillOp
+        return TopKDistillOp(tail=tail, scale=scale, teacher_scale=teacher_scale)(self, teacher_ids, teacher_values)
+
     # -- ops the reference only has inside its fused kernels ----------------------
     def rms_norm(self, gamma=None, eps=1e-6):
         from .op import RMSNormOp

@@ -127,6 +127,11 @@ int agrad_graph_end(agrad_ctx* ctx, uint64_t* graph_id);
 int agrad_graph_launch(agrad_ctx* ctx, uint64_t graph_id);
 int agrad_graph_destroy(agrad_ctx* ctx, uint64_t graph_id);
 
+/* The device address of (buffer_id, offset), after the check that agrad_dispatch makes of every operand: the
+ * `nbytes` from there lie inside one allocation of this context.  For callers that hold buffer ids and call the
+ * typed entry points below. */
+int agrad_buffer_address(agrad_ctx* ctx, uint64_t buffer_id, uint64_t offset, uint64_t nbytes, void** address);
+
 /* ---- typed entry points (device addresses, already offset) ----------------
  * `dtype` is the storage type of activations / gradients / embedding tables;
  * gamma, beta, dgamma, dbeta, cos, sin are always fp32; ids are int32.       */
@@ -486,6 +491,72 @@ int agrad_cross_entropy_fused(agrad_ctx* ctx, int dtype, void* logits, const int
  * (0 = the default, about a second).  No counterpart in the reference; for callers that want a
  * tighter bound on a launch's worst case, and for the test of the give-up path. */
 int agrad_set_team_wait_polls(agrad_ctx* ctx, uint32_t polls);
+
+/* ---- what a model's logits say about given tokens, and learning from another model's -------------
+ * Both operators take logits x[rows, V] with a row stride of ld >= V elements (a vocabulary padded to a
+ * multiple of 64 has ld > V; the columns [V, ld) are neither read nor written), fp32 or bf16, and a
+ * positive finite `scale`, the inverse temperature: z = scale * x, p = softmax(z).  At most 2^22 - 1 rows
+ * a call.  Neither has a counterpart in the reference. */
+
+/* Log probabilities of given tokens.  Per row, with lse = log sum_v exp(z[v]):
+ *   logp     = z[token] - lse                        (tokens and logp are given together or not at all)
+ *   entropy  = -sum_v p[v] log p[v]
+ *   top_ids, top_logp [rows, top]: the `top` <= AGRAD_MAX_TOP classes of the largest logits, descending,
+ *              equal logits by ascending index, and their z - lse (top = 0: none; both pointers NULL)
+ * Each output may be NULL, not all of them.  token -1: no token, logp 0; any other token outside [0, V) sets
+ * the deferred index error (agrad_end_pass / agrad_synchronize) and gives 0.  A class at -inf (a mask) has
+ * probability 0 and is no alternative: slots that find no class get id -1 and -inf.  A row with all classes at
+ * -inf has logp 0, entropy 0, lse -inf and no alternatives.  NaN or +inf in a row: its logp, entropy, lse and
+ * top_logp are NaN (slots without a class stay -inf), its top_ids the order of what is not NaN. */
+#define AGRAD_MAX_TOP 128
+int agrad_token_logprobs_forward(agrad_ctx* ctx, int dtype, const void* logits, const int32_t* tokens,
+                                 float* logp, float* entropy, float* lse, int32_t* top_ids, float* top_logp,
+                                 uint64_t rows, uint32_t V, uint64_t ld, uint32_t top, float scale);
+/* dlogits[v] (+)= scale * (dlogp ([v == token] - p[v]) - dentropy p[v] (log p[v] + entropy)) with the lse and
+ * entropy of the forward call.  dlogp or dentropy may be NULL (0), and with dlogp tokens, with dentropy entropy.
+ * A row without a token takes no dlogp; a row of -inf gets zeros.  dlogits has the logits' stride and may be the
+ * logits (in place).  The alternatives carry no gradient.  AGRAD_ACC_INPUT_GRAD accumulates. */
+int agrad_token_logprobs_backward(agrad_ctx* ctx, int dtype, const void* logits, const int32_t* tokens,
+                                  const float* lse, const float* entropy, const float* dlogp,
+                                  const float* dentropy, void* dlogits,
+                                  uint64_t rows, uint32_t V, uint64_t ld, float scale, uint32_t flags);
+
+/* Distillation from a teacher's top logits: loss[r] = KL(q || p) of the student's p, where q is known by
+ * `top` <= AGRAD_MAX_TOP classes a row (teacher_ids, int32; -1: an unused slot) and values (fp32):
+ *   AGRAD_DISTILL_RENORM  q = softmax(teacher_scale * values) over the row's used slots:
+ *                         loss = sum_k q_k (log q_k - log p[id_k])
+ *   AGRAD_DISTILL_TAIL    values are log probabilities (what agrad_token_logprobs_forward returns), q_k =
+ *                         exp(value), and the mass they leave, q_rest = max(0, 1 - sum q), stands against the
+ *                         student's on all other classes, p_rest:
+ *                         loss = sum_k q_k (log q_k - log p[id_k]) + q_rest (log q_rest - log p_rest),
+ *                         without the last term if q_rest is 0 or no class outside the ids is above -inf.
+ *                         teacher_scale must be 1.
+ * The gradient is scale * (p[v] W - sum of q_k with id_k = v) for the classes among the ids and
+ * scale * p[v] (W - q_rest / p_rest) for the others, W = sum q + q_rest (RENORM: q_rest = 0).  An id that a row
+ * holds twice counts with both its values, its class once.  An id outside [-1, V) sets the deferred index error
+ * and counts as unused.  A value of -inf is a slot of probability 0.  A row without used slots, or whose logits are
+ * all -inf, has loss 0 and a zero gradient; a class at -inf that the teacher gives mass to makes the loss +inf (its
+ * gradient is finite); NaN or +inf makes a row NaN.
+ *   forward   loss, and stats[rows, 4], fp32, for the backward call (may be NULL): the lse of z (-inf: no
+ *             gradient), the lse of the teacher's side (RENORM) or of z outside the ids (TAIL), W, and the factor
+ *             of the classes outside the ids: W, or W p_rest - q_rest
+ *   backward  dlogits (+)= the gradient * dloss[r]
+ *   fused     loss (may be NULL) and dlogits = the gradient * (row_scale[r], or grad_scale if row_scale is NULL)
+ *             in one launch that reads the logits once where a row fits a workgroup's registers
+ * dlogits has the logits' stride and may be the logits (in place). */
+enum { AGRAD_DISTILL_RENORM = 0, AGRAD_DISTILL_TAIL = 1 };
+int agrad_topk_distill_forward(agrad_ctx* ctx, int dtype, const void* logits, const int32_t* teacher_ids,
+                               const float* teacher_values, float* loss, float* stats,
+                               uint64_t rows, uint32_t V, uint64_t ld, uint32_t top,
+                               float scale, float teacher_scale, int mode);
+int agrad_topk_distill_backward(agrad_ctx* ctx, int dtype, const void* logits, const int32_t* teacher_ids,
+                                const float* teacher_values, const float* dloss, const float* stats, void* dlogits,
+                                uint64_t rows, uint32_t V, uint64_t ld, uint32_t top,
+                                float scale, float teacher_scale, int mode, uint32_t flags);
+int agrad_topk_distill_fused(agrad_ctx* ctx, int dtype, const void* logits, const int32_t* teacher_ids,
+                             const float* teacher_values, float* loss, const float* row_scale, void* dlogits,
+                             uint64_t rows, uint32_t V, uint64_t ld, uint32_t top,
+                             float scale, float teacher_scale, float grad_scale, int mode);
 
 /* ---- optimizer step over the parameter slab (the consumer of the gradients above) ---- */
 

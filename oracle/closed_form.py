@@ -157,6 +157,89 @@ def cross_entropy(x, labels):
     return logsumexp(x, axis=-1) - picked
 
 
+def _softmax_rows(z):
+    """(p, log p, lse) of rows z [rows, V]; a row of -inf has p = 0 and lse = -inf"""
+    with np.errstate(divide="ignore", invalid="ignore"):
+        m = z.max(-1, keepdims=True)
+        m = np.where(np.isneginf(m), 0.0, m)
+        e = np.exp(z - m)
+        log_sum = np.log(e.sum(-1, keepdims=True))
+        lse = m + log_sum
+        # (not z - lse: next to a maximum of -3.4e38 the logarithm is lost in a float64 too)
+        logp = np.where(np.isneginf(lse), -np.inf, (z - m) - log_sum)
+    return np.exp(logp), logp, lse[..., 0]
+
+
+def token_logprobs(x, tokens, scale=1.0, top=0):
+    """(logp, entropy, lse, top_ids, top_logp) of rows x [rows, V]; classes at -inf are no alternatives, token -1 is none"""
+    z = f64(x) * float(np.float32(scale))
+    p, logp, lse = _softmax_rows(z)
+    rows, V = z.shape
+    at = logp[np.arange(rows), np.clip(tokens, 0, V - 1)]
+    at = np.where((np.asarray(tokens) >= 0) & ~np.isneginf(lse), at, 0.0)
+    entropy = -np.where(p == 0, 0.0, p * np.where(p == 0, 0.0, logp)).sum(-1)
+    ids, values = np.full((rows, top), -1, np.int64), np.full((rows, top), -np.inf)
+    for r in range(rows):
+        order = [v for v in np.lexsort((np.arange(V), -f64(x)[r]))[:top] if f64(x)[r, v] > -np.inf]
+        ids[r, :len(order)] = order
+        values[r, :len(order)] = logp[r, order]
+    return at, entropy, lse, ids, values
+
+
+def token_logprobs_grad(x, tokens, dlogp, dentropy, scale=1.0):
+    """gradient of sum dlogp * logp + dentropy * entropy (either may be None)"""
+    s = float(np.float32(scale))
+    p, logp, lse = _softmax_rows(f64(x) * s)
+    d = np.zeros_like(p)
+    if dlogp is not None:
+        g = np.where((np.asarray(tokens) >= 0) & ~np.isneginf(lse), f64(dlogp), 0.0)
+        d -= g[:, None] * p
+        d[np.arange(len(g)), np.clip(tokens, 0, p.shape[1] - 1)] += g
+    if dentropy is not None:
+        plogp = p * np.where(p == 0, 0.0, logp)
+        d -= f64(dentropy)[:, None] * (plogp - p * plogp.sum(-1, keepdims=True))
+    return d * s
+
+
+def topk_distill(x, ids, values, scale=1.0, teacher_scale=1.0, tail=False):
+    """(loss, d loss / d x) of rows x [rows, V], a row and a slot at a time"""
+    s, ts = float(np.float32(scale)), float(np.float32(teacher_scale))
+    p, logp, lse = _softmax_rows(f64(x) * s)
+    rows, V = p.shape
+    loss, grad = np.zeros(rows), np.zeros_like(p)
+    for r in range(rows):
+        used = [(int(i), float(v)) for i, v in zip(ids[r], values[r]) if i >= 0]
+        if not used or np.isneginf(lse[r]):
+            continue
+        u = np.array([v for _, v in used], np.float64)
+        if tail:
+            log_q = u
+        else:
+            if np.isneginf(u * ts).all():
+                continue
+            _, log_q, _ = _softmax_rows(u[None] * ts)
+            log_q = log_q[0]
+        q = np.exp(log_q)
+        for (i, _), qk, lq in zip(used, q, log_q):
+            if qk > 0:
+                loss[r] += qk * (lq - logp[r, i])
+            grad[r, i] -= qk
+        mass = q.sum()
+        outside = np.ones(V, bool)
+        outside[[i for i, _ in used]] = False
+        q_rest = max(0.0, 1.0 - mass)
+        if tail and outside.any() and not np.isneginf(logp[r, outside]).all():
+            m = logp[r, outside].max()
+            log_rest = m + np.log(np.exp(logp[r, outside] - m).sum())
+            if q_rest > 0:
+                loss[r] += q_rest * (np.log(q_rest) - log_rest)
+            grad[r] += (mass + q_rest) * p[r]
+            grad[r, outside] -= q_rest * np.exp(logp[r, outside] - log_rest)
+        else:
+            grad[r] += mass * p[r]
+    return loss, grad * s
+
+
 def cross_entropy_grad(x, labels, dloss):
     from scipy.special import softmax
     p = softmax(f64(x), axis=-1)

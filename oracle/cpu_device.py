@@ -20,10 +20,12 @@ from autograd_amd.backend import Backend
 from autograd_amd.device import Device
 from autograd_amd.op import (AddLayerNormOp, AddOp, AddRMSNormOp, ContiguousOp, CrossEntropyLossOp, EmbeddingSumOp,
                              BiasGELUOp, ExpOp, GatherOp, GELUOp, LayerNormOp, LogOp, MulOp, PermuteOp, ReLUSquaredOp, ReshapeOp,
-                             RMSNormOp, RopeOp, RsqrtOp, SoftmaxOp, SwiGLUOp, TransposeOp, ViewOp)
+                             RMSNormOp, RopeOp, RsqrtOp, SoftmaxOp, SwiGLUOp, TokenLogprobsOp, TopKDistillOp, TransposeOp,
+                             ViewOp)
 from autograd_amd.storage import Allocator, Storage
 from autograd_amd.utils import is_bf16, storage_dtype
 
+from . import closed_form as cf
 from . import cpu_ops as K
 
 
@@ -376,6 +378,55 @@ def cpu_cross_entropy_backward(inputs, outputs, scratch=None):
         K.cross_entropy_backward_into(_val(logits), labels.storage.data, _val(loss.grad), acc)
 
 
+# (no counterpart in the reference: the float64 forms, rounded once)
+def _rows(t):
+    v = t if isinstance(t, np.ndarray) else _val(t)
+    return v.reshape(-1, v.shape[-1])
+
+
+def cpu_token_logprobs_forward(inputs, outputs, scratch=None):
+    logits, tokens = inputs
+    op = outputs[0].op.op
+    logp, lse, entropy, top_ids, top_logp = op.split(outputs)
+    values = cf.token_logprobs(_rows(logits), tokens.storage.data.reshape(-1), op.scale, op.top)
+    for t, v in zip((logp, entropy, lse, top_ids, top_logp), values):
+        if t is not None:
+            t.storage.data[...] = v.reshape(t.shape)
+
+
+def cpu_token_logprobs_backward(inputs, outputs, scratch=None):
+    logits, tokens = inputs
+    op = outputs[0].op.op
+    logp, _, entropy, _, _ = op.split(outputs)
+    dent = entropy.grad if entropy is not None else None
+    if not logits.requires_grad or (logp.grad is None and dent is None):
+        return
+    d = cf.token_logprobs_grad(_rows(logits), tokens.storage.data.reshape(-1),
+                               None if logp.grad is None else _val(logp.grad).reshape(-1),
+                               None if dent is None else _val(dent).reshape(-1), op.scale)
+    with _Acc(logits.grad) as acc:
+        acc += d.reshape(acc.shape).astype(np.float32)
+
+
+def _cpu_distill(inputs, op):
+    logits, ids, values = inputs
+    return cf.topk_distill(_rows(logits), _rows(ids.storage.data), _rows(values), op.scale, op.teacher_scale, op.tail)
+
+
+def cpu_distill_forward(inputs, outputs, scratch=None):
+    loss = outputs[0]
+    loss.storage.data[...] = _cpu_distill(inputs, loss.op.op)[0].reshape(loss.shape)
+
+
+def cpu_distill_backward(inputs, outputs, scratch=None):
+    logits, loss = inputs[0], outputs[0]
+    if loss.grad is None or not logits.requires_grad:
+        return
+    d = _cpu_distill(inputs, loss.op.op)[1] * _val(loss.grad).reshape(-1, 1)
+    with _Acc(logits.grad) as acc:
+        acc += d.reshape(acc.shape).astype(np.float32)
+
+
 def cpu_rope_forward(inputs, outputs, scratch=None):
     q, k, cos, sin = inputs
     q2, k2 = outputs
@@ -418,7 +469,8 @@ class CPUBackend(Backend):
             GELUOp: cpu_gelu_forward, BiasGELUOp: cpu_bias_gelu_forward, ReLUSquaredOp: cpu_relu2_forward, SwiGLUOp: cpu_swiglu_forward,
             LayerNormOp: cpu_layernorm_forward, RMSNormOp: cpu_rmsnorm_forward,
             AddLayerNormOp: cpu_add_norm_forward, AddRMSNormOp: cpu_add_norm_forward, RopeOp: cpu_rope_forward,
-            CrossEntropyLossOp: cpu_cross_entropy_forward,
+            CrossEntropyLossOp: cpu_cross_entropy_forward, TokenLogprobsOp: cpu_token_logprobs_forward,
+            TopKDistillOp: cpu_distill_forward,
             MulOp: cpu_mul_forward, ExpOp: cpu_exp_forward, LogOp: cpu_log_forward, RsqrtOp: cpu_rsqrt_forward,
             SoftmaxOp: cpu_softmax_forward,
             ViewOp: cpu_view_forward, ReshapeOp: cpu_view_forward, PermuteOp: cpu_view_forward,
@@ -429,7 +481,8 @@ class CPUBackend(Backend):
             GELUOp: cpu_gelu_backward, BiasGELUOp: cpu_bias_gelu_backward, ReLUSquaredOp: cpu_relu2_backward, SwiGLUOp: cpu_swiglu_backward,
             LayerNormOp: cpu_layernorm_backward, RMSNormOp: cpu_rmsnorm_backward,
             AddLayerNormOp: cpu_add_norm_backward, AddRMSNormOp: cpu_add_norm_backward, RopeOp: cpu_rope_backward,
-            CrossEntropyLossOp: cpu_cross_entropy_backward,
+            CrossEntropyLossOp: cpu_cross_entropy_backward, TokenLogprobsOp: cpu_token_logprobs_backward,
+            TopKDistillOp: cpu_distill_backward,
             MulOp: cpu_mul_backward, ExpOp: cpu_exp_backward, LogOp: cpu_log_backward, RsqrtOp: cpu_rsqrt_backward,
             SoftmaxOp: cpu_softmax_backward,
             ViewOp: cpu_dense_grad_backward, ReshapeOp: cpu_dense_grad_backward, PermuteOp: cpu_permute_backward,

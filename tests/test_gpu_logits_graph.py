@@ -1,0 +1,282 @@
+"""Token log probabilities and top-k distillation through Runtime(device="hip"), beside the oracle device, recorded into
+graphs and from two contexts at once."""
+import ctypes as C
+import threading
+
+import numpy as np
+import pytest
+
+from autograd_amd import capi
+from autograd_amd.optimizer import AdamW
+from autograd_amd.runtime import Runtime
+from autograd_amd.tensor import Tensor
+from autograd_amd.utils import BF16
+from oracle import closed_form as cf
+from oracle import cpu_device
+from tests import logits_ops as L
+
+pytestmark = pytest.mark.gpu
+cpu_device.register()
+
+
+def leaf(device, shape, dtype, grad, val):
+    return Tensor(shape=shape, dtype=dtype, device=device, requires_grad=grad, init_val=val)
+
+
+def compiled(device, loss, **kw):
+    rt = Runtime(device=device, **kw)
+    rt.loss = loss
+    rt.build_topo(loss)
+    rt.bind_memory()
+    rt.is_compiled = True
+    return rt
+
+
+def test_policy_gradient_graph():
+    """loss = logp * advantage + entropy * bonus, where both come from one node; against the oracle device"""
+    rng = np.random.default_rng(1)
+    B, N, V = 3, 5, 301
+    x_np = (2 * rng.standard_normal((B, N, V))).astype(np.float32)
+    t_np = rng.integers(0, V, (B, N)).astype(np.int32)
+    t_np[0, 0] = -1
+    adv, bonus = rng.standard_normal((B, N)).astype(np.float32), np.full((B, N), 0.05, np.float32)
+    got = {}
+    for device in ("cpu", "hip"):
+        for fuse in (True, False):
+            x, t = leaf(device, x_np.shape, np.float32, True, x_np), leaf(device, t_np.shape, np.int32, False, t_np)
+            a, b = leaf(device, adv.shape, np.float32, False, adv), leaf(device, adv.shape, np.float32, False, bonus)
+            r = x.token_logprobs(t, entropy=True, scale=0.8)
+            loss = r.logp * a + r.entropy * b
+            rt = compiled(device, loss, fuse_grad_zeroing=fuse)
+            rt.backward(loss)
+            got[device, fuse] = rt.backend.copy_to_host(loss).copy(), rt.backend.copy_to_host(x.grad).copy()
+            rt.release()
+    want = cf.token_logprobs_grad(x_np.reshape(-1, V), t_np.reshape(-1), adv.reshape(-1), bonus.reshape(-1), 0.8).reshape(x_np.shape)
+    for key, (value, grad) in got.items():
+        # kernel bounds: 2e-5 of values up to 8 in the loss; p (|g| + |h| (|log p| + entropy)) <= 4 with 1e-5 in the gradient
+        np.testing.assert_allclose(value, got["cpu", True][0], rtol=0, atol=2e-5, err_msg=str(key))
+        np.testing.assert_allclose(grad, want, rtol=1e-5, atol=1e-5, err_msg=str(key))
+
+
+def test_alternatives_alone_leave_a_zero_gradient():
+    """logits that need a gradient but whose node gives none: the first writer writes zeros"""
+    rng = np.random.default_rng(2)
+    x_np = rng.standard_normal((1, 4, 50)).astype(np.float32)
+    x = leaf("hip", x_np.shape, np.float32, True, x_np)
+    t = leaf("hip", (1, 4), np.int32, False, np.zeros((1, 4), np.int32))
+    s_np = rng.standard_normal((1, 4, 50)).astype(np.float32)
+    s = leaf("hip", s_np.shape, np.float32, True, s_np)
+    r = x.token_logprobs(t, top=3)
+    loss = s.distill_topk(r.top_ids, r.top_logp, tail=True)
+    rt = compiled("hip", loss)
+    rt.backend.copy_from_host(x.grad, np.full_like(x_np, 5.0))
+    rt.backward(loss)
+    assert not rt.backend.copy_to_host(x.grad).any()
+    ids, top = cf.token_logprobs(x_np[0], np.zeros(4, int), 1.0, 3)[3:]
+    want = cf.topk_distill(s_np[0], ids, top.astype(np.float32), tail=True)[1]
+    np.testing.assert_allclose(rt.backend.copy_to_host(s.grad)[0], want, rtol=1e-5, atol=1e-5)
+    rt.release()
+
+
+def distillation(device, dtype, seed=3, B=4, N=16, V=500, K=12):
+    """an embedding student -> norm -> logits table, its teacher's logits as an input; returns what a step needs"""
+    rng = np.random.default_rng(seed)
+    cast = (lambda a: L.rounded(a, "bf16")) if dtype == BF16 else (lambda a: a.astype(np.float32))
+    table = leaf(device, (40, V), dtype, True, cast(0.5 * rng.standard_normal((40, V))))
+    gamma = leaf(device, (V,), np.float32, True, np.ones(V, np.float32))
+    ids = leaf(device, (B, N), np.int32, False, np.zeros((B, N), np.int32))
+    teacher = leaf(device, (B, N, V), dtype, False, cast(rng.standard_normal((B, N, V))))
+    tokens = leaf(device, (B, N), np.int32, False, np.zeros((B, N), np.int32))
+    said = teacher.token_logprobs(tokens, top=K, entropy=True, scale=0.9)
+    loss = ids.gather(table).rms_norm(gamma).distill_topk(said.top_ids, said.top_logp, tail=True, scale=1.1)
+    return compiled(device, loss), loss, (ids, tokens, teacher), (table, gamma)
+
+
+def batch(rng, V, cast):
+    return (rng.integers(0, 40, (4, 16)).astype(np.int32), rng.integers(0, V, (4, 16)).astype(np.int32),
+            cast(2 * rng.standard_normal((4, 16, V))))
+
+
+@pytest.mark.parametrize("dtype", [np.float32, BF16])
+def test_teacher_and_student_train_together_on_both_devices(dtype):
+    """Four optimizer steps of teacher -> alternatives -> student loss -> gradient -> AdamW on "hip" and on the oracle device.
+    Every step starts from the oracle's parameters, so that each comparison is of one step."""
+    cast = (lambda a: L.rounded(a, "bf16")) if dtype == BF16 else (lambda a: a.astype(np.float32))
+    steps = {}
+    for device in ("cpu", "hip"):
+        steps[device] = distillation(device, dtype)
+    rng = np.random.default_rng(4)
+    opts = {d: AdamW([s[3][1]], lr=1e-2, runtime=s[0]) for d, s in steps.items()}
+    for step in range(4):
+        data = batch(rng, 500, cast)
+        out = {}
+        for device, (rt, loss, feeds, params) in steps.items():
+            for t, v in zip(feeds, data):
+                rt.backend.copy_from_host(t, v)
+            if device == "hip":
+                for mine, theirs in zip(params, steps["cpu"][3]):
+                    rt.backend.copy_from_host(mine, before[id(theirs)])
+            before = {id(p): rt.backend.copy_to_host(p).copy() for p in params} if device == "cpu" else before
+            rt.backward(loss, grad_scale=1.0 / 64)
+            out[device] = [rt.backend.copy_to_host(loss).copy()] + [rt.backend.copy_to_host(p.grad).copy() for p in params]
+            opts[device].step()
+            out[device].append(rt.backend.copy_to_host(params[1]).copy())
+        a, b = out["hip"], out["cpu"]
+        if dtype == BF16:
+            # The student's logits are rounded to bf16 on both devices from fp32 values that differ by 1e-6: where that falls on
+            # two sides of a rounding, a logit of size <= 8 differs by a step, 2^-5, in rare places; p <= 1 of it reaches the loss.
+            np.testing.assert_allclose(a[0], b[0], rtol=0, atol=2 ** -5)
+            scale = np.abs(b[1]).max()
+            assert np.abs(a[1] - b[1]).max() <= 4 * 2 ** -8 * scale + 2 ** -5 * scale     # (three roundings on the way, and that step)
+        else:
+            np.testing.assert_allclose(a[0], b[0], rtol=1e-5, atol=5e-5)     # sum_error(500) on logarithms up to 12
+            for g, w in zip(a[1:3], b[1:3]):
+                assert np.abs(g - w).max() <= 5e-5 * max(1e-3, np.abs(w).max())
+        assert np.isfinite(a[3]).all() and not np.array_equal(a[3], before[id(steps["cpu"][3][1])])
+    for rt, *_ in steps.values():
+        if rt.allocator.device == "hip":
+            rt.release()
+
+
+def test_recorded_step_replays_like_the_eager_one():
+    """the whole step in a graph, replayed with other data and eager work of the same leaves between the replays"""
+    rt, loss, feeds, params = distillation("hip", np.float32)
+    rng = np.random.default_rng(5)
+    datas = [batch(rng, 500, lambda a: a.astype(np.float32)) for _ in range(4)]
+
+    def feed(d):
+        for t, v in zip(feeds, d):
+            rt.backend.copy_from_host(t, v)
+
+    def results():
+        rt.backend.synchronize()
+        return [rt.backend.copy_to_host(t).copy() for t in [loss] + [p.grad for p in params]]
+
+    eager = []
+    for d in datas:
+        feed(d)
+        rt.backward(loss)
+        eager.append(results())
+    feed(datas[0])
+    g = rt.capture(rt.execute)
+    # (the table's gradient is cleared by the rows of the pass before: every replay follows another replay)
+    feed(datas[3])
+    rt.backend.fill(params[0].grad, 0)
+    for again in range(2):
+        for d, want in zip(datas, eager):
+            feed(d)
+            rt.backend.fill(params[0].grad, 0)
+            g.launch()
+            for a, b in zip(results(), want):
+                np.testing.assert_array_equal(a, b)
+    g.destroy()
+    rt.release()
+
+
+def single_rows(ctx, seed):
+    """what two graphs of one context share is its own scratch: a few long rows of both operators"""
+    rng = np.random.default_rng(seed)
+    x = L.store(L.logits(rng, 2, 60000, "bf16"), "bf16")
+    t = rng.integers(0, 60000, 2).astype(np.int32)
+    ids, u = L.teacher(rng, 2, 60000, 9, True)
+    return x, t, ids, u
+
+
+def enqueue(ctx, dev, data):
+    x, t, ids, u = data
+    rows, V = x.shape
+    d = dict(x=dev.up(x), t=dev.up(t), i=dev.up(ids), u=dev.up(u), logp=dev.up(np.zeros(rows, np.float32)), ent=dev.up(np.zeros(rows, np.float32)),
+             top=dev.up(np.zeros((rows, 7), np.int32)), tl=dev.up(np.zeros((rows, 7), np.float32)), loss=dev.up(np.zeros(rows, np.float32)),
+             dx=dev.up(np.zeros_like(x)))
+
+    def launch():
+        ctx.call("agrad_token_logprobs_forward", capi.BF16, L.p(d["x"]), L.p(d["t"]), L.p(d["logp"]), L.p(d["ent"]), None, L.p(d["top"]),
+                 L.p(d["tl"]), rows, V, V, 7, 1.0)
+        ctx.call("agrad_topk_distill_fused", capi.BF16, L.p(d["x"]), L.p(d["i"]), L.p(d["u"]), L.p(d["loss"]), None, L.p(d["dx"]), rows, V, V,
+                 9, 1.0, 1.0, 1.0, 1)
+
+    def results():
+        ctx.synchronize()
+        return {k: d[k].download() for k in ("logp", "ent", "top", "tl", "loss", "dx")}
+
+    return launch, results
+
+
+def test_two_recorded_graphs_and_eager_calls_in_turn(ctx):
+    with L.Device(ctx) as dev:
+        calls = [enqueue(ctx, dev, single_rows(ctx, s)) for s in (1, 2, 3)]
+        want = []
+        for launch, results in calls:
+            launch()
+            want.append(results())
+        graphs = []
+        for launch, _ in calls[:2]:
+            ctx.call("agrad_graph_begin")
+            launch()
+            g = C.c_uint64()
+            ctx.call("agrad_graph_end", C.byref(g))
+            graphs.append(g.value)
+        for _ in range(4):
+            ctx.call("agrad_graph_launch", graphs[0])
+            calls[2][0]()
+            ctx.call("agrad_graph_launch", graphs[1])
+            ctx.call("agrad_graph_launch", graphs[0])
+            for (_, results), w in zip(calls, want):
+                for k, v in results().items():
+                    np.testing.assert_array_equal(v, w[k], err_msg=k)
+        for g in graphs:
+            ctx.call("agrad_graph_destroy", g)
+
+
+def test_two_contexts_at_once(ctx):
+    """calls of two contexts run on two streams: neither reads what the other leaves in its scratch"""
+    other = capi.Context(0)
+    try:
+        data = [single_rows(ctx, s) for s in (11, 12)]
+        with L.Device(ctx) as a, L.Device(other) as b:
+            calls = [enqueue(ctx, a, data[0]), enqueue(other, b, data[1])]
+            want = []
+            for launch, results in calls:
+                launch()
+                want.append(results())
+            errors = []
+
+            def work(c, w):
+                try:
+                    for _ in range(30):
+                        c[0]()
+                    for k, v in c[1]().items():
+                        np.testing.assert_array_equal(v, w[k], err_msg=k)
+                except Exception as e:      # noqa: BLE001
+                    errors.append(e)
+
+            threads = [threading.Thread(target=work, args=(c, w)) for c, w in zip(calls, want)]
+            for t in threads:
+                t.start()
+            for t in threads:
+                t.join()
+            assert not errors, errors
+    finally:
+        other.close()
+
+
+def test_buffers_of_another_context_or_too_small_are_refused():
+    from autograd_amd import hip_ext
+    one, two = hip_ext.HipContext(0), hip_ext.HipContext(0)
+    x, t, o = one.alloc(4 * 64), one.alloc(4 * 8), one.alloc(4 * 8)
+    foreign = two.alloc(4 * 64)
+    one.fill_scalar("", [x], [0], 0.0, 64)
+    one.fill_scalar("", [t], [0], 0.0, 8)
+    offs = [0] * 7
+
+    def call(ids, rows=8, V=8, ld=8, top=0, offs=offs):
+        one.token_logprobs_forward(hip_ext.F32, ids, offs, rows, V, ld, top, 1.0)
+
+    call([x, t, o, 0, 0, 0, 0])
+    one.synchronize()
+    for bad in (dict(ids=[foreign, t, o, 0, 0, 0, 0]), dict(ids=[x, t, o, 0, 0, 0, 0], rows=9), dict(ids=[x, t, o, 0, 0, 0, 0], ld=9),
+                dict(ids=[x, t, o, 0, 0, 0, 0], offs=[4] + [0] * 6), dict(ids=[x, t, o]), dict(ids=[0, t, o, 0, 0, 0, 0]),
+                dict(ids=[x, t, o, 0, 0, o, o], top=2)):
+        with pytest.raises(ValueError):
+            call(**bad)
+    one.synchronize()
