@@ -18,6 +18,7 @@ namespace {
 
 constexpr int kLpBlock = 256;
 constexpr int kLpUnroll = 4;         // vectors a thread keeps in flight
+static_assert(AGRAD_MAX_TOP <= kLpBlock, "a thread an alternative");
 constexpr int kCandidates = 1024;    // candidates of a row's alternatives that LDS holds
 
 struct LpArgs {
@@ -57,11 +58,10 @@ __device__ __forceinline__ void append(Candidates& q, bool has, uint64_t key) {
 }
 
 // Keeps the largest `top` of the candidates, in descending order at the front: a key's place is the number of larger
-// keys, counted.  All threads of the workgroup call it after a barrier; it ends with one.
-template <int BLOCK>
-__device__ __forceinline__ void prune(Candidates& q, uint32_t top) {
-    constexpr int EACH = kCandidates / BLOCK;
-    const uint32_t n = q.count < (uint32_t)kCandidates ? q.count : (uint32_t)kCandidates;
+// keys, counted (n / BLOCK keys a thread, each against all n: a tenth of the barriers of a sorting network, and faster up to
+// some hundred keys, which is what a row leaves).  All threads call it after a barrier; it ends with one.
+template <int BLOCK, int EACH>
+__device__ __forceinline__ void prune_each(Candidates& q, uint32_t n, uint32_t top) {
     uint64_t mine[EACH];
     uint32_t larger[EACH];
 #pragma unroll
@@ -70,6 +70,7 @@ __device__ __forceinline__ void prune(Candidates& q, uint32_t top) {
         mine[i] = at < n ? q.key[at] : 0ull;
         larger[i] = 0;
     }
+#pragma unroll 4
     for (uint32_t j = 0; j < n; ++j) {
         const uint64_t other = q.key[j];
 #pragma unroll
@@ -82,10 +83,35 @@ __device__ __forceinline__ void prune(Candidates& q, uint32_t top) {
     if (threadIdx.x == 0) q.count = n < top ? n : top;
     __syncthreads();
 }
+template <int BLOCK>
+__device__ __forceinline__ void prune(Candidates& q, uint32_t top) {
+    const uint32_t n = q.count < (uint32_t)kCandidates ? q.count : (uint32_t)kCandidates;
+    if (n <= (uint32_t)BLOCK) prune_each<BLOCK, 1>(q, n, top);
+    else prune_each<BLOCK, kCandidates / BLOCK>(q, n, top);
+}
 
-// the alternatives of a whole row, one element a thread and step
+// The upper half of a bound that at least `top` of the threads' values reach, as high as such a bound can be; 0 if fewer
+// than `top` threads have a value (0: none).  Every wave finds it for itself, bit by bit, from all values in LDS.
+template <int BLOCK>
+__device__ __forceinline__ uint32_t bound_of(const uint32_t* values, uint32_t top) {
+    constexpr int EACH = BLOCK / kWave;
+    uint32_t v[EACH];
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) v[i] = values[i * kWave + threadIdx.x % kWave] >> 16;
+    uint32_t bound = 0;
+    for (int bit = 15; bit >= 0; --bit) {
+        const uint32_t higher = bound | (1u << bit);
+        uint32_t count = 0;
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) count += (uint32_t)__popcll(__ballot(v[i] >= higher));
+        if (count >= top) bound = higher;
+    }
+    return bound;
+}
+
+// The alternatives of a whole row, one element a thread and step: right for any row, and slow.
 template <typename T, int BLOCK>
-__device__ __forceinline__ void row_top(const T* base, uint32_t V, uint32_t top, Candidates& q) {
+__device__ __forceinline__ void row_top_by_steps(const T* base, uint32_t V, uint32_t top, Candidates& q) {
     if (threadIdx.x == 0) q.count = 0;
     __syncthreads();
     uint64_t floor_key = 0;
@@ -107,9 +133,69 @@ __device__ __forceinline__ void row_top(const T* base, uint32_t V, uint32_t top,
     prune<BLOCK>(q, top);
 }
 
+// The alternatives of a row of which every thread has seen its share (the vectors whose number is its own modulo BLOCK,
+// an element outside the vectors) and kept the largest logit, `best`.  At least `top` classes reach the top-th largest of
+// those BLOCK values, and hardly more do (70 of 151936 for top = 64, 180 for top = 128, as the shares are interleaved), so
+// the row is not read again: only the shares whose largest logit reaches the bound are, by all threads together.  A row
+// whose largest logits crowd into few shares, or are equal in great number, can leave more candidates than LDS holds and
+// goes the slow way.
+template <typename T, int VEC, int BLOCK>
+__device__ __forceinline__ void row_top(const T* base, uint32_t V, uint32_t top, float best, Candidates& q, uint32_t* shares) {
+    const RowParts<T, VEC> parts(base, V);
+    const uint32_t mine = (uint32_t)(class_key(best, 0u) >> 32);
+    shares[threadIdx.x] = mine;
+    if (threadIdx.x == 0) q.count = 0;
+    __syncthreads();
+    const uint32_t bound = bound_of<BLOCK>(shares, top);
+    __syncthreads();
+    // the shares to look at, listed in any order
+    __shared__ uint32_t listed;
+    if (threadIdx.x == 0) listed = 0;
+    __syncthreads();
+    if (mine != 0u && (mine >> 16) >= bound) shares[atomicAdd(&listed, 1u)] = threadIdx.x;
+    __syncthreads();
+    if (threadIdx.x < parts.extra) {
+        const uint32_t e = parts.extra_at(threadIdx.x);
+        float x[1];
+        VecIO<T, 1>::load(base + e, x);
+        const uint64_t key = class_key(x[0], e);
+        append(q, key != 0ull && (uint32_t)(key >> 48) >= bound, key);
+    }
+    const uint32_t n = listed, pairs = n * ((parts.nvec + BLOCK - 1) / BLOCK);
+    const T* body = base + parts.head;
+    constexpr int U = 4;
+    for (uint32_t i0 = threadIdx.x; i0 < pairs; i0 += BLOCK * U) {
+        float v[U][VEC];
+        uint32_t vec[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t i = i0 + u * BLOCK, tile = i / n;
+            vec[u] = i < pairs ? tile * BLOCK + shares[i - tile * n] : parts.nvec;
+            if (vec[u] < parts.nvec) VecIO<T, VEC>::load(body + (uint64_t)vec[u] * VEC, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t e = parts.head + vec[u] * VEC;
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) {
+                const uint64_t key = vec[u] < parts.nvec ? class_key(v[u][k], e + k) : 0ull;
+                append(q, key != 0ull && (uint32_t)(key >> 48) >= bound, key);
+            }
+        }
+        if (__hip_atomic_load(&q.count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) > (uint32_t)kCandidates) break;
+    }
+    __syncthreads();
+    if (q.count > (uint32_t)kCandidates) {
+        __syncthreads();
+        row_top_by_steps<T, BLOCK>(base, V, top, q);
+    } else {
+        prune<BLOCK>(q, top);
+    }
+}
+
 // ---- forward -----------------------------------------------------------------------------------------
 template <typename T, int VEC, bool ENT>
-__device__ __forceinline__ RowStat row_stat(const T* base, uint32_t V, float c, RowStat* lds) {
+__device__ __forceinline__ RowStat row_stat(const T* base, uint32_t V, float c, RowStat* lds, float& best) {
     const RowParts<T, VEC> parts(base, V);
     RowStat a = empty_stat();
     if (threadIdx.x < parts.extra) {
@@ -129,6 +215,7 @@ __device__ __forceinline__ RowStat row_stat(const T* base, uint32_t V, float c, 
         for (int u = 0; u < kLpUnroll; ++u)
             if (i0 + u * kLpBlock < parts.nvec) absorb_stat<ENT, VEC>(a, v[u], c);
     }
+    best = a.m;
     return block_stat<kLpBlock, ENT>(a, c, lds);
 }
 
@@ -137,9 +224,11 @@ __global__ void __launch_bounds__(kLpBlock)
 logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
     __shared__ RowStat lds[kLpBlock / kWave];
     __shared__ Candidates found;
+    __shared__ uint32_t shares[kLpBlock];
     const uint64_t row = blockIdx.x;
     const T* base = x + row * a.ld;
-    const RowStat t = row_stat<T, VEC, ENT>(base, a.V, a.c, lds);
+    float best;
+    const RowStat t = row_stat<T, VEC, ENT>(base, a.V, a.c, lds, best);
     const bool empty = t.m == -INFINITY && t.s == 0.0f;
     const float log_s = logf(t.s);                                // -inf for an empty row
     if (threadIdx.x == 0) {
@@ -159,7 +248,7 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
         }
     }
     if (a.top != 0) {
-        row_top<T, kLpBlock>(base, a.V, a.top, found);
+        row_top<T, VEC, kLpBlock>(base, a.V, a.top, best, found, shares);
         if (threadIdx.x < a.top) {
             const bool there = threadIdx.x < found.count;
             const uint64_t key = there ? found.key[threadIdx.x] : 0ull;
