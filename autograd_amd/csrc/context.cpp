@@ -33,6 +33,8 @@ struct agrad_ctx {
     std::vector<agrad::ColsumJob> pending;
     // counters and (max, sum) pairs of the workgroup teams of the fused cross-entropy (long rows)
     void* ce_scratch = nullptr;
+    // what the workgroups that share a row of logits leave for each other (logprobs.hip, distill.hip)
+    void* row_scratch = nullptr;
     uint32_t team_polls = 0;               // 0: the kernels' own bound on a team member's wait
 };
 
@@ -639,6 +641,9 @@ int agrad_ctx_create(int device, agrad_ctx** out) {
         e = hipHostGetDevicePointer((void**)&c->err_flag, pinned, 0);
     }
     if (e == hipSuccess) e = hipMalloc(&c->ce_scratch, ce_fused_scratch_bytes());
+    if (e == hipSuccess) e = hipMalloc(&c->row_scratch, shared_rows_bytes());
+    if (e == hipSuccess && launch_fill(c->stream, c->row_scratch, 0u, 4, shared_rows_bytes() / 4) != AGRAD_OK) e = hipErrorUnknown;
+    if (e == hipSuccess) e = hipStreamSynchronize(c->stream);
     if (e != hipSuccess) {
         agrad_ctx_destroy(c);
         return check_hip(e, "context setup");
@@ -654,6 +659,7 @@ int agrad_ctx_destroy(agrad_ctx* ctx) {
     for (auto& kv : ctx->graphs) (void)hipGraphExecDestroy(kv.second);
     for (auto& kv : ctx->allocs) (void)hipFree(reinterpret_cast<void*>(kv.first));
     if (ctx->ce_scratch) (void)hipFree(ctx->ce_scratch);
+    if (ctx->row_scratch) (void)hipFree(ctx->row_scratch);
     if (ctx->err_host) (void)hipHostFree(const_cast<int*>(ctx->err_host));
     if (ctx->ev_start) (void)hipEventDestroy(ctx->ev_start);
     if (ctx->ev_stop) (void)hipEventDestroy(ctx->ev_stop);
@@ -1151,7 +1157,7 @@ int agrad_token_logprobs_forward(agrad_ctx* ctx, int dtype, const void* logits, 
                                  uint64_t ld, uint32_t top, float scale) {
     CTX_OR_FAIL(ctx)
     return launch_logprobs_fwd(ctx->stream, dtype, logits, tokens, logp, entropy, lse, top_ids, top_logp, rows, V, ld, top, scale,
-                               ctx->err_flag);
+                               ctx->err_flag, ctx->row_scratch);
 }
 int agrad_token_logprobs_backward(agrad_ctx* ctx, int dtype, const void* logits, const int32_t* tokens, const float* lse,
                                   const float* entropy, const float* dlogp, const float* dentropy, void* dlogits,

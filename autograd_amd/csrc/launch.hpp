@@ -185,7 +185,9 @@ uint64_t ce_fused_scratch_bytes();
 int logits_check(const char* what, int dtype, const void* x, const void* dx, uint64_t rows, uint32_t V, uint64_t ld, float scale);
 int launch_logprobs_fwd(hipStream_t s, int dtype, const void* logits, const int32_t* tokens, float* logp, float* entropy,
                         float* lse, int32_t* top_ids, float* top_logp, uint64_t rows, uint32_t V, uint64_t ld, uint32_t top,
-                        float scale, int* err_flag);
+                        float scale, int* err_flag, void* scratch);
+// bytes of the memory through which workgroups share rows of logits; all zero before the first launch that uses it
+uint64_t shared_rows_bytes();
 int launch_logprobs_bwd(hipStream_t s, int dtype, const void* logits, const int32_t* tokens, const float* lse,
                         const float* entropy, const float* dlogp, const float* dentropy, void* dlogits, uint64_t rows,
                         uint32_t V, uint64_t ld, float scale, uint32_t flags, int* err_flag);

@@ -25,6 +25,7 @@ struct LpArgs {
     const int32_t* tokens; float* logp; float* entropy; float* lse; int32_t* top_ids; float* top_logp;
     uint64_t ld; uint32_t V, top; float scale, c;
     int* err_flag;
+    SharedRows shared; uint32_t parts;
 };
 
 // ---- alternatives ------------------------------------------------------------------------------------
@@ -109,18 +110,16 @@ __device__ __forceinline__ uint32_t bound_of(const uint32_t* values, uint32_t to
     return bound;
 }
 
-// The alternatives of a whole row, one element a thread and step: right for any row, and slow.
-template <typename T, int BLOCK>
-__device__ __forceinline__ void row_top_by_steps(const T* base, uint32_t V, uint32_t top, Candidates& q) {
+// The largest of n keys, one a thread and step: right whatever they are, and slow.
+template <int BLOCK, typename KeyAt>
+__device__ __forceinline__ void top_by_steps(uint32_t n, uint32_t top, Candidates& q, KeyAt key_at) {
     if (threadIdx.x == 0) q.count = 0;
     __syncthreads();
     uint64_t floor_key = 0;
-    for (uint32_t e0 = 0; e0 < V; e0 += BLOCK) {
-        const uint32_t e = e0 + threadIdx.x;
-        float x[1];
-        VecIO<T, 1>::load(base + (e < V ? e : 0u), x);
-        const uint64_t key = class_key(x[0], e);
-        append(q, e < V && key > floor_key, key);
+    for (uint32_t i0 = 0; i0 < n; i0 += BLOCK) {
+        const uint32_t i = i0 + threadIdx.x;
+        const uint64_t key = i < n ? key_at(i) : 0ull;
+        append(q, key > floor_key, key);
         __syncthreads();
         const bool full = q.count > (uint32_t)(kCandidates - BLOCK);
         __syncthreads();
@@ -133,15 +132,16 @@ __device__ __forceinline__ void row_top_by_steps(const T* base, uint32_t V, uint
     prune<BLOCK>(q, top);
 }
 
-// The alternatives of a row of which every thread has seen its share (the vectors whose number is its own modulo BLOCK,
-// an element outside the vectors) and kept the largest logit, `best`.  At least `top` classes reach the top-th largest of
-// those BLOCK values, and hardly more do (70 of 151936 for top = 64, 180 for top = 128, as the shares are interleaved), so
-// the row is not read again: only the shares whose largest logit reaches the bound are, by all threads together.  A row
-// whose largest logits crowd into few shares, or are equal in great number, can leave more candidates than LDS holds and
-// goes the slow way.
+// The alternatives of a stretch of a row's vectors (the first stretch: and of the elements outside the vectors) of which
+// every thread has seen its share, the vectors whose number is its own modulo BLOCK, and kept the largest logit, `best`.
+// At least `top` classes reach the top-th largest of those BLOCK values, and hardly more do (75 of 151936 for top = 64,
+// 180 for top = 128, as the shares are interleaved), so the row is not read again: only the shares whose largest logit
+// reaches the bound are, by all threads together.  A row whose largest logits crowd into few shares, or are equal in great
+// number, can leave more candidates than LDS holds and goes the slow way.
 template <typename T, int VEC, int BLOCK>
-__device__ __forceinline__ void row_top(const T* base, uint32_t V, uint32_t top, float best, Candidates& q, uint32_t* shares) {
-    const RowParts<T, VEC> parts(base, V);
+__device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& parts, const Stretch& part, uint32_t top, float best,
+                                        Candidates& q, uint32_t* shares) {
+    const uint32_t extra = part.lo == 0 ? parts.extra : 0u;
     const uint32_t mine = (uint32_t)(class_key(best, 0u) >> 32);
     shares[threadIdx.x] = mine;
     if (threadIdx.x == 0) q.count = 0;
@@ -154,14 +154,14 @@ __device__ __forceinline__ void row_top(const T* base, uint32_t V, uint32_t top,
     __syncthreads();
     if (mine != 0u && (mine >> 16) >= bound) shares[atomicAdd(&listed, 1u)] = threadIdx.x;
     __syncthreads();
-    if (threadIdx.x < parts.extra) {
+    if (threadIdx.x < extra) {
         const uint32_t e = parts.extra_at(threadIdx.x);
         float x[1];
         VecIO<T, 1>::load(base + e, x);
         const uint64_t key = class_key(x[0], e);
         append(q, key != 0ull && (uint32_t)(key >> 48) >= bound, key);
     }
-    const uint32_t n = listed, pairs = n * ((parts.nvec + BLOCK - 1) / BLOCK);
+    const uint32_t n = listed, pairs = n * ((part.hi - part.lo + BLOCK - 1) / BLOCK);
     const T* body = base + parts.head;
     constexpr int U = 4;
     for (uint32_t i0 = threadIdx.x; i0 < pairs; i0 += BLOCK * U) {
@@ -170,15 +170,15 @@ __device__ __forceinline__ void row_top(const T* base, uint32_t V, uint32_t top,
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const uint32_t i = i0 + u * BLOCK, tile = i / n;
-            vec[u] = i < pairs ? tile * BLOCK + shares[i - tile * n] : parts.nvec;
-            if (vec[u] < parts.nvec) VecIO<T, VEC>::load(body + (uint64_t)vec[u] * VEC, v[u]);
+            vec[u] = i < pairs ? part.lo + tile * BLOCK + shares[i - tile * n] : part.hi;
+            if (vec[u] < part.hi) VecIO<T, VEC>::load(body + (uint64_t)vec[u] * VEC, v[u]);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const uint32_t e = parts.head + vec[u] * VEC;
 #pragma unroll
             for (int k = 0; k < VEC; ++k) {
-                const uint64_t key = vec[u] < parts.nvec ? class_key(v[u][k], e + k) : 0ull;
+                const uint64_t key = vec[u] < part.hi ? class_key(v[u][k], e + k) : 0ull;
                 append(q, key != 0ull && (uint32_t)(key >> 48) >= bound, key);
             }
         }
@@ -187,36 +187,40 @@ __device__ __forceinline__ void row_top(const T* base, uint32_t V, uint32_t top,
     __syncthreads();
     if (q.count > (uint32_t)kCandidates) {
         __syncthreads();
-        row_top_by_steps<T, BLOCK>(base, V, top, q);
+        const uint32_t in_vectors = (part.hi - part.lo) * VEC;
+        top_by_steps<BLOCK>(in_vectors + extra, top, q, [&](uint32_t i) {
+            const uint32_t e = i < in_vectors ? parts.head + part.lo * VEC + i : parts.extra_at(i - in_vectors);
+            float x[1];
+            VecIO<T, 1>::load(base + e, x);
+            return class_key(x[0], e);
+        });
     } else {
         prune<BLOCK>(q, top);
     }
 }
 
 // ---- forward -----------------------------------------------------------------------------------------
-template <typename T, int VEC, bool ENT>
-__device__ __forceinline__ RowStat row_stat(const T* base, uint32_t V, float c, RowStat* lds, float& best) {
-    const RowParts<T, VEC> parts(base, V);
-    RowStat a = empty_stat();
-    if (threadIdx.x < parts.extra) {
-        float x[1];
-        VecIO<T, 1>::load(base + parts.extra_at(threadIdx.x), x);
-        absorb_stat<ENT, 1>(a, x, c);
+// the `top` largest of the keys that a row's parts left, descending
+template <int BLOCK>
+__device__ __forceinline__ void join_tops(const unsigned long long* keys, uint32_t n, uint32_t top, Candidates& q, uint32_t* shares) {
+    uint32_t best = 0;
+    for (uint32_t i = threadIdx.x; i < n; i += BLOCK) best = max(best, (uint32_t)(get_shared(keys + i) >> 32));
+    shares[threadIdx.x] = best;
+    if (threadIdx.x == 0) q.count = 0;
+    __syncthreads();
+    const uint32_t bound = bound_of<BLOCK>(shares, top);
+    for (uint32_t i0 = 0; i0 < n; i0 += BLOCK) {
+        const uint32_t i = i0 + threadIdx.x;
+        const uint64_t key = i < n ? get_shared(keys + i) : 0ull;
+        append(q, key != 0ull && (uint32_t)(key >> 48) >= bound, key);
     }
-    const T* body = base + parts.head;
-    for (uint32_t i0 = threadIdx.x; i0 < parts.nvec; i0 += kLpBlock * kLpUnroll) {
-        float v[kLpUnroll][VEC];
-#pragma unroll
-        for (int u = 0; u < kLpUnroll; ++u) {
-            const uint32_t i = i0 + u * kLpBlock;
-            if (i < parts.nvec) VecIO<T, VEC>::load(body + (uint64_t)i * VEC, v[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < kLpUnroll; ++u)
-            if (i0 + u * kLpBlock < parts.nvec) absorb_stat<ENT, VEC>(a, v[u], c);
+    __syncthreads();
+    if (q.count > (uint32_t)kCandidates) {
+        __syncthreads();
+        top_by_steps<BLOCK>(n, top, q, [&](uint32_t i) { return (uint64_t)get_shared(keys + i); });
+    } else {
+        prune<BLOCK>(q, top);
     }
-    best = a.m;
-    return block_stat<kLpBlock, ENT>(a, c, lds);
 }
 
 template <typename T, int VEC, bool ENT>
@@ -225,10 +229,50 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
     __shared__ RowStat lds[kLpBlock / kWave];
     __shared__ Candidates found;
     __shared__ uint32_t shares[kLpBlock];
-    const uint64_t row = blockIdx.x;
+    __shared__ uint32_t word;
+    const uint32_t row = blockIdx.x / a.parts, nth = blockIdx.x - row * a.parts;
     const T* base = x + row * a.ld;
-    float best;
-    const RowStat t = row_stat<T, VEC, ENT>(base, a.V, a.c, lds, best);
+    const RowParts<T, VEC> parts(base, a.V);
+    const Stretch part(parts.nvec, nth, a.parts);
+    RowStat t = empty_stat();
+    if (nth == 0 && threadIdx.x < parts.extra) {
+        float v[1];
+        VecIO<T, 1>::load(base + parts.extra_at(threadIdx.x), v);
+        absorb_stat<ENT, 1>(t, v, a.c);
+    }
+    const T* body = base + parts.head;
+    for (uint32_t i0 = part.lo + threadIdx.x; i0 < part.hi; i0 += kLpBlock * kLpUnroll) {
+        float v[kLpUnroll][VEC];
+#pragma unroll
+        for (int u = 0; u < kLpUnroll; ++u) {
+            const uint32_t i = i0 + u * kLpBlock;
+            if (i < part.hi) VecIO<T, VEC>::load(body + (uint64_t)i * VEC, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < kLpUnroll; ++u)
+            if (i0 + u * kLpBlock < part.hi) absorb_stat<ENT, VEC>(t, v[u], a.c);
+    }
+    const float best = t.m;
+    t = block_stat<kLpBlock, ENT>(t, a.c, lds);
+    if (a.top != 0) row_top<T, VEC, kLpBlock>(base, parts, part, a.top, best, found, shares);
+    if (a.parts > 1) {
+        if (threadIdx.x == 0) {
+            float* to = a.shared.stats + 4 * (uint64_t)blockIdx.x;
+            put_shared(to, t.m);
+            put_shared(to + 1, t.s);
+            if (ENT) put_shared(to + 2, t.d);
+        }
+        unsigned long long* keys = a.shared.keys + (uint64_t)row * a.parts * a.top;
+        if (threadIdx.x < a.top) put_shared(keys + nth * a.top + threadIdx.x, (unsigned long long)(threadIdx.x < found.count ? found.key[threadIdx.x] : 0ull));
+        if (!workgroup_arrives_last(a.shared.tickets + row, a.parts, &word)) return;
+        t = empty_stat();
+        if (threadIdx.x < a.parts) {
+            const float* from = a.shared.stats + 4 * ((uint64_t)row * a.parts + threadIdx.x);
+            t = RowStat{get_shared(from), get_shared(from + 1), ENT ? get_shared(from + 2) : 0.0f};
+        }
+        t = block_stat<kLpBlock, ENT>(t, a.c, lds);
+        if (a.top != 0) join_tops<kLpBlock>(keys, a.parts * a.top, a.top, found, shares);
+    }
     const bool empty = t.m == -INFINITY && t.s == 0.0f;
     const float log_s = logf(t.s);                                // -inf for an empty row
     if (threadIdx.x == 0) {
@@ -247,15 +291,12 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
             a.logp[row] = lp;
         }
     }
-    if (a.top != 0) {
-        row_top<T, VEC, kLpBlock>(base, a.V, a.top, best, found, shares);
-        if (threadIdx.x < a.top) {
-            const bool there = threadIdx.x < found.count;
-            const uint64_t key = there ? found.key[threadIdx.x] : 0ull;
-            const uint64_t to = row * a.top + threadIdx.x;
-            a.top_ids[to] = there ? (int32_t)key_index(key) : -1;
-            a.top_logp[to] = there ? (key_logit(key) - t.m) * a.scale - log_s : -INFINITY;
-        }
+    if (threadIdx.x < a.top) {
+        const bool there = threadIdx.x < found.count;
+        const uint64_t key = there ? found.key[threadIdx.x] : 0ull;
+        const uint64_t to = (uint64_t)row * a.top + threadIdx.x;
+        a.top_ids[to] = there ? (int32_t)key_index(key) : -1;
+        a.top_logp[to] = there ? (key_logit(key) - t.m) * a.scale - log_s : -INFINITY;
     }
 }
 
@@ -329,10 +370,11 @@ logprobs_bwd_kernel(const T* x, T* dx, const LpBwdArgs a, const FastDiv32 chunks
 }
 
 template <typename T>
-int lp_fwd_typed(hipStream_t s, const T* x, const LpArgs& a, uint64_t rows) {
+int lp_fwd_typed(hipStream_t s, const T* x, LpArgs a, uint64_t rows) {
     constexpr int WIDE = WideVec<T>::value;
     const bool wide = a.V >= 4 * WIDE;
-    const dim3 grid((uint32_t)rows), block(kLpBlock);
+    a.parts = a.shared.tickets != nullptr ? row_parts(rows, a.V / WIDE) : 1u;
+    const dim3 grid((uint32_t)rows * a.parts), block(kLpBlock);
     if (wide && a.entropy) hipLaunchKernelGGL((logprobs_fwd_kernel<T, WIDE, true>), grid, block, 0, s, x, a);
     else if (wide) hipLaunchKernelGGL((logprobs_fwd_kernel<T, WIDE, false>), grid, block, 0, s, x, a);
     else if (a.entropy) hipLaunchKernelGGL((logprobs_fwd_kernel<T, 1, true>), grid, block, 0, s, x, a);
@@ -366,6 +408,24 @@ int lp_bwd_typed(hipStream_t s, const T* x, T* dx, LpBwdArgs a, uint64_t rows) {
 
 }  // namespace
 
+uint64_t shared_rows_bytes() { return kSharedRowsBytes; }
+
+SharedRows shared_rows(void* scratch) {
+    char* at = static_cast<char*>(scratch);
+    return SharedRows{reinterpret_cast<float*>(at), reinterpret_cast<unsigned long long*>(at + 16ull * kSharedParts),
+                      reinterpret_cast<uint32_t*>(at + (16ull + 8ull * AGRAD_MAX_TOP) * kSharedParts)};
+}
+
+// Parts of a row: as many as make some thousand workgroups of all rows (four a CU: the loads of a few more waves than that
+// fill the memory's queues), but none shorter than two vectors a thread (a part costs its workgroup's reductions, and the
+// parts are put together one after the other).
+uint32_t row_parts(uint64_t rows, uint32_t vectors) {
+    uint64_t parts = kSharedParts / rows;
+    if (parts > vectors / 512u) parts = vectors / 512u;
+    if (parts > kMaxParts) parts = kMaxParts;
+    return parts < 1 ? 1u : (uint32_t)parts;
+}
+
 int logits_check(const char* what, int dtype, const void* x, const void* dx, uint64_t rows, uint32_t V, uint64_t ld, float scale) {
     if (dtype != AGRAD_F32 && dtype != AGRAD_BF16) return set_error(AGRAD_EINVAL, "%s: unknown dtype %d", what, dtype);
     if (V == 0 || V >= 0x7fffffffu) return set_error(AGRAD_EINVAL, "%s: %u classes", what, V);
@@ -381,7 +441,7 @@ int logits_check(const char* what, int dtype, const void* x, const void* dx, uin
 
 int launch_logprobs_fwd(hipStream_t s, int dtype, const void* logits, const int32_t* tokens, float* logp, float* entropy,
                         float* lse, int32_t* top_ids, float* top_logp, uint64_t rows, uint32_t V, uint64_t ld, uint32_t top,
-                        float scale, int* err_flag) {
+                        float scale, int* err_flag, void* scratch) {
     const char* what = "token log probabilities";
     if (int rc = logits_check(what, dtype, logits, nullptr, rows, V, ld, scale)) return rc;
     if (top > AGRAD_MAX_TOP) return set_error(AGRAD_EINVAL, "%s: at most %u alternatives, got %u", what, AGRAD_MAX_TOP, top);
@@ -392,7 +452,7 @@ int launch_logprobs_fwd(hipStream_t s, int dtype, const void* logits, const int3
         return set_error(AGRAD_EINVAL, "%s: top_ids and top_logp are given exactly when top > 0", what);
     if (logp == nullptr && entropy == nullptr && lse == nullptr && top == 0) return set_error(AGRAD_EINVAL, "%s: nothing to compute", what);
     const float c = (float)((double)scale * 1.4426950408889634);
-    const LpArgs a{tokens, logp, entropy, lse, top_ids, top_logp, ld, V, top, scale, c, err_flag};
+    const LpArgs a{tokens, logp, entropy, lse, top_ids, top_logp, ld, V, top, scale, c, err_flag, shared_rows(scratch), 1u};
     if (dtype == AGRAD_F32) return lp_fwd_typed<float>(s, (const float*)logits, a, rows);
     return lp_fwd_typed<bf16_t>(s, (const bf16_t*)logits, a, rows);
 }

@@ -8,6 +8,7 @@
 // a part in which no class is finite has m = -inf and s = 0.
 #pragma once
 
+#include "../../include/autograd_hip.h"
 #include "common.hpp"
 
 #include <math.h>
@@ -79,6 +80,55 @@ struct RowParts {
     // place of the i-th element outside the vectors
     __device__ __forceinline__ uint32_t extra_at(uint32_t i) const { return i < head ? i : tail_start + (i - head); }
 };
+
+// ---- a row shared by several workgroups --------------------------------------------------------------
+// Where there are fewer rows than fill the GPU, `parts` workgroups take a stretch of a row's vectors each, leave what they
+// found in memory that the context owns, and count themselves; the one that counts last puts the parts together.  Nobody
+// waits for anybody.  The counters are zero between launches (the last one puts its counter back), and all launches of a
+// context run on its one stream, recorded ones too, so that no two launches use the memory at once.
+constexpr uint32_t kSharedParts = 1024;      // workgroups of a launch that share rows, at most
+constexpr uint32_t kMaxParts = 64;           // parts of one row, at most
+struct SharedRows {
+    float* stats;             // [kSharedParts, 4]
+    unsigned long long* keys; // [kSharedParts, AGRAD_MAX_TOP]
+    uint32_t* tickets;        // [kSharedParts]
+};
+constexpr uint64_t kSharedRowsBytes = (uint64_t)kSharedParts * (16 + 8 * AGRAD_MAX_TOP + 4);
+
+template <typename V>
+__device__ __forceinline__ void put_shared(V* to, V value) { __hip_atomic_store(to, value, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename V>
+__device__ __forceinline__ V get_shared(const V* from) { return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// True, in every thread, for the workgroup whose arrival is number `expected`.  What it reads with get_shared is what the
+// others wrote with put_shared: device-scope stores are acknowledged once they are past the XCD's L2, every wave waits
+// for the acknowledgement of its own before the barrier, and the counter moves behind the barrier.
+__device__ __forceinline__ bool workgroup_arrives_last(uint32_t* ticket, uint32_t expected, uint32_t* lds_word) {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");          // (keeps the compiler from moving stores down)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const uint32_t old = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (old + 1u == expected) put_shared(ticket, 0u);
+        *lds_word = old + 1u == expected ? 1u : 0u;
+    }
+    __syncthreads();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+    return *lds_word != 0u;
+}
+
+// the stretch of `part` among `parts` in n vectors
+struct Stretch {
+    uint32_t lo, hi;
+    __device__ __forceinline__ Stretch(uint32_t n, uint32_t part, uint32_t parts) {
+        const uint32_t per = (n + parts - 1) / parts;
+        lo = part * per < n ? part * per : n;
+        hi = lo + per < n ? lo + per : n;
+    }
+};
+
+SharedRows shared_rows(void* scratch);                         // the three arrays in that memory
+uint32_t row_parts(uint64_t rows, uint32_t vectors);           // how many workgroups take a row
 
 // ---- workgroup reductions: lanes by butterflies, then the waves in order; every thread gets the result ----
 template <int BLOCK, bool ENT>
