@@ -20,6 +20,8 @@ constexpr int kLpBlock = 256;
 constexpr int kLpUnroll = 4;         // vectors a thread keeps in flight
 static_assert(AGRAD_MAX_TOP <= kLpBlock, "a thread an alternative");
 constexpr int kCandidates = 1024;    // candidates of a row's alternatives that LDS holds
+constexpr int kVectors = 384;        // vectors with candidates
+constexpr int kMaxShared = 4096;     // keys that the parts of a row leave
 
 struct LpArgs {
     const int32_t* tokens; float* logp; float* entropy; float* lse; int32_t* top_ids; float* top_logp;
@@ -31,10 +33,12 @@ struct LpArgs {
 // ---- alternatives ------------------------------------------------------------------------------------
 // A class is a 64-bit key: the logit as an integer of the same order above, the complement of the index below; keys
 // are distinct and descend in the order in which alternatives are given.  0 is no class.
-__device__ __forceinline__ uint64_t class_key(float x, uint32_t index) {
+__device__ __forceinline__ uint32_t ordered(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);                   // (-0 ties with 0)
-    const uint32_t ordered = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-    return x > -INFINITY ? ((uint64_t)ordered << 32) | (0xffffffffu - index) : 0ull;       // -inf and NaN: no alternative
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ uint64_t class_key(float x, uint32_t index) {
+    return x > -INFINITY ? ((uint64_t)ordered(x) << 32) | (0xffffffffu - index) : 0ull;       // -inf and NaN: no alternative
 }
 __device__ __forceinline__ float key_logit(uint64_t key) {
     const uint32_t o = (uint32_t)(key >> 32);
@@ -42,27 +46,38 @@ __device__ __forceinline__ float key_logit(uint64_t key) {
 }
 __device__ __forceinline__ uint32_t key_index(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
 
+// What a workgroup finds: vectors with a logit that reaches the bound, then the classes that do.
+template <typename T, int VEC>
 struct Candidates {
     uint64_t key[kCandidates];
-    uint32_t count;
+    typename RawVec<T, VEC>::type raw[kVectors];
+    uint32_t at[kVectors];          // the vector's number
+    uint32_t shares[kLpBlock];
+    uint32_t count, vectors, listed, bound;
 };
 
-// Appends the keys of the lanes that have one.  The places depend on the order in which waves arrive, the set does not.
-__device__ __forceinline__ void append(Candidates& q, bool has, uint64_t key) {
+// A place in a list for each lane that has something for it.  The places depend on the order in which waves arrive, the
+// set does not.
+__device__ __forceinline__ uint32_t take_place(uint32_t& count, bool has) {
     const uint64_t lanes = __ballot(has);
-    if (lanes == 0) return;
+    if (lanes == 0) return 0xffffffffu;
     const uint32_t lane = threadIdx.x % kWave, first = (uint32_t)__builtin_ctzll(lanes);
     uint32_t at = 0;
-    if (lane == first) at = atomicAdd(&q.count, (uint32_t)__popcll(lanes));
-    at = (uint32_t)__shfl((int)at, (int)first) + (uint32_t)__popcll(lanes & ((1ull << lane) - 1));
-    if (has && at < (uint32_t)kCandidates) q.key[at] = key;
+    if (lane == first) at = atomicAdd(&count, (uint32_t)__popcll(lanes));
+    at = (uint32_t)__builtin_amdgcn_readlane((int)at, (int)first);
+    return has ? at + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0u)) : 0xffffffffu;
+}
+template <typename C>
+__device__ __forceinline__ void append(C& q, bool has, uint64_t key) {
+    const uint32_t at = take_place(q.count, has);
+    if (at < (uint32_t)kCandidates) q.key[at] = key;
 }
 
 // Keeps the largest `top` of the candidates, in descending order at the front: a key's place is the number of larger
-// keys, counted (n / BLOCK keys a thread, each against all n: a tenth of the barriers of a sorting network, and faster up to
-// some hundred keys, which is what a row leaves).  All threads call it after a barrier; it ends with one.
-template <int BLOCK, int EACH>
-__device__ __forceinline__ void prune_each(Candidates& q, uint32_t n, uint32_t top) {
+// keys, counted (each key against all n: a tenth of the barriers of a sorting network, and faster up to some hundred
+// keys, which is what a row leaves).  All threads call it after a barrier; it ends with one.
+template <int BLOCK, int EACH, typename C>
+__device__ __forceinline__ void prune_each(C& q, uint32_t n, uint32_t top) {
     uint64_t mine[EACH];
     uint32_t larger[EACH];
 #pragma unroll
@@ -71,11 +86,13 @@ __device__ __forceinline__ void prune_each(Candidates& q, uint32_t n, uint32_t t
         mine[i] = at < n ? q.key[at] : 0ull;
         larger[i] = 0;
     }
+    if (threadIdx.x / kWave * kWave < n) {                       // (waves without a key have nothing to count)
 #pragma unroll 4
-    for (uint32_t j = 0; j < n; ++j) {
-        const uint64_t other = q.key[j];
+        for (uint32_t j = 0; j < n; ++j) {
+            const uint64_t other = q.key[j];
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) larger[i] += other > mine[i] ? 1u : 0u;
+            for (int i = 0; i < EACH; ++i) larger[i] += other > mine[i] ? 1u : 0u;
+        }
     }
     __syncthreads();
 #pragma unroll
@@ -84,35 +101,45 @@ __device__ __forceinline__ void prune_each(Candidates& q, uint32_t n, uint32_t t
     if (threadIdx.x == 0) q.count = n < top ? n : top;
     __syncthreads();
 }
-template <int BLOCK>
-__device__ __forceinline__ void prune(Candidates& q, uint32_t top) {
+template <int BLOCK, typename C>
+__device__ __forceinline__ void prune(C& q, uint32_t top) {
     const uint32_t n = q.count < (uint32_t)kCandidates ? q.count : (uint32_t)kCandidates;
     if (n <= (uint32_t)BLOCK) prune_each<BLOCK, 1>(q, n, top);
     else prune_each<BLOCK, kCandidates / BLOCK>(q, n, top);
 }
 
 // The upper half of a bound that at least `top` of the threads' values reach, as high as such a bound can be; 0 if fewer
-// than `top` threads have a value (0: none).  Every wave finds it for itself, bit by bit, from all values in LDS.
-template <int BLOCK>
-__device__ __forceinline__ uint32_t bound_of(const uint32_t* values, uint32_t top) {
+// than `top` threads have a value (0: none).  One wave finds it bit by bit; it ends with a barrier.
+template <int BLOCK, typename C>
+__device__ __forceinline__ uint32_t bound_of(C& q, uint32_t mine, uint32_t top) {
     constexpr int EACH = BLOCK / kWave;
-    uint32_t v[EACH];
+    q.shares[threadIdx.x] = mine;
+    if (threadIdx.x == 0) q.count = q.vectors = q.listed = 0;
+    __syncthreads();
+    if (threadIdx.x < kWave) {
+        uint32_t v[EACH];
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) v[i] = values[i * kWave + threadIdx.x % kWave] >> 16;
-    uint32_t bound = 0;
-    for (int bit = 15; bit >= 0; --bit) {
-        const uint32_t higher = bound | (1u << bit);
-        uint32_t count = 0;
+        for (int i = 0; i < EACH; ++i) v[i] = q.shares[i * kWave + threadIdx.x] >> 16;
+        uint32_t bound = 0;
 #pragma unroll
-        for (int i = 0; i < EACH; ++i) count += (uint32_t)__popcll(__ballot(v[i] >= higher));
-        if (count >= top) bound = higher;
+        for (int bit = 15; bit >= 0; --bit) {
+            const uint32_t higher = bound | (1u << bit);
+            uint32_t count = 0;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) count += (uint32_t)__popcll(__ballot(v[i] >= higher));
+            if (count >= top) bound = higher;
+        }
+        if (threadIdx.x == 0) q.bound = bound;
     }
-    return bound;
+    __syncthreads();
+    return q.bound;
 }
+// the least logit that reaches it
+__device__ __forceinline__ float bound_logit(uint32_t bound) { return bound == 0 ? -3.4028234663852886e38f : key_logit((uint64_t)bound << 48); }
 
 // The largest of n keys, one a thread and step: right whatever they are, and slow.
-template <int BLOCK, typename KeyAt>
-__device__ __forceinline__ void top_by_steps(uint32_t n, uint32_t top, Candidates& q, KeyAt key_at) {
+template <int BLOCK, typename C, typename KeyAt>
+__device__ __forceinline__ void top_by_steps(uint32_t n, uint32_t top, C& q, KeyAt key_at) {
     if (threadIdx.x == 0) q.count = 0;
     __syncthreads();
     uint64_t floor_key = 0;
@@ -136,56 +163,75 @@ __device__ __forceinline__ void top_by_steps(uint32_t n, uint32_t top, Candidate
 // every thread has seen its share, the vectors whose number is its own modulo BLOCK, and kept the largest logit, `best`.
 // At least `top` classes reach the top-th largest of those BLOCK values, and hardly more do (75 of 151936 for top = 64,
 // 180 for top = 128, as the shares are interleaved), so the row is not read again: only the shares whose largest logit
-// reaches the bound are, by all threads together.  A row whose largest logits crowd into few shares, or are equal in great
-// number, can leave more candidates than LDS holds and goes the slow way.
-template <typename T, int VEC, int BLOCK>
+// reaches the bound are, by all threads together -- or none, where the threads still hold their vectors (HELD; tops:
+// their largest logits).  First whole vectors are picked by their largest logit, then classes among those: a test and a
+// place for every class read again cost more than the row's exponentials (8192 rows of 128256 bf16, top 64: 610 us, with
+// the vectors first 410).  A row whose largest logits crowd into few shares, or are equal in great number, can leave
+// more than LDS holds and goes the slow way.
+template <typename T, int VEC, int BLOCK, bool HELD>
 __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& parts, const Stretch& part, uint32_t top, float best,
-                                        Candidates& q, uint32_t* shares) {
+                                        const typename RawVec<T, VEC>::type (&held)[kLpUnroll], const float (&tops)[kLpUnroll],
+                                        Candidates<T, VEC>& q) {
+    typedef RawVec<T, VEC> Raw;
     const uint32_t extra = part.lo == 0 ? parts.extra : 0u;
     const uint32_t mine = (uint32_t)(class_key(best, 0u) >> 32);
-    shares[threadIdx.x] = mine;
-    if (threadIdx.x == 0) q.count = 0;
-    __syncthreads();
-    const uint32_t bound = bound_of<BLOCK>(shares, top);
-    __syncthreads();
-    // the shares to look at, listed in any order
-    __shared__ uint32_t listed;
-    if (threadIdx.x == 0) listed = 0;
-    __syncthreads();
-    if (mine != 0u && (mine >> 16) >= bound) shares[atomicAdd(&listed, 1u)] = threadIdx.x;
-    __syncthreads();
+    const uint32_t bound = bound_of<BLOCK>(q, mine, top);
+    const float least = bound_logit(bound);
+    const T* body = base + parts.head;
+    auto pick = [&](bool has, uint32_t number, const typename Raw::type& raw) {
+        const uint32_t at = take_place(q.vectors, has);
+        if (at < (uint32_t)kVectors) {
+            q.raw[at] = raw;
+            q.at[at] = number;
+        }
+    };
     if (threadIdx.x < extra) {
         const uint32_t e = parts.extra_at(threadIdx.x);
         float x[1];
         VecIO<T, 1>::load(base + e, x);
-        const uint64_t key = class_key(x[0], e);
-        append(q, key != 0ull && (uint32_t)(key >> 48) >= bound, key);
+        append(q, x[0] >= least, class_key(x[0], e));
     }
-    const uint32_t n = listed, pairs = n * ((part.hi - part.lo + BLOCK - 1) / BLOCK);
-    const T* body = base + parts.head;
-    constexpr int U = 4;
-    for (uint32_t i0 = threadIdx.x; i0 < pairs; i0 += BLOCK * U) {
-        float v[U][VEC];
-        uint32_t vec[U];
+    if constexpr (HELD) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint32_t i = i0 + u * BLOCK, tile = i / n;
-            vec[u] = i < pairs ? part.lo + tile * BLOCK + shares[i - tile * n] : part.hi;
-            if (vec[u] < part.hi) VecIO<T, VEC>::load(body + (uint64_t)vec[u] * VEC, v[u]);
-        }
+        for (int u = 0; u < kLpUnroll; ++u) pick(tops[u] >= least, part.lo + u * BLOCK + threadIdx.x, held[u]);
+    } else {
+        const uint32_t place = take_place(q.listed, mine != 0u && (mine >> 16) >= bound);
+        if (place < (uint32_t)BLOCK) q.shares[place] = threadIdx.x;          // (bound_of has ended with the values)
+        __syncthreads();
+        const uint32_t n = q.listed, pairs = n * ((part.hi - part.lo + BLOCK - 1) / BLOCK);
+        constexpr int U = 4;
+        for (uint32_t i0 = threadIdx.x; i0 < pairs; i0 += BLOCK * U) {
+            typename Raw::type raw[U];
+            uint32_t number[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint32_t e = parts.head + vec[u] * VEC;
-#pragma unroll
-            for (int k = 0; k < VEC; ++k) {
-                const uint64_t key = vec[u] < part.hi ? class_key(v[u][k], e + k) : 0ull;
-                append(q, key != 0ull && (uint32_t)(key >> 48) >= bound, key);
+            for (int u = 0; u < U; ++u) {
+                const uint32_t i = i0 + u * BLOCK, tile = i / n;
+                number[u] = i < pairs ? part.lo + tile * BLOCK + q.shares[i - tile * n] : part.hi;
+                raw[u] = Raw::load(body + (uint64_t)(number[u] < part.hi ? number[u] : part.lo) * VEC);
             }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                float v[VEC];
+                Raw::unpack(raw[u], v);
+                float largest = v[0];
+#pragma unroll
+                for (int k = 1; k < VEC; ++k) largest = fmaxf(largest, v[k]);
+                pick(number[u] < part.hi && largest >= least, number[u], raw[u]);
+            }
+            if (__hip_atomic_load(&q.vectors, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) > (uint32_t)kVectors) break;
         }
-        if (__hip_atomic_load(&q.count, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) > (uint32_t)kCandidates) break;
     }
     __syncthreads();
-    if (q.count > (uint32_t)kCandidates) {
+    const uint32_t picked = q.vectors;
+    const uint32_t classes = picked <= (uint32_t)kVectors ? picked * VEC : 0u;
+    for (uint32_t i = threadIdx.x; i < classes; i += BLOCK) {
+        float x[1];
+        const T one = reinterpret_cast<const T*>(q.raw)[i];
+        RawVec<T, 1>::unpack(one, x);
+        append(q, x[0] >= least, class_key(x[0], parts.head + q.at[i / VEC] * VEC + i % VEC));
+    }
+    __syncthreads();
+    if (picked > (uint32_t)kVectors || q.count > (uint32_t)kCandidates) {
         __syncthreads();
         const uint32_t in_vectors = (part.hi - part.lo) * VEC;
         top_by_steps<BLOCK>(in_vectors + extra, top, q, [&](uint32_t i) {
@@ -199,21 +245,26 @@ __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& p
     }
 }
 
-// ---- forward -----------------------------------------------------------------------------------------
-// the `top` largest of the keys that a row's parts left, descending
-template <int BLOCK>
-__device__ __forceinline__ void join_tops(const unsigned long long* keys, uint32_t n, uint32_t top, Candidates& q, uint32_t* shares) {
+// The `top` largest of the n keys that a row's parts left, descending: key k of part j is at k * parts + j, so that the
+// parts' first keys, among which the row's largest are, fall to different threads.
+template <int BLOCK, typename C>
+__device__ __forceinline__ void join_tops(const unsigned long long* keys, uint32_t n, uint32_t top, C& q) {
+    constexpr int EACH = kMaxShared / BLOCK;
+    uint64_t mine[EACH];
     uint32_t best = 0;
-    for (uint32_t i = threadIdx.x; i < n; i += BLOCK) best = max(best, (uint32_t)(get_shared(keys + i) >> 32));
-    shares[threadIdx.x] = best;
-    if (threadIdx.x == 0) q.count = 0;
-    __syncthreads();
-    const uint32_t bound = bound_of<BLOCK>(shares, top);
-    for (uint32_t i0 = 0; i0 < n; i0 += BLOCK) {
-        const uint32_t i = i0 + threadIdx.x;
-        const uint64_t key = i < n ? get_shared(keys + i) : 0ull;
-        append(q, key != 0ull && (uint32_t)(key >> 48) >= bound, key);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const uint32_t at = threadIdx.x + i * BLOCK;
+        mine[i] = 0;
+        if (i * BLOCK < n) mine[i] = get_shared(keys + (at < n ? at : 0u));
+        if (at >= n) mine[i] = 0;
     }
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) best = max(best, (uint32_t)(mine[i] >> 32));
+    const uint32_t bound = bound_of<BLOCK>(q, best, top);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+        if (i * BLOCK < n) append(q, mine[i] != 0ull && (uint32_t)(mine[i] >> 48) >= bound, mine[i]);
     __syncthreads();
     if (q.count > (uint32_t)kCandidates) {
         __syncthreads();
@@ -223,38 +274,65 @@ __device__ __forceinline__ void join_tops(const unsigned long long* keys, uint32
     }
 }
 
-template <typename T, int VEC, bool ENT>
+// ---- forward -----------------------------------------------------------------------------------------
+// A workgroup reads a row, or a part of it, once, kLpUnroll vectors a thread in flight; with HELD the part is no longer than
+// those, and they stay in registers for the alternatives.
+template <typename T, int VEC, bool ENT, bool HELD>
 __global__ void __launch_bounds__(kLpBlock)
 logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
     __shared__ RowStat lds[kLpBlock / kWave];
-    __shared__ Candidates found;
-    __shared__ uint32_t shares[kLpBlock];
+    __shared__ Candidates<T, VEC> found;
     __shared__ uint32_t word;
+    typedef RawVec<T, VEC> Raw;
     const uint32_t row = blockIdx.x / a.parts, nth = blockIdx.x - row * a.parts;
     const T* base = x + row * a.ld;
     const RowParts<T, VEC> parts(base, a.V);
     const Stretch part(parts.nvec, nth, a.parts);
+    const T* body = base + parts.head;
+    typename Raw::type raw[kLpUnroll];
+    float tops[kLpUnroll];
     RowStat t = empty_stat();
+    auto read = [&](uint32_t i0) {
+#pragma unroll
+        for (int u = 0; u < kLpUnroll; ++u) {
+            const uint32_t i = i0 + u * kLpBlock;
+            raw[u] = Raw::load(body + (uint64_t)(i < part.hi ? i : part.lo) * VEC);
+        }
+    };
+    auto absorb = [&](uint32_t i0) {
+#pragma unroll
+        for (int u = 0; u < kLpUnroll; ++u) {
+            tops[u] = -INFINITY;
+            if (i0 + u * kLpBlock < part.hi) {
+                float v[VEC];
+                Raw::unpack(raw[u], v);
+                tops[u] = absorb_stat<ENT, VEC>(t, v, a.c);
+            }
+        }
+    };
+    uint32_t i0 = part.lo + threadIdx.x;
+    if (HELD && part.lo < part.hi) read(i0);
+    // the token's logit, and the elements outside the vectors
+    const int32_t token = a.tokens != nullptr ? a.tokens[row] : -1;
+    const bool asked = token >= 0 && (uint32_t)token < a.V;
+    float at[1];
+    VecIO<T, 1>::load(base + (asked ? token : 0), at);
     if (nth == 0 && threadIdx.x < parts.extra) {
         float v[1];
         VecIO<T, 1>::load(base + parts.extra_at(threadIdx.x), v);
         absorb_stat<ENT, 1>(t, v, a.c);
     }
-    const T* body = base + parts.head;
-    for (uint32_t i0 = part.lo + threadIdx.x; i0 < part.hi; i0 += kLpBlock * kLpUnroll) {
-        float v[kLpUnroll][VEC];
-#pragma unroll
-        for (int u = 0; u < kLpUnroll; ++u) {
-            const uint32_t i = i0 + u * kLpBlock;
-            if (i < part.hi) VecIO<T, VEC>::load(body + (uint64_t)i * VEC, v[u]);
+    if constexpr (HELD) {
+        absorb(i0);
+    } else {
+        for (; i0 < part.hi; i0 += kLpBlock * kLpUnroll) {
+            read(i0);
+            absorb(i0);
         }
-#pragma unroll
-        for (int u = 0; u < kLpUnroll; ++u)
-            if (i0 + u * kLpBlock < part.hi) absorb_stat<ENT, VEC>(t, v[u], a.c);
     }
     const float best = t.m;
     t = block_stat<kLpBlock, ENT>(t, a.c, lds);
-    if (a.top != 0) row_top<T, VEC, kLpBlock>(base, parts, part, a.top, best, found, shares);
+    if (a.top != 0) row_top<T, VEC, kLpBlock, HELD>(base, parts, part, a.top, best, raw, tops, found);
     if (a.parts > 1) {
         if (threadIdx.x == 0) {
             float* to = a.shared.stats + 4 * (uint64_t)blockIdx.x;
@@ -263,7 +341,8 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
             if (ENT) put_shared(to + 2, t.d);
         }
         unsigned long long* keys = a.shared.keys + (uint64_t)row * a.parts * a.top;
-        if (threadIdx.x < a.top) put_shared(keys + nth * a.top + threadIdx.x, (unsigned long long)(threadIdx.x < found.count ? found.key[threadIdx.x] : 0ull));
+        if (threadIdx.x < a.top)
+            put_shared(keys + threadIdx.x * a.parts + nth, (unsigned long long)(threadIdx.x < found.count ? found.key[threadIdx.x] : 0ull));
         if (!workgroup_arrives_last(a.shared.tickets + row, a.parts, &word)) return;
         t = empty_stat();
         if (threadIdx.x < a.parts) {
@@ -271,7 +350,7 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
             t = RowStat{get_shared(from), get_shared(from + 1), ENT ? get_shared(from + 2) : 0.0f};
         }
         t = block_stat<kLpBlock, ENT>(t, a.c, lds);
-        if (a.top != 0) join_tops<kLpBlock>(keys, a.parts * a.top, a.top, found, shares);
+        if (a.top != 0) join_tops<kLpBlock>(keys, a.parts * a.top, a.top, found);
     }
     const bool empty = t.m == -INFINITY && t.s == 0.0f;
     const float log_s = logf(t.s);                                // -inf for an empty row
@@ -279,16 +358,8 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
         if (a.lse != nullptr) a.lse[row] = empty ? -INFINITY : t.m * a.scale + log_s;
         if (ENT) a.entropy[row] = empty ? 0.0f : log_s - kLn2 * (t.d / t.s);
         if (a.tokens != nullptr) {
-            const int32_t token = a.tokens[row];
-            float lp = 0.0f;
-            if (token >= 0 && (uint32_t)token < a.V) {
-                float at[1];
-                VecIO<T, 1>::load(base + token, at);
-                if (!empty) lp = (at[0] - t.m) * a.scale - log_s;
-            } else if (token != -1) {
-                *a.err_flag = 1;
-            }
-            a.logp[row] = lp;
+            if (!asked && token != -1) *a.err_flag = 1;
+            a.logp[row] = asked && !empty ? (at[0] - t.m) * a.scale - log_s : 0.0f;
         }
     }
     if (threadIdx.x < a.top) {
@@ -369,16 +440,26 @@ logprobs_bwd_kernel(const T* x, T* dx, const LpBwdArgs a, const FastDiv32 chunks
     lp_store<T, VEC>(out + first, v, a.accumulate);
 }
 
+template <typename T, int VEC>
+void lp_fwd_launch(hipStream_t s, const T* x, const LpArgs& a, uint64_t rows) {
+    const dim3 grid((uint32_t)rows * a.parts), block(kLpBlock);
+    const bool held = (a.V / VEC + a.parts - 1) / a.parts <= (uint32_t)kLpBlock * kLpUnroll;
+    if (held && a.entropy) hipLaunchKernelGGL((logprobs_fwd_kernel<T, VEC, true, true>), grid, block, 0, s, x, a);
+    else if (held) hipLaunchKernelGGL((logprobs_fwd_kernel<T, VEC, false, true>), grid, block, 0, s, x, a);
+    else if (a.entropy) hipLaunchKernelGGL((logprobs_fwd_kernel<T, VEC, true, false>), grid, block, 0, s, x, a);
+    else hipLaunchKernelGGL((logprobs_fwd_kernel<T, VEC, false, false>), grid, block, 0, s, x, a);
+}
+
 template <typename T>
 int lp_fwd_typed(hipStream_t s, const T* x, LpArgs a, uint64_t rows) {
     constexpr int WIDE = WideVec<T>::value;
-    const bool wide = a.V >= 4 * WIDE;
-    a.parts = a.shared.tickets != nullptr ? row_parts(rows, a.V / WIDE) : 1u;
-    const dim3 grid((uint32_t)rows * a.parts), block(kLpBlock);
-    if (wide && a.entropy) hipLaunchKernelGGL((logprobs_fwd_kernel<T, WIDE, true>), grid, block, 0, s, x, a);
-    else if (wide) hipLaunchKernelGGL((logprobs_fwd_kernel<T, WIDE, false>), grid, block, 0, s, x, a);
-    else if (a.entropy) hipLaunchKernelGGL((logprobs_fwd_kernel<T, 1, true>), grid, block, 0, s, x, a);
-    else hipLaunchKernelGGL((logprobs_fwd_kernel<T, 1, false>), grid, block, 0, s, x, a);
+    if (a.V >= 4 * WIDE) {
+        a.parts = row_parts(rows, a.V / WIDE);
+        if (a.top != 0 && a.parts * a.top > (uint32_t)kMaxShared) a.parts = kMaxShared / a.top;
+        lp_fwd_launch<T, WIDE>(s, x, a, rows);
+    } else {
+        lp_fwd_launch<T, 1>(s, x, a, rows);
+    }
     return check_hip(hipGetLastError(), "token log probabilities launch");
 }
 

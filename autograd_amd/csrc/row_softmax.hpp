@@ -40,8 +40,9 @@ __device__ __forceinline__ RowStat merge_stat(const RowStat& a, const RowStat& b
 }
 
 // one group of N values into a running part
+// (returns the largest of them, -inf if none is a number)
 template <bool ENT, int N>
-__device__ __forceinline__ void absorb_stat(RowStat& a, const float (&v)[N], float c) {
+__device__ __forceinline__ float absorb_stat(RowStat& a, const float (&v)[N], float c) {
     float top = v[0];
 #pragma unroll
     for (int k = 1; k < N; ++k) top = fmaxf(top, v[k]);
@@ -50,7 +51,7 @@ __device__ __forceinline__ void absorb_stat(RowStat& a, const float (&v)[N], flo
 #pragma unroll
         for (int k = 0; k < N; ++k)
             if (v[k] != v[k]) a.s = v[k];
-        return;
+        return -INFINITY;
     }
 #pragma unroll
     for (int k = 0; k < N; ++k) {
@@ -59,6 +60,7 @@ __device__ __forceinline__ void absorb_stat(RowStat& a, const float (&v)[N], flo
         a.s = a.s + e;
         if constexpr (ENT) a.d = __builtin_fmaf(e, fmaxf(t, -200.0f), a.d);       // (-inf: 0 * -200)
     }
+    return top;
 }
 
 // how a row of V elements that starts at `base` splits into single elements, aligned vectors, single elements
@@ -130,14 +132,25 @@ struct Stretch {
 SharedRows shared_rows(void* scratch);                         // the three arrays in that memory
 uint32_t row_parts(uint64_t rows, uint32_t vectors);           // how many workgroups take a row
 
-// ---- workgroup reductions: lanes by butterflies, then the waves in order; every thread gets the result ----
+// ---- workgroup reductions: the lanes of a wave, then the waves in order; every thread gets the result ----
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, dpp_move<kDppQuadXor1>(v));
+    v = fmaxf(v, dpp_move<kDppQuadXor2>(v));
+    v = fmaxf(v, dpp_move<kDppRowHalfMirror>(v));
+    v = fmaxf(v, dpp_move<kDppRowMirror>(v));
+    v = fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), kSwizzleXor16)));
+    const float lo = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 0));
+    const float hi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 32));
+    return fmaxf(lo, hi);
+}
+
+// The maximum first, then one rescaling a thread and plain sums: a merge of two parts in each of six steps costs twelve
+// exponentials.
 template <int BLOCK, bool ENT>
 __device__ __forceinline__ RowStat block_stat(RowStat a, float c, RowStat* lds) {
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-        RowStat o{__shfl_xor(a.m, off), __shfl_xor(a.s, off), ENT ? __shfl_xor(a.d, off) : 0.0f};
-        a = merge_stat<ENT>(a, o, c);
-    }
+    a = about<ENT>(a, wave_max(a.m), c);
+    if constexpr (ENT) wave_sum2(a.s, a.d);
+    else a.s = wave_sum(a.s);
     if constexpr (BLOCK == kWave) return a;
     if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = a;
     __syncthreads();
