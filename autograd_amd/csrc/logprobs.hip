@@ -11,6 +11,7 @@
 #include "row_softmax.hpp"
 
 #include <cmath>
+#include <type_traits>
 
 namespace agrad {
 
@@ -20,7 +21,10 @@ constexpr int kLpBlock = 256;
 constexpr int kLpUnroll = 4;         // vectors a thread keeps in flight
 static_assert(AGRAD_MAX_TOP <= kLpBlock, "a thread an alternative");
 constexpr int kCandidates = 1024;    // candidates of a row's alternatives that LDS holds
-constexpr int kVectors = 384;        // vectors with candidates
+constexpr int kLine = 8;             // vectors of a line
+constexpr int kLines = 8192;         // lines that LDS holds
+constexpr int kListed = 512;         // lines with candidates
+struct Nothing {};
 constexpr int kMaxShared = 4096;     // keys that the parts of a row leave
 
 struct LpArgs {
@@ -46,14 +50,16 @@ __device__ __forceinline__ float key_logit(uint64_t key) {
 }
 __device__ __forceinline__ uint32_t key_index(uint64_t key) { return 0xffffffffu - (uint32_t)key; }
 
-// What a workgroup finds: vectors with a logit that reaches the bound, then the classes that do.
-template <typename T, int VEC>
+// What a workgroup finds.  A line is kLine neighbouring vectors (128 bytes); of each the row's one pass leaves the upper half
+// of its largest logit, which is done with before the first key is written.
 struct Candidates {
-    uint64_t key[kCandidates];
-    typename RawVec<T, VEC>::type raw[kVectors];
-    uint32_t at[kVectors];          // the vector's number
+    union {
+        uint64_t key[kCandidates];
+        uint16_t line[kLines];
+    };
+    uint32_t list[kListed];         // lines that hold candidates
     uint32_t shares[kLpBlock];
-    uint32_t count, vectors, listed, bound;
+    uint32_t count, listed, bound;
 };
 
 // A place in a list for each lane that has something for it.  The places depend on the order in which waves arrive, the
@@ -67,8 +73,7 @@ __device__ __forceinline__ uint32_t take_place(uint32_t& count, bool has) {
     at = (uint32_t)__builtin_amdgcn_readlane((int)at, (int)first);
     return has ? at + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0u)) : 0xffffffffu;
 }
-template <typename C>
-__device__ __forceinline__ void append(C& q, bool has, uint64_t key) {
+__device__ __forceinline__ void append(Candidates& q, bool has, uint64_t key) {
     const uint32_t at = take_place(q.count, has);
     if (at < (uint32_t)kCandidates) q.key[at] = key;
 }
@@ -76,8 +81,8 @@ __device__ __forceinline__ void append(C& q, bool has, uint64_t key) {
 // Keeps the largest `top` of the candidates, in descending order at the front: a key's place is the number of larger
 // keys, counted (each key against all n: a tenth of the barriers of a sorting network, and faster up to some hundred
 // keys, which is what a row leaves).  All threads call it after a barrier; it ends with one.
-template <int BLOCK, int EACH, typename C>
-__device__ __forceinline__ void prune_each(C& q, uint32_t n, uint32_t top) {
+template <int BLOCK, int EACH>
+__device__ __forceinline__ void prune_each(Candidates& q, uint32_t n, uint32_t top) {
     uint64_t mine[EACH];
     uint32_t larger[EACH];
 #pragma unroll
@@ -101,8 +106,8 @@ __device__ __forceinline__ void prune_each(C& q, uint32_t n, uint32_t top) {
     if (threadIdx.x == 0) q.count = n < top ? n : top;
     __syncthreads();
 }
-template <int BLOCK, typename C>
-__device__ __forceinline__ void prune(C& q, uint32_t top) {
+template <int BLOCK>
+__device__ __forceinline__ void prune(Candidates& q, uint32_t top) {
     const uint32_t n = q.count < (uint32_t)kCandidates ? q.count : (uint32_t)kCandidates;
     if (n <= (uint32_t)BLOCK) prune_each<BLOCK, 1>(q, n, top);
     else prune_each<BLOCK, kCandidates / BLOCK>(q, n, top);
@@ -110,11 +115,11 @@ __device__ __forceinline__ void prune(C& q, uint32_t top) {
 
 // The upper half of a bound that at least `top` of the threads' values reach, as high as such a bound can be; 0 if fewer
 // than `top` threads have a value (0: none).  One wave finds it bit by bit; it ends with a barrier.
-template <int BLOCK, typename C>
-__device__ __forceinline__ uint32_t bound_of(C& q, uint32_t mine, uint32_t top) {
+template <int BLOCK>
+__device__ __forceinline__ uint32_t bound_of(Candidates& q, uint32_t mine, uint32_t top) {
     constexpr int EACH = BLOCK / kWave;
     q.shares[threadIdx.x] = mine;
-    if (threadIdx.x == 0) q.count = q.vectors = q.listed = 0;
+    if (threadIdx.x == 0) q.count = q.listed = 0;
     __syncthreads();
     if (threadIdx.x < kWave) {
         uint32_t v[EACH];
@@ -134,12 +139,17 @@ __device__ __forceinline__ uint32_t bound_of(C& q, uint32_t mine, uint32_t top) 
     __syncthreads();
     return q.bound;
 }
-// the least logit that reaches it
-__device__ __forceinline__ float bound_logit(uint32_t bound) { return bound == 0 ? -3.4028234663852886e38f : key_logit((uint64_t)bound << 48); }
+// A logit that every class reaching the bound has at least, with few others: all that is more than -inf, for 0; next to
+// zero, where the numbers below it share an upper half with -0, a little less than the bound.
+__device__ __forceinline__ float bound_logit(uint32_t bound) {
+    return bound == 0 ? -3.4028234663852886e38f : bound == 0x8000u ? -1.2e-38f : key_logit((uint64_t)bound << 48);
+}
+// the order of the upper halves of fp32 numbers (-0 with 0)
+__device__ __forceinline__ uint32_t ordered_half(uint32_t h) { return (h & 0x8000u) && h != 0x8000u ? ~h & 0xffffu : h | 0x8000u; }
 
 // The largest of n keys, one a thread and step: right whatever they are, and slow.
-template <int BLOCK, typename C, typename KeyAt>
-__device__ __forceinline__ void top_by_steps(uint32_t n, uint32_t top, C& q, KeyAt key_at) {
+template <int BLOCK, typename KeyAt>
+__device__ __forceinline__ void top_by_steps(uint32_t n, uint32_t top, Candidates& q, KeyAt key_at) {
     if (threadIdx.x == 0) q.count = 0;
     __syncthreads();
     uint64_t floor_key = 0;
@@ -162,78 +172,73 @@ __device__ __forceinline__ void top_by_steps(uint32_t n, uint32_t top, C& q, Key
 // The alternatives of a stretch of a row's vectors (the first stretch: and of the elements outside the vectors) of which
 // every thread has seen its share, the vectors whose number is its own modulo BLOCK, and kept the largest logit, `best`.
 // At least `top` classes reach the top-th largest of those BLOCK values, and hardly more do (75 of 151936 for top = 64,
-// 180 for top = 128, as the shares are interleaved), so the row is not read again: only the shares whose largest logit
-// reaches the bound are, by all threads together -- or none, where the threads still hold their vectors (HELD; tops:
-// their largest logits).  First whole vectors are picked by their largest logit, then classes among those: a test and a
-// place for every class read again cost more than the row's exponentials (8192 rows of 128256 bf16, top 64: 610 us, with
-// the vectors first 410).  A row whose largest logits crowd into few shares, or are equal in great number, can leave
-// more than LDS holds and goes the slow way.
+// 180 for top = 128, as the shares are interleaved).  With them known, the row is not read again but for the lines whose
+// largest logit reaches the bound -- or not at all, where the threads still hold their vectors (HELD; tops: their largest
+// logits).  (Reading the shares again instead of lines reads the whole row: eight threads have a part in each 128 bytes.
+// 8192 rows of 128256 bf16, top 64: 595 us.)  A row whose largest logits are equal in great number, or crowd into few
+// shares, can leave more than LDS holds and goes the slow way.
 template <typename T, int VEC, int BLOCK, bool HELD>
 __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& parts, const Stretch& part, uint32_t top, float best,
                                         const typename RawVec<T, VEC>::type (&held)[kLpUnroll], const float (&tops)[kLpUnroll],
-                                        Candidates<T, VEC>& q) {
+                                        Candidates& q) {
     typedef RawVec<T, VEC> Raw;
-    const uint32_t extra = part.lo == 0 ? parts.extra : 0u;
-    const uint32_t mine = (uint32_t)(class_key(best, 0u) >> 32);
-    const uint32_t bound = bound_of<BLOCK>(q, mine, top);
+    const uint32_t extra = part.lo == 0 ? parts.extra : 0u, vectors = part.hi - part.lo;
+    const uint32_t bound = bound_of<BLOCK>(q, (uint32_t)(class_key(best, 0u) >> 32), top);
     const float least = bound_logit(bound);
     const T* body = base + parts.head;
-    auto pick = [&](bool has, uint32_t number, const typename Raw::type& raw) {
-        const uint32_t at = take_place(q.vectors, has);
-        if (at < (uint32_t)kVectors) {
-            q.raw[at] = raw;
-            q.at[at] = number;
-        }
+    bool fits = true;
+    auto append_vector = [&](bool has, uint32_t number, const typename Raw::type& raw) {
+        float v[VEC];
+        Raw::unpack(raw, v);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) append(q, has && v[k] >= least, class_key(v[k], parts.head + number * VEC + k));
     };
+    if constexpr (HELD) {
+#pragma unroll
+        for (int u = 0; u < kLpUnroll; ++u)
+            if (__ballot(tops[u] >= least) != 0) append_vector(tops[u] >= least, part.lo + u * BLOCK + threadIdx.x, held[u]);
+    } else {
+        const uint32_t all_lines = (vectors + kLine - 1) / kLine, lines = all_lines <= (uint32_t)kLines ? all_lines : 0u;
+        const uint32_t from = bound < 0x80u ? 0x80u : bound;                 // (-inf is 0x7f)
+        for (uint32_t j0 = 0; j0 < lines; j0 += BLOCK * 8) {
+            const uint32_t j = j0 + threadIdx.x * 8;
+            u32x4 w = *reinterpret_cast<const u32x4*>(q.line + (j < lines ? j : 0u));
+            const uint32_t pair[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t h = k % 2 ? pair[k / 2] >> 16 : pair[k / 2] & 0xffffu;
+                const uint32_t at = take_place(q.listed, j + k < lines && ordered_half(h) >= from);
+                if (at < (uint32_t)kListed) q.list[at] = j + k;
+            }
+        }
+        __syncthreads();
+        const uint32_t n = q.listed;
+        fits = n <= (uint32_t)kListed && lines == all_lines;
+        const uint32_t again = fits ? n * kLine : 0u;
+        constexpr int U = 2;
+        for (uint32_t i0 = threadIdx.x; i0 / kWave * kWave < again; i0 += BLOCK * U) {
+            typename Raw::type raw[U];
+            uint32_t number[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t i = i0 + u * BLOCK;
+                number[u] = i < again ? q.list[i / kLine] * kLine + i % kLine : vectors;
+                raw[u] = Raw::load(body + (uint64_t)(part.lo + (number[u] < vectors ? number[u] : 0u)) * VEC);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) append_vector(number[u] < vectors, part.lo + number[u], raw[u]);
+        }
+    }
     if (threadIdx.x < extra) {
         const uint32_t e = parts.extra_at(threadIdx.x);
         float x[1];
         VecIO<T, 1>::load(base + e, x);
         append(q, x[0] >= least, class_key(x[0], e));
     }
-    if constexpr (HELD) {
-#pragma unroll
-        for (int u = 0; u < kLpUnroll; ++u) pick(tops[u] >= least, part.lo + u * BLOCK + threadIdx.x, held[u]);
-    } else {
-        const uint32_t place = take_place(q.listed, mine != 0u && (mine >> 16) >= bound);
-        if (place < (uint32_t)BLOCK) q.shares[place] = threadIdx.x;          // (bound_of has ended with the values)
-        __syncthreads();
-        const uint32_t n = q.listed, pairs = n * ((part.hi - part.lo + BLOCK - 1) / BLOCK);
-        constexpr int U = 4;
-        for (uint32_t i0 = threadIdx.x; i0 < pairs; i0 += BLOCK * U) {
-            typename Raw::type raw[U];
-            uint32_t number[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const uint32_t i = i0 + u * BLOCK, tile = i / n;
-                number[u] = i < pairs ? part.lo + tile * BLOCK + q.shares[i - tile * n] : part.hi;
-                raw[u] = Raw::load(body + (uint64_t)(number[u] < part.hi ? number[u] : part.lo) * VEC);
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                float v[VEC];
-                Raw::unpack(raw[u], v);
-                float largest = v[0];
-#pragma unroll
-                for (int k = 1; k < VEC; ++k) largest = fmaxf(largest, v[k]);
-                pick(number[u] < part.hi && largest >= least, number[u], raw[u]);
-            }
-            if (__hip_atomic_load(&q.vectors, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) > (uint32_t)kVectors) break;
-        }
-    }
     __syncthreads();
-    const uint32_t picked = q.vectors;
-    const uint32_t classes = picked <= (uint32_t)kVectors ? picked * VEC : 0u;
-    for (uint32_t i = threadIdx.x; i < classes; i += BLOCK) {
-        float x[1];
-        const T one = reinterpret_cast<const T*>(q.raw)[i];
-        RawVec<T, 1>::unpack(one, x);
-        append(q, x[0] >= least, class_key(x[0], parts.head + q.at[i / VEC] * VEC + i % VEC));
-    }
-    __syncthreads();
-    if (picked > (uint32_t)kVectors || q.count > (uint32_t)kCandidates) {
+    if (!fits || q.count > (uint32_t)kCandidates) {
         __syncthreads();
-        const uint32_t in_vectors = (part.hi - part.lo) * VEC;
+        const uint32_t in_vectors = vectors * VEC;
         top_by_steps<BLOCK>(in_vectors + extra, top, q, [&](uint32_t i) {
             const uint32_t e = i < in_vectors ? parts.head + part.lo * VEC + i : parts.extra_at(i - in_vectors);
             float x[1];
@@ -247,8 +252,8 @@ __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& p
 
 // The `top` largest of the n keys that a row's parts left, descending: key k of part j is at k * parts + j, so that the
 // parts' first keys, among which the row's largest are, fall to different threads.
-template <int BLOCK, typename C>
-__device__ __forceinline__ void join_tops(const unsigned long long* keys, uint32_t n, uint32_t top, C& q) {
+template <int BLOCK>
+__device__ __forceinline__ void join_tops(const unsigned long long* keys, uint32_t n, uint32_t top, Candidates& q) {
     constexpr int EACH = kMaxShared / BLOCK;
     uint64_t mine[EACH];
     uint32_t best = 0;
@@ -275,13 +280,14 @@ __device__ __forceinline__ void join_tops(const unsigned long long* keys, uint32
 }
 
 // ---- forward -----------------------------------------------------------------------------------------
-// A workgroup reads a row, or a part of it, once, kLpUnroll vectors a thread in flight; with HELD the part is no longer than
-// those, and they stay in registers for the alternatives.
-template <typename T, int VEC, bool ENT, bool HELD>
+// A workgroup reads a row, or a part of it, once, kLpUnroll vectors a thread in flight.  With HELD the part is no longer than
+// those, and they stay in registers for the alternatives; with LINES the pass leaves every line's largest logit for them.
+enum LpMode { PLAIN, LINES, HELD };
+template <typename T, int VEC, bool ENT, LpMode MODE>
 __global__ void __launch_bounds__(kLpBlock)
 logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
     __shared__ RowStat lds[kLpBlock / kWave];
-    __shared__ Candidates<T, VEC> found;
+    __shared__ std::conditional_t<MODE == PLAIN, Nothing, Candidates> found;
     __shared__ uint32_t word;
     typedef RawVec<T, VEC> Raw;
     const uint32_t row = blockIdx.x / a.parts, nth = blockIdx.x - row * a.parts;
@@ -310,8 +316,7 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
             }
         }
     };
-    uint32_t i0 = part.lo + threadIdx.x;
-    if (HELD && part.lo < part.hi) read(i0);
+    if (MODE == HELD && part.lo < part.hi) read(part.lo + threadIdx.x);
     // the token's logit, and the elements outside the vectors
     const int32_t token = a.tokens != nullptr ? a.tokens[row] : -1;
     const bool asked = token >= 0 && (uint32_t)token < a.V;
@@ -322,17 +327,29 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
         VecIO<T, 1>::load(base + parts.extra_at(threadIdx.x), v);
         absorb_stat<ENT, 1>(t, v, a.c);
     }
-    if constexpr (HELD) {
-        absorb(i0);
+    if constexpr (MODE == HELD) {
+        absorb(part.lo + threadIdx.x);
     } else {
-        for (; i0 < part.hi; i0 += kLpBlock * kLpUnroll) {
-            read(i0);
-            absorb(i0);
+        for (uint32_t i0 = part.lo; i0 < part.hi; i0 += kLpBlock * kLpUnroll) {       // (the same for all lanes)
+            read(i0 + threadIdx.x);
+            absorb(i0 + threadIdx.x);
+            if constexpr (MODE == LINES) {
+                static_assert(kLine == 8, "the lanes of half a DPP row");
+#pragma unroll
+                for (int u = 0; u < kLpUnroll; ++u) {
+                    float m = fmaxf(tops[u], dpp_move<kDppQuadXor1>(tops[u]));
+                    m = fmaxf(m, dpp_move<kDppQuadXor2>(m));
+                    m = fmaxf(m, dpp_move<kDppRowHalfMirror>(m));
+                    const uint32_t line = (i0 - part.lo + u * kLpBlock + threadIdx.x) / kLine;
+                    if (threadIdx.x % kLine == 0 && line < (uint32_t)kLines) found.line[line] = (uint16_t)(__float_as_uint(m) >> 16);
+                }
+            }
         }
     }
     const float best = t.m;
     t = block_stat<kLpBlock, ENT>(t, a.c, lds);
-    if (a.top != 0) row_top<T, VEC, kLpBlock, HELD>(base, parts, part, a.top, best, raw, tops, found);
+    if constexpr (MODE != PLAIN)
+        if (a.top != 0) row_top<T, VEC, kLpBlock, MODE == HELD>(base, parts, part, a.top, best, raw, tops, found);
     if (a.parts > 1) {
         if (threadIdx.x == 0) {
             float* to = a.shared.stats + 4 * (uint64_t)blockIdx.x;
@@ -341,8 +358,9 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
             if (ENT) put_shared(to + 2, t.d);
         }
         unsigned long long* keys = a.shared.keys + (uint64_t)row * a.parts * a.top;
-        if (threadIdx.x < a.top)
-            put_shared(keys + threadIdx.x * a.parts + nth, (unsigned long long)(threadIdx.x < found.count ? found.key[threadIdx.x] : 0ull));
+        if constexpr (MODE != PLAIN)
+            if (threadIdx.x < a.top)
+                put_shared(keys + threadIdx.x * a.parts + nth, (unsigned long long)(threadIdx.x < found.count ? found.key[threadIdx.x] : 0ull));
         if (!workgroup_arrives_last(a.shared.tickets + row, a.parts, &word)) return;
         t = empty_stat();
         if (threadIdx.x < a.parts) {
@@ -350,7 +368,8 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
             t = RowStat{get_shared(from), get_shared(from + 1), ENT ? get_shared(from + 2) : 0.0f};
         }
         t = block_stat<kLpBlock, ENT>(t, a.c, lds);
-        if (a.top != 0) join_tops<kLpBlock>(keys, a.parts * a.top, a.top, found);
+        if constexpr (MODE != PLAIN)
+            if (a.top != 0) join_tops<kLpBlock>(keys, a.parts * a.top, a.top, found);
     }
     const bool empty = t.m == -INFINITY && t.s == 0.0f;
     const float log_s = logf(t.s);                                // -inf for an empty row
@@ -362,7 +381,8 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
             a.logp[row] = asked && !empty ? (at[0] - t.m) * a.scale - log_s : 0.0f;
         }
     }
-    if (threadIdx.x < a.top) {
+    if constexpr (MODE != PLAIN) {
+        if (threadIdx.x >= a.top) return;
         const bool there = threadIdx.x < found.count;
         const uint64_t key = there ? found.key[threadIdx.x] : 0ull;
         const uint64_t to = (uint64_t)row * a.top + threadIdx.x;
@@ -440,25 +460,45 @@ logprobs_bwd_kernel(const T* x, T* dx, const LpBwdArgs a, const FastDiv32 chunks
     lp_store<T, VEC>(out + first, v, a.accumulate);
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, LpMode MODE>
 void lp_fwd_launch(hipStream_t s, const T* x, const LpArgs& a, uint64_t rows) {
     const dim3 grid((uint32_t)rows * a.parts), block(kLpBlock);
-    const bool held = (a.V / VEC + a.parts - 1) / a.parts <= (uint32_t)kLpBlock * kLpUnroll;
-    if (held && a.entropy) hipLaunchKernelGGL((logprobs_fwd_kernel<T, VEC, true, true>), grid, block, 0, s, x, a);
-    else if (held) hipLaunchKernelGGL((logprobs_fwd_kernel<T, VEC, false, true>), grid, block, 0, s, x, a);
-    else if (a.entropy) hipLaunchKernelGGL((logprobs_fwd_kernel<T, VEC, true, false>), grid, block, 0, s, x, a);
-    else hipLaunchKernelGGL((logprobs_fwd_kernel<T, VEC, false, false>), grid, block, 0, s, x, a);
+    if (a.entropy) hipLaunchKernelGGL((logprobs_fwd_kernel<T, VEC, true, MODE>), grid, block, 0, s, x, a);
+    else hipLaunchKernelGGL((logprobs_fwd_kernel<T, VEC, false, MODE>), grid, block, 0, s, x, a);
 }
 
 template <typename T>
 int lp_fwd_typed(hipStream_t s, const T* x, LpArgs a, uint64_t rows) {
     constexpr int WIDE = WideVec<T>::value;
-    if (a.V >= 4 * WIDE) {
-        a.parts = row_parts(rows, a.V / WIDE);
-        if (a.top != 0 && a.parts * a.top > (uint32_t)kMaxShared) a.parts = kMaxShared / a.top;
-        lp_fwd_launch<T, WIDE>(s, x, a, rows);
-    } else {
-        lp_fwd_launch<T, 1>(s, x, a, rows);
+    if (a.V < 4 * WIDE) {
+        lp_fwd_launch<T, 1, HELD>(s, x, a, rows);
+        return check_hip(hipGetLastError(), "token log probabilities launch");
+    }
+    const uint32_t vectors = a.V / WIDE;
+    a.parts = row_parts(rows, vectors);
+    uint64_t slab = rows;
+    if (a.top != 0) {
+        if (a.parts * a.top > (uint32_t)kMaxShared) a.parts = kMaxShared / a.top;
+        // a part's lines have to fit LDS: rows of more than kLines lines are cut, so many rows a launch as the parts' memory takes
+        const uint32_t least = vectors / (uint32_t)(kLines * kLine) + 1;
+        if (least > a.parts) {
+            a.parts = least < kMaxShared / a.top ? least : kMaxShared / a.top;
+            if (a.parts > kMaxParts) a.parts = kMaxParts;
+            slab = kSharedParts / a.parts;
+        }
+    }
+    const bool held = (vectors + a.parts - 1) / a.parts <= (uint32_t)kLpBlock * kLpUnroll;
+    for (uint64_t r0 = 0; r0 < rows; r0 += slab) {
+        const uint64_t n = rows - r0 < slab ? rows - r0 : slab;
+        LpArgs b = a;
+        if (b.tokens) { b.tokens += r0; b.logp += r0; }
+        if (b.entropy) b.entropy += r0;
+        if (b.lse) b.lse += r0;
+        if (b.top) { b.top_ids += r0 * b.top; b.top_logp += r0 * b.top; }
+        const T* from = x + r0 * a.ld;
+        if (held) lp_fwd_launch<T, WIDE, HELD>(s, from, b, n);
+        else if (a.top != 0) lp_fwd_launch<T, WIDE, LINES>(s, from, b, n);
+        else lp_fwd_launch<T, WIDE, PLAIN>(s, from, b, n);
     }
     return check_hip(hipGetLastError(), "token log probabilities launch");
 }
