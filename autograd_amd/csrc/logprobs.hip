@@ -73,6 +73,20 @@ __device__ __forceinline__ uint32_t take_place(uint32_t& count, bool has) {
     at = (uint32_t)__builtin_amdgcn_readlane((int)at, (int)first);
     return has ? at + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0u)) : 0xffffffffu;
 }
+// The same for several of a lane's, at most 15: the first of its places.  All lanes of the wave take part.
+__device__ __forceinline__ uint32_t take_places(uint32_t& count, uint32_t mine) {
+    uint32_t before = 0, total = 0;
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        const uint64_t lanes = __ballot((mine >> b) & 1u);
+        before += __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0u)) << b;
+        total += (uint32_t)__popcll(lanes) << b;
+    }
+    if (total == 0) return 0;
+    uint32_t at = 0;
+    if (threadIdx.x % kWave == 0) at = atomicAdd(&count, total);
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + before;
+}
 __device__ __forceinline__ void append(Candidates& q, bool has, uint64_t key) {
     const uint32_t at = take_place(q.count, has);
     if (at < (uint32_t)kCandidates) q.key[at] = key;
@@ -190,8 +204,17 @@ __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& p
     auto append_vector = [&](bool has, uint32_t number, const typename Raw::type& raw) {
         float v[VEC];
         Raw::unpack(raw, v);
+        uint32_t mine = 0;
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) append(q, has && v[k] >= least, class_key(v[k], parts.head + number * VEC + k));
+        for (int k = 0; k < VEC; ++k) mine += has && v[k] >= least ? 1u : 0u;
+        uint32_t at = take_places(q.count, mine);
+        if (mine == 0) return;
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) {
+            if (!(v[k] >= least)) continue;
+            if (at < (uint32_t)kCandidates) q.key[at] = class_key(v[k], parts.head + number * VEC + k);
+            ++at;
+        }
     };
     if constexpr (HELD) {
 #pragma unroll
@@ -204,12 +227,15 @@ __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& p
             const uint32_t j = j0 + threadIdx.x * 8;
             u32x4 w = *reinterpret_cast<const u32x4*>(q.line + (j < lines ? j : 0u));
             const uint32_t pair[4] = {w.x, w.y, w.z, w.w};
+            uint32_t reach = 0;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const uint32_t h = k % 2 ? pair[k / 2] >> 16 : pair[k / 2] & 0xffffu;
-                const uint32_t at = take_place(q.listed, j + k < lines && ordered_half(h) >= from);
-                if (at < (uint32_t)kListed) q.list[at] = j + k;
+                if (j + k < lines && ordered_half(h) >= from) reach |= 1u << k;
             }
+            uint32_t at = take_places(q.listed, (uint32_t)__popc(reach));
+            for (; reach != 0; reach &= reach - 1u, ++at)
+                if (at < (uint32_t)kListed) q.list[at] = j + (uint32_t)__builtin_ctz(reach);
         }
         __syncthreads();
         const uint32_t n = q.listed;
@@ -330,9 +356,10 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
     if constexpr (MODE == HELD) {
         absorb(part.lo + threadIdx.x);
     } else {
-        for (uint32_t i0 = part.lo; i0 < part.hi; i0 += kLpBlock * kLpUnroll) {       // (the same for all lanes)
-            read(i0 + threadIdx.x);
-            absorb(i0 + threadIdx.x);
+        const uint32_t lane = threadIdx.x % kWave;
+        for (uint32_t i0 = part.lo + (threadIdx.x - lane); i0 < part.hi; i0 += kLpBlock * kLpUnroll) {     // (whole waves)
+            read(i0 + lane);
+            absorb(i0 + lane);
             if constexpr (MODE == LINES) {
                 static_assert(kLine == 8, "the lanes of half a DPP row");
 #pragma unroll
@@ -340,8 +367,8 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
                     float m = fmaxf(tops[u], dpp_move<kDppQuadXor1>(tops[u]));
                     m = fmaxf(m, dpp_move<kDppQuadXor2>(m));
                     m = fmaxf(m, dpp_move<kDppRowHalfMirror>(m));
-                    const uint32_t line = (i0 - part.lo + u * kLpBlock + threadIdx.x) / kLine;
-                    if (threadIdx.x % kLine == 0 && line < (uint32_t)kLines) found.line[line] = (uint16_t)(__float_as_uint(m) >> 16);
+                    const uint32_t line = (i0 - part.lo + u * kLpBlock + lane) / kLine;
+                    if (lane % kLine == 0 && line < (uint32_t)kLines) found.line[line] = (uint16_t)(__float_as_uint(m) >> 16);
                 }
             }
         }
