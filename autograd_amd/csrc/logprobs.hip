@@ -54,10 +54,13 @@ __device__ __forceinline__ uint32_t key_index(uint64_t key) { return 0xffffffffu
 // of its largest logit, which is done with before the first key is written.
 struct Candidates {
     union {
-        uint64_t key[kCandidates];
+        struct {
+            uint64_t key[kCandidates];
+            u32x4 raw[kListed];     // vectors that hold candidates (of threads that kept theirs)
+        };
         uint16_t line[kLines];
     };
-    uint32_t list[kListed];         // lines that hold candidates
+    uint32_t list[kListed];         // lines, or those vectors, that hold candidates
     uint32_t shares[kLpBlock];
     uint32_t count, listed, bound;
 };
@@ -106,7 +109,7 @@ __device__ __forceinline__ void prune_each(Candidates& q, uint32_t n, uint32_t t
         larger[i] = 0;
     }
     if (threadIdx.x / kWave * kWave < n) {                       // (waves without a key have nothing to count)
-#pragma unroll 4
+#pragma unroll 8
         for (uint32_t j = 0; j < n; ++j) {
             const uint64_t other = q.key[j];
 #pragma unroll
@@ -128,9 +131,11 @@ __device__ __forceinline__ void prune(Candidates& q, uint32_t top) {
 }
 
 // The upper half of a bound that at least `top` of the threads' values reach, as high as such a bound can be; 0 if fewer
-// than `top` threads have a value (0: none).  One wave finds it bit by bit; it ends with a barrier.
+// than `top` threads have a value (0: none).  highest: the upper half of the largest.  One wave finds it, two bits at a time,
+// among the 256 halves up to the highest -- two octaves of the logit -- or, where that is not enough, bit by bit among
+// all; it ends with a barrier.
 template <int BLOCK>
-__device__ __forceinline__ uint32_t bound_of(Candidates& q, uint32_t mine, uint32_t top) {
+__device__ __forceinline__ uint32_t bound_of(Candidates& q, uint32_t mine, uint32_t highest, uint32_t top) {
     constexpr int EACH = BLOCK / kWave;
     q.shares[threadIdx.x] = mine;
     if (threadIdx.x == 0) q.count = q.listed = 0;
@@ -139,14 +144,24 @@ __device__ __forceinline__ uint32_t bound_of(Candidates& q, uint32_t mine, uint3
         uint32_t v[EACH];
 #pragma unroll
         for (int i = 0; i < EACH; ++i) v[i] = q.shares[i * kWave + threadIdx.x] >> 16;
-        uint32_t bound = 0;
-#pragma unroll
-        for (int bit = 15; bit >= 0; --bit) {
-            const uint32_t higher = bound | (1u << bit);
+        auto enough = [&](uint32_t from) {
             uint32_t count = 0;
 #pragma unroll
-            for (int i = 0; i < EACH; ++i) count += (uint32_t)__popcll(__ballot(v[i] >= higher));
-            if (count >= top) bound = higher;
+            for (int i = 0; i < EACH; ++i) count += (uint32_t)__popcll(__ballot(v[i] >= from));
+            return count >= top;
+        };
+        uint32_t bound = highest > 0x80u + 255u ? highest - 255u : 0x80u;
+        if (enough(bound)) {
+#pragma unroll
+            for (int bit = 6; bit >= 0; bit -= 2) {
+                const uint32_t one = 1u << bit;
+                const bool a = enough(bound + one), b = enough(bound + 2 * one), c = enough(bound + 3 * one);
+                bound += (a ? one : 0u) + (b ? one : 0u) + (c ? one : 0u);
+            }
+        } else {
+            bound = 0;
+            for (int bit = 15; bit >= 0; --bit)
+                if (enough(bound | (1u << bit))) bound |= 1u << bit;
         }
         if (threadIdx.x == 0) q.bound = bound;
     }
@@ -192,12 +207,12 @@ __device__ __forceinline__ void top_by_steps(uint32_t n, uint32_t top, Candidate
 // 8192 rows of 128256 bf16, top 64: 595 us.)  A row whose largest logits are equal in great number, or crowd into few
 // shares, can leave more than LDS holds and goes the slow way.
 template <typename T, int VEC, int BLOCK, bool HELD>
-__device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& parts, const Stretch& part, uint32_t top, float best,
+__device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& parts, const Stretch& part, uint32_t top, float best, float largest,
                                         const typename RawVec<T, VEC>::type (&held)[kLpUnroll], const float (&tops)[kLpUnroll],
                                         Candidates& q) {
     typedef RawVec<T, VEC> Raw;
     const uint32_t extra = part.lo == 0 ? parts.extra : 0u, vectors = part.hi - part.lo;
-    const uint32_t bound = bound_of<BLOCK>(q, (uint32_t)(class_key(best, 0u) >> 32), top);
+    const uint32_t bound = bound_of<BLOCK>(q, (uint32_t)(class_key(best, 0u) >> 32), ordered(largest) >> 16, top);
     const float least = bound_logit(bound);
     const T* body = base + parts.head;
     bool fits = true;
@@ -217,9 +232,29 @@ __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& p
         }
     };
     if constexpr (HELD) {
+        // first whole vectors, then classes, an element a thread: a place for each class of four vectors costs more
+        uint32_t reach = 0;
 #pragma unroll
-        for (int u = 0; u < kLpUnroll; ++u)
-            if (__ballot(tops[u] >= least) != 0) append_vector(tops[u] >= least, part.lo + u * BLOCK + threadIdx.x, held[u]);
+        for (int u = 0; u < kLpUnroll; ++u) reach += tops[u] >= least ? 1u : 0u;
+        uint32_t at = take_places(q.listed, reach);
+#pragma unroll
+        for (int u = 0; u < kLpUnroll; ++u) {
+            if (!(tops[u] >= least)) continue;
+            if (at < (uint32_t)kListed) {
+                reinterpret_cast<typename Raw::type*>(q.raw)[at] = held[u];
+                q.list[at] = part.lo + u * BLOCK + threadIdx.x;
+            }
+            ++at;
+        }
+        __syncthreads();
+        const uint32_t n = q.listed;
+        fits = n <= (uint32_t)kListed;
+        const uint32_t classes = fits ? n * VEC : 0u;
+        for (uint32_t i = threadIdx.x; i / kWave * kWave < classes; i += BLOCK) {
+            float v[1];
+            RawVec<T, 1>::unpack(reinterpret_cast<const T*>(q.raw)[i < classes ? i : 0u], v);
+            append(q, i < classes && v[0] >= least, class_key(v[0], parts.head + q.list[i < classes ? i / VEC : 0u] * VEC + i % VEC));
+        }
     } else {
         const uint32_t all_lines = (vectors + kLine - 1) / kLine, lines = all_lines <= (uint32_t)kLines ? all_lines : 0u;
         const uint32_t from = bound < 0x80u ? 0x80u : bound;                 // (-inf is 0x7f)
@@ -278,24 +313,28 @@ __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& p
 
 // The `top` largest of the n keys that a row's parts left, descending: key k of part j is at k * parts + j, so that the
 // parts' first keys, among which the row's largest are, fall to different threads.
+struct KeyList {
+    uint64_t key[kMaxShared / kLpBlock];          // a thread's share
+    __device__ __forceinline__ KeyList(const unsigned long long* keys, uint32_t n) {
+#pragma unroll
+        for (int i = 0; i < kMaxShared / kLpBlock; ++i) {
+            const uint32_t at = threadIdx.x + i * kLpBlock;
+            key[i] = 0;
+            if (i * (uint32_t)kLpBlock < n) key[i] = get_shared(keys + (at < n ? at : 0u));
+            if (at >= n) key[i] = 0;
+        }
+    }
+};
 template <int BLOCK>
-__device__ __forceinline__ void join_tops(const unsigned long long* keys, uint32_t n, uint32_t top, Candidates& q) {
+__device__ __forceinline__ void join_tops(const KeyList& mine, const unsigned long long* keys, uint32_t n, uint32_t top, float largest, Candidates& q) {
     constexpr int EACH = kMaxShared / BLOCK;
-    uint64_t mine[EACH];
     uint32_t best = 0;
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-        const uint32_t at = threadIdx.x + i * BLOCK;
-        mine[i] = 0;
-        if (i * BLOCK < n) mine[i] = get_shared(keys + (at < n ? at : 0u));
-        if (at >= n) mine[i] = 0;
-    }
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) best = max(best, (uint32_t)(mine[i] >> 32));
-    const uint32_t bound = bound_of<BLOCK>(q, best, top);
+    for (int i = 0; i < EACH; ++i) best = max(best, (uint32_t)(mine.key[i] >> 32));
+    const uint32_t bound = bound_of<BLOCK>(q, best, ordered(largest) >> 16, top);
 #pragma unroll
     for (int i = 0; i < EACH; ++i)
-        if (i * BLOCK < n) append(q, mine[i] != 0ull && (uint32_t)(mine[i] >> 48) >= bound, mine[i]);
+        if (i * (uint32_t)BLOCK < n) append(q, mine.key[i] != 0ull && (uint32_t)(mine.key[i] >> 48) >= bound, mine.key[i]);
     __syncthreads();
     if (q.count > (uint32_t)kCandidates) {
         __syncthreads();
@@ -376,7 +415,7 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
     const float best = t.m;
     t = block_stat<kLpBlock, ENT>(t, a.c, lds);
     if constexpr (MODE != PLAIN)
-        if (a.top != 0) row_top<T, VEC, kLpBlock, MODE == HELD>(base, parts, part, a.top, best, raw, tops, found);
+        if (a.top != 0) row_top<T, VEC, kLpBlock, MODE == HELD>(base, parts, part, a.top, best, t.m, raw, tops, found);
     if (a.parts > 1) {
         if (threadIdx.x == 0) {
             float* to = a.shared.stats + 4 * (uint64_t)blockIdx.x;
@@ -394,9 +433,13 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
             const float* from = a.shared.stats + 4 * ((uint64_t)row * a.parts + threadIdx.x);
             t = RowStat{get_shared(from), get_shared(from + 1), ENT ? get_shared(from + 2) : 0.0f};
         }
-        t = block_stat<kLpBlock, ENT>(t, a.c, lds);
-        if constexpr (MODE != PLAIN)
-            if (a.top != 0) join_tops<kLpBlock>(keys, a.parts * a.top, a.top, found);
+        if constexpr (MODE != PLAIN) {
+            const KeyList mine(keys, a.parts * a.top);                // (asked for before the statistics are put together)
+            t = block_stat<kLpBlock, ENT>(t, a.c, lds);
+            if (a.top != 0) join_tops<kLpBlock>(mine, keys, a.parts * a.top, a.top, t.m, found);
+        } else {
+            t = block_stat<kLpBlock, ENT>(t, a.c, lds);
+        }
     }
     const bool empty = t.m == -INFINITY && t.s == 0.0f;
     const float log_s = logf(t.s);                                // -inf for an empty row
@@ -564,11 +607,13 @@ SharedRows shared_rows(void* scratch) {
                       reinterpret_cast<uint32_t*>(at + (16ull + 8ull * AGRAD_MAX_TOP) * kSharedParts)};
 }
 
-// Parts of a row: as many as make some thousand workgroups of all rows (four a CU: the loads of a few more waves than that
-// fill the memory's queues), but none shorter than two vectors a thread (a part costs its workgroup's reductions, and the
-// parts are put together one after the other).
+// Parts of a row: as many as make 512 workgroups of all rows, or 1024 where the parts stay longer than 4096 vectors, but
+// none shorter than 512, two vectors a thread (a part costs its workgroup's reductions, and the parts are put together one
+// after the other).  48 rows of 18992 vectors, with 8 alternatives: 10 parts each 17.2 us, 21 parts 18.4, 5 parts 18.6, 2
+// parts 27.4; 256 rows of 16032: 4 parts 24.8, 2 parts 26.9, 1 part 31.9; one row: parts of 518 11.8, of 1069 13.2.
 uint32_t row_parts(uint64_t rows, uint32_t vectors) {
-    uint64_t parts = kSharedParts / rows;
+    uint64_t parts = 512 / rows;
+    if (parts == 0 || vectors / parts > 4096) parts = kSharedParts / rows;
     if (parts > vectors / 512u) parts = vectors / 512u;
     if (parts > kMaxParts) parts = kMaxParts;
     return parts < 1 ? 1u : (uint32_t)parts;

@@ -89,7 +89,7 @@ struct RowParts {
 // waits for anybody.  The counters are zero between launches (the last one puts its counter back), and all launches of a
 // context run on its one stream, recorded ones too, so that no two launches use the memory at once.
 constexpr uint32_t kSharedParts = 1024;      // workgroups of a launch that share rows, at most
-constexpr uint32_t kMaxParts = 64;           // parts of one row, at most
+constexpr uint32_t kMaxParts = 32;           // parts of one row, at most
 struct SharedRows {
     float* stats;             // [kSharedParts, 4]
     unsigned long long* keys; // [kSharedParts, AGRAD_MAX_TOP]
@@ -154,9 +154,20 @@ __device__ __forceinline__ RowStat block_stat(RowStat a, float c, RowStat* lds) 
     if constexpr (BLOCK == kWave) return a;
     if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = a;
     __syncthreads();
-    a = lds[0];
+    constexpr int W = BLOCK / kWave;
+    RowStat each[W];
+    float M = -INFINITY;
 #pragma unroll
-    for (int w = 1; w < BLOCK / kWave; ++w) a = merge_stat<ENT>(a, lds[w], c);
+    for (int w = 0; w < W; ++w) each[w] = lds[w];
+#pragma unroll
+    for (int w = 0; w < W; ++w) M = fmaxf(M, each[w].m);
+    a = RowStat{M, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+        const RowStat x = about<ENT>(each[w], M, c);
+        a.s = a.s + x.s;
+        if constexpr (ENT) a.d = a.d + x.d;
+    }
     __syncthreads();
     return a;
 }
