@@ -1171,7 +1171,7 @@ int agrad_topk_distill_forward(agrad_ctx* ctx, int dtype, const void* logits, co
                                uint32_t top, float scale, float teacher_scale, int mode) {
     CTX_OR_FAIL(ctx)
     return launch_distill_fwd(ctx->stream, dtype, logits, teacher_ids, teacher_values, loss, stats, rows, V, ld, top, scale,
-                              teacher_scale, mode, ctx->err_flag);
+                              teacher_scale, mode, ctx->err_flag, ctx->row_scratch);
 }
 int agrad_topk_distill_backward(agrad_ctx* ctx, int dtype, const void* logits, const int32_t* teacher_ids,
                                 const float* teacher_values, const float* dloss, const float* stats, void* dlogits,
@@ -1186,7 +1186,7 @@ int agrad_topk_distill_fused(agrad_ctx* ctx, int dtype, const void* logits, cons
                              uint32_t V, uint64_t ld, uint32_t top, float scale, float teacher_scale, float grad_scale, int mode) {
     CTX_OR_FAIL(ctx)
     return launch_distill_fused(ctx->stream, dtype, logits, teacher_ids, teacher_values, loss, row_scale, dlogits, rows, V, ld, top,
-                                scale, teacher_scale, grad_scale, mode, ctx->err_flag);
+                                scale, teacher_scale, grad_scale, mode, ctx->err_flag, ctx->row_scratch);
 }
 
 int agrad_adamw8bit_step(agrad_ctx* ctx, int grad_dtype, float* p, const void* g, uint8_t* qm, uint8_t* qv,

@@ -13,8 +13,12 @@
 //            dx = scale * (d loss / d z) * upstream
 //
 // The classes outside the ids are summed up on their own, not as 1 - sum p[id]: a student that is sure of itself has a
-// p_rest far below the rounding of 1, down to below the smallest number.  The test for "outside" costs a row's stream one
-// look at an LDS bit a vector.
+// p_rest far below the rounding of 1, down to below the smallest number.  For that the ids of a row are marked in a bit map
+// in LDS, a bit a class, and a vector of logits looks its bits up: three instructions a vector of 16 bytes.  The gradient
+// treats all classes as classes outside, and the few among the ids are stored over that.
+//
+// HBM bounds all of it: the forward pass reads the logits once, the backward pass reads them and writes the gradient, and
+// loss and gradient in one launch read once and write once where a workgroup's registers hold the row.
 #include "launch.hpp"
 #include "row_softmax.hpp"
 
@@ -25,30 +29,21 @@ namespace agrad {
 namespace {
 
 constexpr int kDsBlock = 256;
-constexpr int kDsUnroll = 4;
-constexpr uint32_t kSetWords = 512;          // bits of the vectors that hold an id, by the vector's number modulo 16384
-static_assert(AGRAD_MAX_TOP <= kDsBlock, "a thread a teacher slot");
+constexpr int kDsUnroll = 4;                       // vectors a thread keeps in flight
+constexpr uint32_t kMapWords = 5120;               // of the bit map: 163840 classes of a row, or of a part of one
+constexpr uint32_t kMapBits = kMapWords * 32;
+static_assert(AGRAD_MAX_TOP <= kDsBlock && AGRAD_MAX_TOP == 2 * kWave, "a thread a teacher slot, the slots of two waves");
 
 struct DsArgs {
     const int32_t* ids; const float* values;
-    uint64_t ld; uint32_t V, top; float scale, c, teacher_scale; uint32_t tail;
+    uint64_t ld; uint32_t V, top; float scale, c, teacher_scale;
     int* err_flag;
 };
 struct DsOut {
-    float* loss; float* stats;                                     // forward
-    const float* row_scale; float grad_scale;                      // loss and gradient in one launch
+    float* loss; float* stats;                     // forward
+    const float* row_scale; float grad_scale;      // loss and gradient in one launch
+    SharedRows shared; uint32_t parts;
 };
-
-// a row's teacher slots in LDS: the class of each (-1: unused), its probability, log probability
-struct Slots {
-    int32_t id[AGRAD_MAX_TOP];
-    float q[AGRAD_MAX_TOP];
-    uint32_t bits[kSetWords];
-};
-
-__device__ __forceinline__ bool set_bit(const Slots& s, uint32_t vec) {
-    return (s.bits[(vec >> 5) & (kSetWords - 1)] >> (vec & 31u)) & 1u;
-}
 
 __device__ __forceinline__ int32_t slot_id(const DsArgs& a, uint64_t row, uint32_t k, bool report) {
     if (k >= a.top) return -1;
@@ -58,16 +53,54 @@ __device__ __forceinline__ int32_t slot_id(const DsArgs& a, uint64_t row, uint32
     return -1;
 }
 
-// The teacher's side of a row, thread k its slot k: log q (of an unused slot -inf), and for everyone sum q (0: no slots)
-// and, in RENORM, the log of the softmax's denominator.
+// ---- the bit map of a row's ids -----------------------------------------------------------------------
+template <int BLOCK>
+__device__ __forceinline__ void clear_map(uint32_t* map, uint32_t classes) {
+    const uint32_t n = (classes + 127) / 128;
+    for (uint32_t i = threadIdx.x; i < n; i += BLOCK) reinterpret_cast<u32x4*>(map)[i] = u32x4{0u, 0u, 0u, 0u};
+}
+// (first: the class of bit 0)
+__device__ __forceinline__ void mark(uint32_t* map, int32_t id, uint32_t first, uint32_t classes) {
+    const uint32_t at = (uint32_t)id - first;
+    if (id >= 0 && at < classes) atomicOr(&map[at / 32], 1u << (at % 32));
+}
+// the bits of the vec-th vector
+template <int VEC>
+__device__ __forceinline__ uint32_t bits_of(const uint32_t* map, uint32_t vec) {
+    const uint32_t at = vec * VEC;
+    return (map[at / 32] >> (at % 32)) & ((1u << VEC) - 1u);
+}
+__device__ __forceinline__ void mask_raw(f32x4& r, uint32_t bits) {
+    if (bits & 1u) r.x = -INFINITY;
+    if (bits & 2u) r.y = -INFINITY;
+    if (bits & 4u) r.z = -INFINITY;
+    if (bits & 8u) r.w = -INFINITY;
+}
+__device__ __forceinline__ uint32_t mask_pair(uint32_t w, uint32_t bits) {
+    if (bits & 1u) w = (w & 0xffff0000u) | 0xff80u;
+    if (bits & 2u) w = (w & 0x0000ffffu) | 0xff800000u;
+    return w;
+}
+__device__ __forceinline__ void mask_raw(u32x4& r, uint32_t bits) {
+    r.x = mask_pair(r.x, bits);
+    r.y = mask_pair(r.y, bits >> 2);
+    r.z = mask_pair(r.z, bits >> 4);
+    r.w = mask_pair(r.w, bits >> 6);
+}
+__device__ __forceinline__ void mask_raw(float& r, uint32_t bits) { if (bits) r = -INFINITY; }
+__device__ __forceinline__ void mask_raw(bf16_t& r, uint32_t bits) { if (bits) r = 0xff80; }
+
+// ---- the teacher's side of a row ------------------------------------------------------------------------
+// Thread k has slot k: log q (of an unused slot -inf).  For everyone: sum q, the softmax's denominator (RENORM; +inf: no slots
+// to learn from).
 struct Teacher {
     float log_q, mass, lse;
 };
-template <int BLOCK>
+template <int BLOCK, bool TAIL>
 __device__ __forceinline__ Teacher teacher_row(const DsArgs& a, uint64_t row, int32_t id, float* lds) {
     const float u = id >= 0 ? a.values[row * a.top + threadIdx.x] : -INFINITY;
     Teacher t;
-    if (a.tail) {
+    if (TAIL) {
         t.log_q = u;
         t.lse = 0.0f;
         t.mass = block_total<BLOCK>(expf(u), lds);
@@ -77,172 +110,188 @@ __device__ __forceinline__ Teacher teacher_row(const DsArgs& a, uint64_t row, in
     const float m = block_largest<BLOCK>(w, lds);
     const float e = m == -INFINITY ? (w != w ? w : 0.0f) : expf(w - m);
     const float total = block_total<BLOCK>(e, lds);
-    if (total == 0.0f) return Teacher{-INFINITY, 0.0f, INFINITY};         // no slots: nothing to learn from
+    if (total == 0.0f) return Teacher{-INFINITY, 0.0f, INFINITY};
     t.lse = m + logf(total);
     t.log_q = w - t.lse;
     t.mass = 1.0f;
     return t;
 }
 
-// marks the vectors that hold an id
-template <int VEC>
-__device__ __forceinline__ void mark_slots(Slots& s, int32_t id, uint32_t head, uint32_t nvec) {
-    if (id >= (int32_t)head) {
-        const uint32_t vec = ((uint32_t)id - head) / VEC;
-        if (vec < nvec) atomicOr(&s.bits[(vec >> 5) & (kSetWords - 1)], 1u << (vec & 31u));
+// Slots in LDS.  A class that a row names twice counts with both its q; only its first slot stands for it.
+struct Slots {
+    int32_t id[AGRAD_MAX_TOP];
+    float q[AGRAD_MAX_TOP];
+};
+struct Own {
+    bool first;
+    float taken;              // sum of the q of this slot's class, in slot order
+};
+__device__ __forceinline__ Own own_slot(const Slots& s, uint32_t n, uint32_t k, int32_t id) {
+    Own o{id >= 0, 0.0f};
+    if (id < 0) return o;
+    for (uint32_t j = 0; j < n; j += 4) {            // (slots past n hold -1)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+            if (s.id[j + i] != id) continue;
+            o.taken = o.taken + s.q[j + i];
+            if (j + i < k) o.first = false;
+        }
     }
+    return o;
 }
 
-// The student's side of a row: all classes, and in TAIL those outside the ids.
-struct Student {
-    RowStat all, rest;
+// ---- what a row's gradient is made of --------------------------------------------------------------------
+// all: log of the student's whole sum about m, the largest logit (m = -inf: no gradient); log_rest: log of p_rest (TAIL;
+// -inf: no class outside), mass: sum q.  This is what a forward call leaves for its backward call, so that a row of logits
+// far from 0 loses nothing (an lse of 1e6 would have lost log p).
+struct RowSums {
+    float m, all, log_rest, mass;
 };
-template <typename T, int VEC, int BLOCK, bool TAIL>
-__device__ __forceinline__ Student student_row(const T* base, const DsArgs& a, const Slots& slots, int32_t id, float at, bool first,
-                                               RowStat* lds) {
+struct RowGrad {
+    float m;
+    float out_log, out;       // outside the ids:  out exp((x - m) scale - out_log)
+    float all, mass;          // among them:       mass exp((x - m) scale - all) - q
+};
+template <bool TAIL>
+__device__ __forceinline__ RowGrad row_grad(const RowSums& s) {
+    RowGrad g{s.m, s.all, s.mass, s.all, s.mass};
+    if (TAIL) {
+        if (s.log_rest == -INFINITY) {
+            g.out = 0.0f;                                          // no class outside has mass
+        } else {
+            const float q_rest = fmaxf(1.0f - s.mass, 0.0f);
+            g.mass = s.mass + q_rest;
+            g.out_log = s.all + s.log_rest;
+            g.out = g.mass * expf(s.log_rest) - q_rest;
+        }
+    }
+    return g;
+}
+// the gradient of a class among the ids, times `mul`
+__device__ __forceinline__ float own_grad(const RowGrad& g, const DsArgs& a, float at, float taken, float mul) {
+    return (expf((at - g.m) * a.scale - g.all) * g.mass - taken) * mul;
+}
+
+// Loss and sums of a row from what a pass over it found: `pass` is the sum over all classes, or (TAIL) over those outside the
+// ids; at: the logit of this thread's slot.  used: some slot of the row is.
+template <int BLOCK, bool TAIL>
+__device__ __forceinline__ RowSums finish_row(const DsArgs& a, const RowStat& pass, const Teacher& t, int32_t id, float q, float at, bool first,
+                                              bool used, float* lds, RowStat* lds_stat, float& loss) {
+    RowStat all = pass;
+    if (TAIL) {
+        RowStat own = empty_stat();
+        if (first) {
+            float v[1] = {at};
+            absorb_stat<false, 1>(own, v, a.c);
+        }
+        all = merge_stat<false>(pass, block_stat<BLOCK, false>(own, a.c, lds_stat), a.c);
+    }
+    const float log_s = logf(all.s);
+    float term = 0.0f;
+    if (id >= 0 && !(q == 0.0f)) term = q * (t.log_q - ((at - all.m) * a.scale - log_s));
+    loss = block_total<BLOCK>(term, lds);
+    RowSums s{all.m, log_s, -INFINITY, t.mass};
+    if (TAIL && !(pass.m == -INFINITY && pass.s == 0.0f)) {
+        s.log_rest = (pass.m - all.m) * a.scale + (logf(pass.s) - log_s);
+        const float q_rest = fmaxf(1.0f - t.mass, 0.0f);
+        if (q_rest > 0.0f) loss = loss + q_rest * (logf(q_rest) - s.log_rest);
+    }
+    if (!used || t.lse == INFINITY || (all.m == -INFINITY && all.s == 0.0f)) {
+        loss = 0.0f;
+        s = RowSums{-INFINITY, 0.0f, -INFINITY, 0.0f};
+    }
+    return s;
+}
+
+// ---- forward: a workgroup a row, or a part of one ----------------------------------------------------------
+template <typename T, int VEC, bool TAIL>
+__global__ void __launch_bounds__(kDsBlock)
+distill_fwd_kernel(const T* __restrict__ x, const DsArgs a, const DsOut o) {
+    __shared__ __align__(16) uint32_t map[TAIL ? kMapWords : 4];
+    __shared__ Slots slots;
+    __shared__ float lds[kDsBlock / kWave];
+    __shared__ RowStat lds_stat[kDsBlock / kWave];
+    __shared__ uint32_t word;
+    typedef RawVec<T, VEC> Raw;
+    const uint32_t row = blockIdx.x / o.parts, nth = blockIdx.x - row * o.parts, k = threadIdx.x;
+    const T* base = x + row * a.ld;
     const RowParts<T, VEC> parts(base, a.V);
-    RowStat r = empty_stat();
-    if (threadIdx.x < parts.extra) {
-        const uint32_t e = parts.extra_at(threadIdx.x);
+    const Stretch part(parts.nvec, nth, o.parts);
+    const T* body = base + parts.head;
+    const int32_t id = slot_id(a, row, k, nth == 0);
+    float at[1];
+    VecIO<T, 1>::load(base + (id >= 0 ? id : 0), at);
+    if (k < AGRAD_MAX_TOP) slots.id[k] = id;
+    if (TAIL) {
+        const uint32_t classes = (part.hi - part.lo) * VEC;
+        clear_map<kDsBlock>(map, classes);
+        __syncthreads();
+        mark(map, id, parts.head + part.lo * VEC, classes);
+        __syncthreads();
+    }
+    RowStat t = empty_stat();
+    for (uint32_t i0 = part.lo + k; i0 < part.hi; i0 += kDsBlock * kDsUnroll) {
+        typename Raw::type raw[kDsUnroll];
+#pragma unroll
+        for (int u = 0; u < kDsUnroll; ++u) {
+            const uint32_t i = i0 + u * kDsBlock;
+            raw[u] = Raw::load(body + (uint64_t)(i < part.hi ? i : part.lo) * VEC);
+        }
+#pragma unroll
+        for (int u = 0; u < kDsUnroll; ++u) {
+            const uint32_t i = i0 + u * kDsBlock;
+            if (i >= part.hi) continue;
+            if (TAIL) {
+                const uint32_t bits = bits_of<VEC>(map, i - part.lo);
+                if (bits != 0) mask_raw(raw[u], bits);
+            }
+            float v[VEC];
+            Raw::unpack(raw[u], v);
+            absorb_stat<false, VEC>(t, v, a.c);
+        }
+    }
+    if (nth == 0 && k < parts.extra) {
+        const uint32_t e = parts.extra_at(k);
         float v[1];
         VecIO<T, 1>::load(base + e, v);
         if (TAIL)
-            for (uint32_t k = 0; k < a.top; ++k)
-                if (slots.id[k] == (int32_t)e) v[0] = -INFINITY;
-        absorb_stat<false, 1>(r, v, a.c);
+            for (uint32_t j = 0; j < a.top; ++j)
+                if (slots.id[j] == (int32_t)e) v[0] = -INFINITY;
+        absorb_stat<false, 1>(t, v, a.c);
     }
-    const T* body = base + parts.head;
-    for (uint32_t i0 = threadIdx.x; i0 < parts.nvec; i0 += BLOCK * kDsUnroll) {
-        float v[kDsUnroll][VEC];
-#pragma unroll
-        for (int u = 0; u < kDsUnroll; ++u) {
-            const uint32_t i = i0 + u * BLOCK;
-            if (i < parts.nvec) VecIO<T, VEC>::load(body + (uint64_t)i * VEC, v[u]);
+    t = block_stat<kDsBlock, false>(t, a.c, lds_stat);
+    if (o.parts > 1) {
+        if (k == 0) {
+            float* to = o.shared.stats + 4 * (uint64_t)blockIdx.x;
+            put_shared(to, t.m);
+            put_shared(to + 1, t.s);
         }
-#pragma unroll
-        for (int u = 0; u < kDsUnroll; ++u) {
-            const uint32_t i = i0 + u * BLOCK;
-            if (i >= parts.nvec) continue;
-            if (TAIL && set_bit(slots, i)) {
-                const uint32_t e = parts.head + i * VEC;
-                for (uint32_t k = 0; k < a.top; ++k) {
-                    const uint32_t off = (uint32_t)slots.id[k] - e;
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j)
-                        if (off == (uint32_t)j) v[u][j] = -INFINITY;
-                }
-            }
-            absorb_stat<false, VEC>(r, v[u], a.c);
+        if (!workgroup_arrives_last(o.shared.tickets + row, o.parts, &word)) return;
+        t = empty_stat();
+        if (k < o.parts) {
+            const float* from = o.shared.stats + 4 * ((uint64_t)row * o.parts + k);
+            t = RowStat{get_shared(from), get_shared(from + 1), 0.0f};
         }
+        t = block_stat<kDsBlock, false>(t, a.c, lds_stat);
     }
-    r = block_stat<BLOCK, false>(r, a.c, lds);
-    if (!TAIL) return Student{r, r};
-    // the ids' own classes, each once
-    RowStat own = empty_stat();
-    if (id >= 0 && first) {
-        float v[1] = {at};
-        absorb_stat<false, 1>(own, v, a.c);
-    }
-    own = block_stat<BLOCK, false>(own, a.c, lds);
-    return Student{merge_stat<false>(r, own, a.c), r};
-}
-
-// What a row's gradient is made of: the classes outside the ids have exp(z - lse_out) out, those among them
-// exp(z - lse) mass - q.  lse = -inf: the row has no gradient.
-struct RowGrad {
-    float lse, lse_out, mass, out;
-};
-
-// Everything of a row but its gradient: the slots in LDS, the loss, and what the gradient needs.
-template <typename T, int VEC, int BLOCK, bool TAIL>
-__device__ __forceinline__ RowGrad row_loss(const T* base, uint64_t row, const DsArgs& a, Slots& slots, float* lds, RowStat* lds_stat,
-                                            float* loss_out, float& teacher_lse) {
-    const RowParts<T, VEC> parts(base, a.V);
-    const uint32_t k = threadIdx.x;
-    const int32_t id = slot_id(a, row, k, true);
-    float at[1];                                   // the student's logit of this thread's slot
-    VecIO<T, 1>::load(base + (id >= 0 ? id : 0), at);
-    for (uint32_t i = k; i < kSetWords; i += BLOCK) slots.bits[i] = 0;
     const bool used = __syncthreads_or(id >= 0) != 0;
-    const Teacher t = teacher_row<BLOCK>(a, row, id, lds);
-    const float q = expf(t.log_q);
-    if (k < AGRAD_MAX_TOP) {
-        slots.id[k] = id;
-        slots.q[k] = q;
-    }
-    __syncthreads();
-    mark_slots<VEC>(slots, id, parts.head, parts.nvec);
-    bool first = true;
-    if (TAIL && id >= 0)
+    const Teacher teach = teacher_row<kDsBlock, TAIL>(a, row, id, lds);
+    const float q = expf(teach.log_q);
+    bool first = id >= 0;
+    if (TAIL && first)
         for (uint32_t j = 0; j < k; ++j) first = first && slots.id[j] != id;
-    __syncthreads();
-    const Student s = student_row<T, VEC, BLOCK, TAIL>(base, a, slots, id, at[0], first, lds_stat);
-    const bool none = !used || t.lse == INFINITY || (s.all.m == -INFINITY && s.all.s == 0.0f);
-    const float log_s = logf(s.all.s);
-    float term = 0.0f;
-    if (id >= 0 && !(q == 0.0f)) term = q * (t.log_q - ((at[0] - s.all.m) * a.scale - log_s));
-    float loss = block_total<BLOCK>(term, lds);
-    RowGrad g;
-    g.lse = s.all.m * a.scale + log_s;
-    g.lse_out = g.lse;
-    g.mass = t.mass;
-    g.out = t.mass;
-    if (TAIL) {
-        if (s.rest.m == -INFINITY && s.rest.s == 0.0f) {       // no class outside the ids has mass
-            g.lse_out = INFINITY;
-        } else {
-            const float q_rest = fmaxf(1.0f - t.mass, 0.0f), log_rest = logf(s.rest.s);
-            const float log_p_rest = (s.rest.m - s.all.m) * a.scale + (log_rest - log_s);
-            if (q_rest > 0.0f) loss = loss + q_rest * (logf(q_rest) - log_p_rest);
-            g.lse_out = s.rest.m * a.scale + log_rest;
-            g.mass = t.mass + q_rest;
-            g.out = g.mass * expf(log_p_rest) - q_rest;
+    float loss;
+    const RowSums s = finish_row<kDsBlock, TAIL>(a, t, teach, id, q, at[0], first, used, lds, lds_stat, loss);
+    if (k == 0) {
+        if (o.loss != nullptr) o.loss[row] = loss;
+        if (o.stats != nullptr) {
+            float* to = o.stats + row * 4ull;
+            to[0] = s.m; to[1] = s.all; to[2] = TAIL ? s.log_rest : teach.lse; to[3] = s.mass;
         }
     }
-    teacher_lse = t.lse;
-    if (none) {
-        loss = 0.0f;
-        g = RowGrad{-INFINITY, INFINITY, 0.0f, 0.0f};
-    }
-    if (k == 0 && loss_out != nullptr) loss_out[row] = loss;
-    return g;
 }
 
-// one vector of the gradient: first: its first class; near: it may hold an id
-template <int VEC>
-__device__ __forceinline__ void ds_grad(float (&v)[VEC], const RowGrad& g, float scale, float mul, uint32_t first, bool near, const int32_t* id,
-                                        const float* q, uint32_t n) {
-    float x[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-        x[j] = v[j] * scale;
-        v[j] = __builtin_amdgcn_exp2f((x[j] - g.lse_out) * kLog2eHi) * g.out;
-    }
-    if (near) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            bool in_set = false;
-            float taken = 0.0f;
-            for (uint32_t k = 0; k < n; ++k) {
-                if ((uint32_t)id[k] == first + (uint32_t)j) {
-                    in_set = true;
-                    taken = taken + q[k];
-                }
-            }
-            if (in_set) v[j] = __builtin_amdgcn_exp2f((x[j] - g.lse) * kLog2eHi) * g.mass - taken;
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = v[j] * mul;
-}
-
-// (a row without a gradient: zeros, whatever its logits hold)
-template <int VEC>
-__device__ __forceinline__ void ds_zero(float (&v)[VEC]) {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = 0.0f;
-}
-
+// ---- backward: a workgroup a chunk of a row ------------------------------------------------------------------
 template <typename T, int VEC>
 __device__ __forceinline__ void ds_store(T* to, float (&d)[VEC], uint32_t accumulate) {
     if (accumulate) {
@@ -256,123 +305,231 @@ __device__ __forceinline__ void ds_store(T* to, float (&d)[VEC], uint32_t accumu
 
 template <typename T, int VEC, bool TAIL>
 __global__ void __launch_bounds__(kDsBlock)
-distill_fwd_kernel(const T* __restrict__ x, const DsArgs a, const DsOut o) {
-    __shared__ Slots slots;
-    __shared__ float lds[kDsBlock / kWave];
-    __shared__ RowStat lds_stat[kDsBlock / kWave];
-    const uint64_t row = blockIdx.x;
-    float teacher_lse;
-    const RowGrad g = row_loss<T, VEC, kDsBlock, TAIL>(x + row * a.ld, row, a, slots, lds, lds_stat, o.loss, teacher_lse);
-    if (threadIdx.x == 0 && o.stats != nullptr) {
-        float* to = o.stats + row * 4;
-        to[0] = g.lse; to[1] = TAIL ? g.lse_out : teacher_lse; to[2] = g.mass; to[3] = g.out;
-    }
-}
-
-// loss and gradient of a row in one workgroup (x and dx may be the same memory)
-template <typename T, int VEC, bool TAIL>
-__global__ void __launch_bounds__(kDsBlock)
-distill_fused_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
-    __shared__ Slots slots;
-    __shared__ float lds[kDsBlock / kWave];
-    __shared__ RowStat lds_stat[kDsBlock / kWave];
-    const uint64_t row = blockIdx.x;
-    const T* base = x + row * a.ld;
-    T* out = dx + row * a.ld;
-    float teacher_lse;
-    const RowGrad g = row_loss<T, VEC, kDsBlock, TAIL>(base, row, a, slots, lds, lds_stat, o.loss, teacher_lse);
-    const float mul = a.scale * (o.row_scale != nullptr ? o.row_scale[row] : o.grad_scale);
-    const bool none = g.lse == -INFINITY;
-    const RowParts<T, VEC> parts(base, a.V);
-    if (threadIdx.x < parts.extra) {
-        const uint32_t e = parts.extra_at(threadIdx.x);
-        float v[1];
-        VecIO<T, 1>::load(base + e, v);
-        if (none) ds_zero<1>(v);
-        else ds_grad<1>(v, g, a.scale, mul, e, true, slots.id, slots.q, a.top);
-        VecIO<T, 1>::store(out + e, v);
-    }
-    for (uint32_t i = threadIdx.x; i < parts.nvec; i += kDsBlock) {
-        const uint32_t e = parts.head + i * VEC;
-        float v[VEC];
-        VecIO<T, VEC>::load(base + e, v);
-        if (none) ds_zero<VEC>(v);
-        else ds_grad<VEC>(v, g, a.scale, mul, e, set_bit(slots, i), slots.id, slots.q, a.top);
-        VecIO<T, VEC>::store(out + e, v);
-    }
-}
-
-// the gradient with the row's statistics given: a workgroup a chunk of a row
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kDsBlock)
-distill_bwd_kernel(const T* x, T* dx, const DsArgs a, const float* dloss, const float* stats, uint32_t accumulate, const FastDiv32 chunks) {
-    __shared__ int32_t ids[AGRAD_MAX_TOP];
-    __shared__ float qs[AGRAD_MAX_TOP];
-    __shared__ uint32_t in_wave[2];
+distill_bwd_kernel(const T* x, T* dx, const DsArgs a, const float* dloss, const float* row_scale, float grad_scale, const float* stats,
+                   uint32_t accumulate, const FastDiv32 chunks) {
+    // the chunk's ids in slot order, then what is stored over their classes, and by which thread: the one that stores the vector
+    __shared__ Slots here;
+    __shared__ float value[AGRAD_MAX_TOP];
+    __shared__ uint32_t owner[AGRAD_MAX_TOP];
+    __shared__ uint32_t in_wave[kDsBlock / kWave];
+    typedef RawVec<T, VEC> Raw;
     const uint32_t row = chunks.div(blockIdx.x), chunk = blockIdx.x - row * chunks.d, tid = threadIdx.x;
     const T* base = x + (uint64_t)row * a.ld;
     T* out = dx + (uint64_t)row * a.ld;
     const RowParts<T, VEC> parts(base, a.V);
-    const uint32_t span = kDsBlock * kDsUnroll;                      // vectors of a chunk
-    float v[kDsUnroll][VEC];
+    constexpr uint32_t span = kDsBlock * kDsUnroll;                  // vectors of a chunk
+    const uint32_t i0 = chunk * span + tid;
+    typename Raw::type raw[kDsUnroll];
 #pragma unroll
     for (int u = 0; u < kDsUnroll; ++u) {
-        const uint32_t i = chunk * span + u * kDsBlock + tid;
-        if (i < parts.nvec) VecIO<T, VEC>::load(base + parts.head + (uint64_t)i * VEC, v[u]);
+        const uint32_t i = i0 + u * kDsBlock;
+        raw[u] = Raw::load(base + parts.head + (uint64_t)(i < parts.nvec ? i : 0u) * VEC);
     }
+    const uint32_t extra = chunk == 0 ? parts.extra : 0u, e = parts.extra_at(tid);
+    float xe[1];
+    VecIO<T, 1>::load(base + (tid < extra ? e : 0u), xe);
     const float* st = stats + (uint64_t)row * 4;
-    const RowGrad g{st[0], a.tail ? st[1] : st[0], st[2], st[3]};
-    const float teacher_lse = st[1];
-    const float mul = a.scale * dloss[row];
-    const bool none = g.lse == -INFINITY;
-    // the slots whose class lies in this chunk (chunk 0: or outside the vectors), in slot order
-    static_assert(AGRAD_MAX_TOP <= 2 * kWave, "the slots of two waves");
-    const int32_t id = slot_id(a, row, tid, chunk == 0);
+    const RowGrad g = row_grad<TAIL>(RowSums{st[0], st[1], TAIL ? st[2] : -INFINITY, st[3]});
+    const float mul = a.scale * (dloss != nullptr ? dloss[row] : row_scale != nullptr ? row_scale[row] : grad_scale);
+    const bool none = g.m == -INFINITY;
+
+    const int32_t id = slot_id(a, row, tid, chunk == 0 && dloss != nullptr);
     const uint32_t vec = id >= (int32_t)parts.head ? ((uint32_t)id - parts.head) / VEC : 0xffffffffu;
-    const bool outside_vectors = id >= 0 && vec >= parts.nvec;
-    const bool here = !none && id >= 0 && (outside_vectors ? chunk == 0 : vec / span == chunk);
-    const uint64_t lanes = __ballot(here);
-    if (tid < 2 * kWave && tid % kWave == 0) in_wave[tid / kWave] = (uint32_t)__popcll(lanes);
-    __syncthreads();
-    if (here) {
-        const uint32_t at = (tid >= kWave ? in_wave[0] : 0u) + (uint32_t)__popcll(lanes & ((1ull << (tid % kWave)) - 1));
-        const float u = a.values[(uint64_t)row * a.top + tid];
-        ids[at] = id;
-        qs[at] = a.tail ? expf(u) : expf(u * a.teacher_scale - teacher_lse);
-    }
+    const bool in_vectors = vec < parts.nvec;
+    const bool mine = !none && id >= 0 && (in_vectors ? vec / span == chunk : chunk == 0);
+    const uint64_t lanes = __ballot(mine);
+    if (tid % kWave == 0) in_wave[tid / kWave] = (uint32_t)__popcll(lanes);
+    if (tid < AGRAD_MAX_TOP) here.id[tid] = -1;
     __syncthreads();
     const uint32_t n = in_wave[0] + in_wave[1];
-    if (chunk == 0 && tid < parts.extra) {
-        const uint32_t e = parts.extra_at(tid);
-        float w[1];
-        VecIO<T, 1>::load(base + e, w);
-        if (none) ds_zero<1>(w);
-        else ds_grad<1>(w, g, a.scale, mul, e, true, ids, qs, n);
-        ds_store<T, 1>(out + e, w, accumulate);
+    if (n != 0) {                                                   // (uniform)
+        uint32_t place = 0;
+        float at[1], old[1], q = 0.0f;
+        if (mine) {
+            place = (tid >= kWave ? in_wave[0] : 0u) + (uint32_t)__popcll(lanes & ((1ull << (tid % kWave)) - 1));
+            const float u = a.values[(uint64_t)row * a.top + tid];
+            VecIO<T, 1>::load(base + id, at);
+            if (accumulate) VecIO<T, 1>::load(out + id, old);
+            q = TAIL ? expf(u) : expf(u * a.teacher_scale - st[2]);
+            here.id[place] = id;
+            here.q[place] = q;
+        }
+        __syncthreads();
+        if (mine) {
+            const Own own = own_slot(here, n, place, id);
+            float d = own_grad(g, a, at[0], own.taken, mul);
+            if (accumulate) d = old[0] + d;
+            value[place] = d;
+            const uint32_t who = in_vectors ? vec % kDsBlock : ((uint32_t)id < parts.head ? (uint32_t)id : parts.head + ((uint32_t)id - parts.tail_start));
+            owner[place] = own.first ? who : 0xffffffffu;
+        }
+    }
+    __syncthreads();
+
+    if (none) {                                                  // (zeros, whatever the logits hold)
+        if (accumulate) return;
+        float v[VEC] = {};
+        float d[1] = {0.0f};
+        if (tid < extra) VecIO<T, 1>::store(out + e, d);
+#pragma unroll
+        for (int u = 0; u < kDsUnroll; ++u)
+            if (i0 + u * kDsBlock < parts.nvec) VecIO<T, VEC>::store(out + parts.head + (uint64_t)(i0 + u * kDsBlock) * VEC, v);
+        return;
+    }
+    const float k = g.out * mul, b = -g.out_log * kLog2eHi;
+    if (tid < extra) {
+        float d[1] = {__builtin_amdgcn_exp2f(__builtin_fmaf(xe[0] - g.m, a.c, b)) * k};
+        ds_store<T, 1>(out + e, d, accumulate);
     }
 #pragma unroll
     for (int u = 0; u < kDsUnroll; ++u) {
-        const uint32_t i = chunk * span + u * kDsBlock + tid;
+        const uint32_t i = i0 + u * kDsBlock;
         if (i >= parts.nvec) continue;
-        const uint32_t e = parts.head + i * VEC;
-        bool near = false;
-        for (uint32_t k = 0; k < n; ++k) near = near || (uint32_t)ids[k] - e < (uint32_t)VEC;
-        if (none) ds_zero<VEC>(v[u]);
-        else ds_grad<VEC>(v[u], g, a.scale, mul, e, near, ids, qs, n);
-        ds_store<T, VEC>(out + e, v[u], accumulate);
+        float v[VEC];
+        Raw::unpack(raw[u], v);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(v[j] - g.m, a.c, b)) * k;
+        ds_store<T, VEC>(out + parts.head + (uint64_t)i * VEC, v, accumulate);
+    }
+    // (a later store of the same thread to the same place: in order)
+    for (uint32_t j = 0; j < n; ++j) {
+        if (owner[j] != tid) continue;
+        float d[1] = {value[j]};
+        VecIO<T, 1>::store(out + here.id[j], d);
     }
 }
 
-template <typename T>
-int ds_fwd_typed(hipStream_t s, const T* x, const DsArgs& a, const DsOut& o, uint64_t rows) {
-    constexpr int WIDE = WideVec<T>::value;
-    const bool wide = a.V >= 4 * WIDE;
-    const dim3 grid((uint32_t)rows), block(kDsBlock);
-    if (wide && a.tail) hipLaunchKernelGGL((distill_fwd_kernel<T, WIDE, true>), grid, block, 0, s, x, a, o);
-    else if (wide) hipLaunchKernelGGL((distill_fwd_kernel<T, WIDE, false>), grid, block, 0, s, x, a, o);
-    else if (a.tail) hipLaunchKernelGGL((distill_fwd_kernel<T, 1, true>), grid, block, 0, s, x, a, o);
-    else hipLaunchKernelGGL((distill_fwd_kernel<T, 1, false>), grid, block, 0, s, x, a, o);
-    return check_hip(hipGetLastError(), "top-k distillation launch");
+// ---- loss and gradient in one launch, the row in registers in between ------------------------------------------
+// Two 512-thread workgroups share a CU up to 20 vectors a thread; longer rows take one of 1024 threads.  x and dx may be
+// the same memory.
+template <typename T, int VEC, int NV, int BLOCK, bool TAIL>
+__global__ void __launch_bounds__(BLOCK)
+distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
+    __shared__ __align__(16) uint32_t map[TAIL ? (NV * BLOCK * VEC + 31) / 32 + 4 : 4];
+    __shared__ Slots slots;
+    __shared__ float lds[BLOCK / kWave];
+    __shared__ RowStat lds_stat[BLOCK / kWave];
+    typedef RawVec<T, VEC> Raw;
+    const uint32_t row = blockIdx.x, tid = threadIdx.x;
+    const T* base = x + row * a.ld;
+    T* out = dx + row * a.ld;
+    const RowParts<T, VEC> parts(base, a.V);
+    const T* body = base + parts.head;
+    // every load of the row, then the slots' and the elements outside the vectors
+    typename Raw::type raw[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const uint32_t at = (uint32_t)i * BLOCK + tid;
+        raw[i] = Raw::load(body + (uint64_t)(at < parts.nvec ? at : 0u) * VEC);
+    }
+    const uint32_t e = parts.extra_at(tid);
+    float xe = -INFINITY;
+    {
+        float v[1];
+        VecIO<T, 1>::load(base + (tid < parts.extra ? e : 0u), v);
+        if (tid < parts.extra) xe = v[0];
+    }
+    const int32_t id = slot_id(a, row, tid, true);
+    float at[1];
+    VecIO<T, 1>::load(base + (id >= 0 ? id : 0), at);
+    if (TAIL) clear_map<BLOCK>(map, parts.nvec * VEC);
+    const bool used = __syncthreads_or(id >= 0) != 0;
+    if (TAIL) mark(map, id, parts.head, parts.nvec * VEC);
+    const Teacher teach = teacher_row<BLOCK, TAIL>(a, row, id, lds);
+    const float q = expf(teach.log_q);
+    if (tid < AGRAD_MAX_TOP) {
+        slots.id[tid] = id;
+        slots.q[tid] = q;
+    }
+    __syncthreads();
+    const Own own = own_slot(slots, a.top, tid, id);
+    if (TAIL) {
+        if (tid < parts.extra)
+            for (uint32_t j = 0; j < a.top; ++j)
+                if (slots.id[j] == (int32_t)e) xe = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const uint32_t vec = (uint32_t)i * BLOCK + tid;
+            const uint32_t bits = vec < parts.nvec ? bits_of<VEC>(map, vec) : 0u;
+            if (bits != 0) mask_raw(raw[i], bits);
+            unpack_again(raw[i]);
+        }
+    }
+
+    float m = xe;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float v[VEC];
+        Raw::unpack(raw[i], v);
+        if ((uint32_t)i * BLOCK + tid < parts.nvec) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) m = fmaxf(m, v[j]);
+        }
+    }
+    m = block_largest<BLOCK>(m, lds);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) unpack_again(raw[i]);
+    const float shift = m > -INFINITY ? m : 0.0f;
+    float sum = tid < parts.extra ? __builtin_amdgcn_exp2f((xe - shift) * a.c) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float v[VEC];
+        Raw::unpack(raw[i], v);
+        float some = 0.0f;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            v[j] = __builtin_amdgcn_exp2f((v[j] - shift) * a.c);
+            some = some + v[j];
+        }
+        if ((uint32_t)i * BLOCK + tid < parts.nvec) sum = sum + some;
+        if constexpr (sizeof(T) == 4) raw[i] = typename Raw::type{v[0], v[1], v[2], v[3]};      // keeps the exponentials
+    }
+    sum = block_total<BLOCK>(sum, lds);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) unpack_again(raw[i]);
+    float loss;
+    const RowSums s = finish_row<BLOCK, TAIL>(a, RowStat{m, sum, 0.0f}, teach, id, q, at[0], own.first, used, lds, lds_stat, loss);
+    if (tid == 0 && o.loss != nullptr) o.loss[row] = loss;
+    const RowGrad g = row_grad<TAIL>(s);
+    const float mul = a.scale * (o.row_scale != nullptr ? o.row_scale[row] : o.grad_scale);
+    const bool none = g.m == -INFINITY;
+    // the exponentials are about the largest logit outside the ids (RENORM: of all), whose sum is `sum`
+    if (none) {                                                  // (zeros, whatever the logits hold)
+        float v[VEC] = {};
+        float d[1] = {0.0f};
+        if (tid < parts.extra) VecIO<T, 1>::store(out + e, d);
+        for (uint32_t vec = tid; vec < parts.nvec; vec += BLOCK) VecIO<T, VEC>::store(out + parts.head + (uint64_t)vec * VEC, v);
+        return;
+    }
+    const float k = sum == 0.0f ? 0.0f : g.out * mul / sum;
+    if (tid < parts.extra) {
+        float d[1] = {__builtin_amdgcn_exp2f((xe - shift) * a.c) * k};
+        VecIO<T, 1>::store(out + e, d);
+    }
+    // (the thread's number is read anew: what the compiler would keep of it, an index and an address a vector, costs the
+    // longest rows their last registers)
+    uint32_t again = tid;
+    asm volatile("" : "+v"(again));
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const uint32_t vec = (uint32_t)i * BLOCK + again;
+        float v[VEC];
+        Raw::unpack(raw[i], v);
+        if constexpr (sizeof(T) != 4) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) v[j] = __builtin_amdgcn_exp2f((v[j] - shift) * a.c);
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) v[j] = v[j] * k;
+        if (vec < parts.nvec) VecIO<T, VEC>::store(out + parts.head + (uint64_t)vec * VEC, v);
+    }
+    // the classes among the ids, over what the vectors' threads stored: every wave waits for its stores before the barrier
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (own.first) {
+        float d[1] = {own_grad(g, a, at[0], own.taken, mul)};
+        VecIO<T, 1>::store(out + id, d);
+    }
 }
 
 inline bool one_alignment(const void* x, const void* dx) {
@@ -380,20 +537,39 @@ inline bool one_alignment(const void* x, const void* dx) {
 }
 
 template <typename T>
-int ds_fused_typed(hipStream_t s, const T* x, T* dx, const DsArgs& a, const DsOut& o, uint64_t rows) {
+int ds_fwd_typed(hipStream_t s, const T* x, const DsArgs& a, DsOut o, uint64_t rows, bool tail) {
     constexpr int WIDE = WideVec<T>::value;
-    const bool wide = a.V >= 4 * WIDE && one_alignment(x, dx);
-    const dim3 grid((uint32_t)rows), block(kDsBlock);
-    if (wide && a.tail) hipLaunchKernelGGL((distill_fused_kernel<T, WIDE, true>), grid, block, 0, s, x, dx, a, o);
-    else if (wide) hipLaunchKernelGGL((distill_fused_kernel<T, WIDE, false>), grid, block, 0, s, x, dx, a, o);
-    else if (a.tail) hipLaunchKernelGGL((distill_fused_kernel<T, 1, true>), grid, block, 0, s, x, dx, a, o);
-    else hipLaunchKernelGGL((distill_fused_kernel<T, 1, false>), grid, block, 0, s, x, dx, a, o);
+    const bool wide = a.V >= 4 * WIDE;
+    const uint32_t vectors = wide ? a.V / WIDE : a.V;
+    o.parts = wide ? row_parts(rows, vectors) : 1u;
+    uint64_t slab = rows;
+    if (tail && vectors / o.parts + 1 > kMapBits / WIDE) {
+        // a part's classes have to fit the bit map: rows longer than it are cut, so many rows a launch as the parts' memory takes
+        o.parts = vectors / (kMapBits / WIDE - 1) + 1;
+        if (o.parts > kMaxParts) return set_error(AGRAD_EINVAL, "top-k distillation with a tail: %u classes are too many", a.V);
+        slab = kSharedParts / o.parts;
+    }
+    for (uint64_t r0 = 0; r0 < rows; r0 += slab) {
+        const uint64_t n = rows - r0 < slab ? rows - r0 : slab;
+        DsArgs b = a;
+        DsOut p = o;
+        b.ids += r0 * a.top;
+        b.values += r0 * a.top;
+        if (p.loss) p.loss += r0;
+        if (p.stats) p.stats += 4 * r0;
+        const dim3 grid((uint32_t)n * o.parts), block(kDsBlock);
+        const T* from = x + r0 * a.ld;
+        if (wide && tail) hipLaunchKernelGGL((distill_fwd_kernel<T, WIDE, true>), grid, block, 0, s, from, b, p);
+        else if (wide) hipLaunchKernelGGL((distill_fwd_kernel<T, WIDE, false>), grid, block, 0, s, from, b, p);
+        else if (tail) hipLaunchKernelGGL((distill_fwd_kernel<T, 1, true>), grid, block, 0, s, from, b, p);
+        else hipLaunchKernelGGL((distill_fwd_kernel<T, 1, false>), grid, block, 0, s, from, b, p);
+    }
     return check_hip(hipGetLastError(), "top-k distillation launch");
 }
 
 template <typename T>
-int ds_bwd_typed(hipStream_t s, const T* x, T* dx, const DsArgs& a, const float* dloss, const float* stats, uint32_t accumulate,
-                 uint64_t rows) {
+int ds_bwd_typed(hipStream_t s, const T* x, T* dx, const DsArgs& a, const float* dloss, const float* row_scale, float grad_scale,
+                 const float* stats, uint32_t accumulate, uint64_t rows, bool tail) {
     constexpr int WIDE = WideVec<T>::value;
     const bool wide = a.V >= 4 * WIDE && one_alignment(x, dx);
     const uint32_t vec = wide ? WIDE : 1, span = kDsBlock * kDsUnroll;
@@ -406,10 +582,52 @@ int ds_bwd_typed(hipStream_t s, const T* x, T* dx, const DsArgs& a, const float*
         b.ids += r0 * a.top;
         b.values += r0 * a.top;
         const dim3 grid((uint32_t)(n * chunks)), block(kDsBlock);
-        if (wide) hipLaunchKernelGGL((distill_bwd_kernel<T, WIDE>), grid, block, 0, s, x + r0 * a.ld, dx + r0 * a.ld, b, dloss + r0, stats + 4 * r0, accumulate, FastDiv32(chunks));
-        else hipLaunchKernelGGL((distill_bwd_kernel<T, 1>), grid, block, 0, s, x + r0 * a.ld, dx + r0 * a.ld, b, dloss + r0, stats + 4 * r0, accumulate, FastDiv32(chunks));
+#define AGRAD_DS(VEC, TAIL) hipLaunchKernelGGL((distill_bwd_kernel<T, VEC, TAIL>), grid, block, 0, s, x + r0 * a.ld, dx + r0 * a.ld, b, dloss ? dloss + r0 : nullptr, row_scale ? row_scale + r0 : nullptr, grad_scale, stats + 4 * r0, accumulate, FastDiv32(chunks))
+        if (wide && tail) AGRAD_DS(WIDE, true);
+        else if (wide) AGRAD_DS(WIDE, false);
+        else if (tail) AGRAD_DS(1, true);
+        else AGRAD_DS(1, false);
+#undef AGRAD_DS
     }
     return check_hip(hipGetLastError(), "top-k distillation backward launch");
+}
+
+template <typename T, bool TAIL>
+bool ds_held_launch(hipStream_t s, const T* x, T* dx, const DsArgs& a, const DsOut& o, uint64_t rows) {
+    constexpr int WIDE = WideVec<T>::value;
+    const uint32_t vectors = a.V / WIDE;
+    const dim3 grid((uint32_t)rows);
+#define AGRAD_DS(N, BLOCK) \
+    if (vectors <= (uint32_t)(N) * BLOCK) { hipLaunchKernelGGL((distill_held_kernel<T, WIDE, N, BLOCK, TAIL>), grid, dim3(BLOCK), 0, s, x, dx, a, o); return true; }
+    AGRAD_DS(1, 256) AGRAD_DS(4, 256) AGRAD_DS(4, 512) AGRAD_DS(8, 512) AGRAD_DS(12, 512) AGRAD_DS(16, 512) AGRAD_DS(20, 512)
+    AGRAD_DS(12, 1024) AGRAD_DS(16, 1024) AGRAD_DS(20, 1024)
+#undef AGRAD_DS
+    return false;
+}
+
+// Rows that no workgroup's registers hold (fp32 beyond 81920 classes, bf16 beyond 163840), rows of a few classes, and logits and
+// gradient at different places within 16 bytes: the forward pass, then the backward pass, over as many rows at a time as the
+// context's memory holds sums for.
+template <typename T>
+int ds_fused_typed(hipStream_t s, const T* x, T* dx, const DsArgs& a, const DsOut& o, uint64_t rows, bool tail) {
+    constexpr int WIDE = WideVec<T>::value;
+    if (a.V >= 4 * WIDE && one_alignment(x, dx)) {
+        if (tail ? ds_held_launch<T, true>(s, x, dx, a, o, rows) : ds_held_launch<T, false>(s, x, dx, a, o, rows))
+            return check_hip(hipGetLastError(), "top-k distillation step launch");
+    }
+    for (uint64_t r0 = 0; r0 < rows; r0 += kSumRows) {
+        const uint64_t n = rows - r0 < kSumRows ? rows - r0 : kSumRows;
+        DsArgs b = a;
+        DsOut p = o;
+        b.ids += r0 * a.top;
+        b.values += r0 * a.top;
+        if (p.loss) p.loss += r0;
+        p.stats = o.shared.sums;
+        if (int rc = ds_fwd_typed<T>(s, x + r0 * a.ld, b, p, n, tail)) return rc;
+        if (int rc = ds_bwd_typed<T>(s, x + r0 * a.ld, dx + r0 * a.ld, b, nullptr, o.row_scale ? o.row_scale + r0 : nullptr, o.grad_scale,
+                                     o.shared.sums, 0u, n, tail)) return rc;
+    }
+    return AGRAD_OK;
 }
 
 int ds_args(const char* what, int dtype, const void* logits, const int32_t* ids, const float* values, const void* dlogits,
@@ -423,21 +641,23 @@ int ds_args(const char* what, int dtype, const void* logits, const int32_t* ids,
         return set_error(AGRAD_EINVAL, "%s: log probabilities with a tail are taken as they are (teacher_scale 1)", what);
     if (rows != 0 && (logits == nullptr || ids == nullptr || values == nullptr)) return set_error(AGRAD_EINVAL, "%s: null operand", what);
     const float c = (float)((double)scale * 1.4426950408889634);
-    *a = DsArgs{ids, values, ld, V, top, scale, c, teacher_scale, mode == AGRAD_DISTILL_TAIL ? 1u : 0u, err_flag};
+    *a = DsArgs{ids, values, ld, V, top, scale, c, teacher_scale, err_flag};
     return AGRAD_OK;
 }
 
 }  // namespace
 
 int launch_distill_fwd(hipStream_t s, int dtype, const void* logits, const int32_t* ids, const float* values, float* loss, float* stats,
-                       uint64_t rows, uint32_t V, uint64_t ld, uint32_t top, float scale, float teacher_scale, int mode, int* err_flag) {
+                       uint64_t rows, uint32_t V, uint64_t ld, uint32_t top, float scale, float teacher_scale, int mode, int* err_flag,
+                       void* scratch) {
     DsArgs a;
     if (int rc = ds_args("top-k distillation", dtype, logits, ids, values, nullptr, rows, V, ld, top, scale, teacher_scale, mode, err_flag, &a)) return rc;
     if (rows == 0) return AGRAD_OK;
     if (loss == nullptr) return set_error(AGRAD_EINVAL, "top-k distillation: null loss");
-    const DsOut o{loss, stats, nullptr, 0.0f};
-    if (dtype == AGRAD_F32) return ds_fwd_typed<float>(s, (const float*)logits, a, o, rows);
-    return ds_fwd_typed<bf16_t>(s, (const bf16_t*)logits, a, o, rows);
+    const DsOut o{loss, stats, nullptr, 0.0f, shared_rows(scratch), 1u};
+    const bool tail = mode == AGRAD_DISTILL_TAIL;
+    if (dtype == AGRAD_F32) return ds_fwd_typed<float>(s, (const float*)logits, a, o, rows, tail);
+    return ds_fwd_typed<bf16_t>(s, (const bf16_t*)logits, a, o, rows, tail);
 }
 
 int launch_distill_bwd(hipStream_t s, int dtype, const void* logits, const int32_t* ids, const float* values, const float* dloss,
@@ -449,20 +669,22 @@ int launch_distill_bwd(hipStream_t s, int dtype, const void* logits, const int32
     if (rows == 0) return AGRAD_OK;
     if (dloss == nullptr || stats == nullptr || dlogits == nullptr) return set_error(AGRAD_EINVAL, "top-k distillation backward: null operand");
     const uint32_t acc = (flags & AGRAD_ACC_INPUT_GRAD) ? 1u : 0u;
-    if (dtype == AGRAD_F32) return ds_bwd_typed<float>(s, (const float*)logits, (float*)dlogits, a, dloss, stats, acc, rows);
-    return ds_bwd_typed<bf16_t>(s, (const bf16_t*)logits, (bf16_t*)dlogits, a, dloss, stats, acc, rows);
+    const bool tail = mode == AGRAD_DISTILL_TAIL;
+    if (dtype == AGRAD_F32) return ds_bwd_typed<float>(s, (const float*)logits, (float*)dlogits, a, dloss, nullptr, 0.0f, stats, acc, rows, tail);
+    return ds_bwd_typed<bf16_t>(s, (const bf16_t*)logits, (bf16_t*)dlogits, a, dloss, nullptr, 0.0f, stats, acc, rows, tail);
 }
 
 int launch_distill_fused(hipStream_t s, int dtype, const void* logits, const int32_t* ids, const float* values, float* loss,
                          const float* row_scale, void* dlogits, uint64_t rows, uint32_t V, uint64_t ld, uint32_t top, float scale,
-                         float teacher_scale, float grad_scale, int mode, int* err_flag) {
+                         float teacher_scale, float grad_scale, int mode, int* err_flag, void* scratch) {
     DsArgs a;
     if (int rc = ds_args("top-k distillation step", dtype, logits, ids, values, dlogits, rows, V, ld, top, scale, teacher_scale, mode, err_flag, &a)) return rc;
     if (rows == 0) return AGRAD_OK;
     if (dlogits == nullptr) return set_error(AGRAD_EINVAL, "top-k distillation step: null gradient");
-    const DsOut o{loss, nullptr, row_scale, grad_scale};
-    if (dtype == AGRAD_F32) return ds_fused_typed<float>(s, (const float*)logits, (float*)dlogits, a, o, rows);
-    return ds_fused_typed<bf16_t>(s, (const bf16_t*)logits, (bf16_t*)dlogits, a, o, rows);
+    const DsOut o{loss, nullptr, row_scale, grad_scale, shared_rows(scratch), 1u};
+    const bool tail = mode == AGRAD_DISTILL_TAIL;
+    if (dtype == AGRAD_F32) return ds_fused_typed<float>(s, (const float*)logits, (float*)dlogits, a, o, rows, tail);
+    return ds_fused_typed<bf16_t>(s, (const bf16_t*)logits, (bf16_t*)dlogits, a, o, rows, tail);
 }
 
 }  // namespace agrad

@@ -193,12 +193,13 @@ int launch_logprobs_bwd(hipStream_t s, int dtype, const void* logits, const int3
                         uint32_t V, uint64_t ld, float scale, uint32_t flags, int* err_flag);
 // distill.hip: the divergence from a teacher's top logits; stats [rows, 4] carries what the backward call needs
 int launch_distill_fwd(hipStream_t s, int dtype, const void* logits, const int32_t* ids, const float* values, float* loss, float* stats,
-                       uint64_t rows, uint32_t V, uint64_t ld, uint32_t top, float scale, float teacher_scale, int mode, int* err_flag);
+                       uint64_t rows, uint32_t V, uint64_t ld, uint32_t top, float scale, float teacher_scale, int mode, int* err_flag,
+                       void* scratch);
 int launch_distill_bwd(hipStream_t s, int dtype, const void* logits, const int32_t* ids, const float* values, const float* dloss,
                        const float* stats, void* dlogits, uint64_t rows, uint32_t V, uint64_t ld, uint32_t top, float scale,
                        float teacher_scale, int mode, uint32_t flags, int* err_flag);
 int launch_distill_fused(hipStream_t s, int dtype, const void* logits, const int32_t* ids, const float* values, float* loss,
                          const float* row_scale, void* dlogits, uint64_t rows, uint32_t V, uint64_t ld, uint32_t top, float scale,
-                         float teacher_scale, float grad_scale, int mode, int* err_flag);
+                         float teacher_scale, float grad_scale, int mode, int* err_flag, void* scratch);
 
 }  // namespace agrad

@@ -604,7 +604,8 @@ uint64_t shared_rows_bytes() { return kSharedRowsBytes; }
 SharedRows shared_rows(void* scratch) {
     char* at = static_cast<char*>(scratch);
     return SharedRows{reinterpret_cast<float*>(at), reinterpret_cast<unsigned long long*>(at + 16ull * kSharedParts),
-                      reinterpret_cast<uint32_t*>(at + (16ull + 8ull * AGRAD_MAX_TOP) * kSharedParts)};
+                      reinterpret_cast<uint32_t*>(at + (16ull + 8ull * AGRAD_MAX_TOP) * kSharedParts),
+                      reinterpret_cast<float*>(at + (16ull + 8ull * AGRAD_MAX_TOP + 4ull) * kSharedParts)};
 }
 
 // Parts of a row: as many as make 512 workgroups of all rows, or 1024 where the parts stay longer than 4096 vectors, but

@@ -63,6 +63,11 @@ __device__ __forceinline__ float absorb_stat(RowStat& a, const float (&v)[N], fl
     return top;
 }
 
+// Tells the compiler that a packed vector may have changed: what it unpacked from it before is unpacked again where it is
+// next needed, instead of being kept in twice the registers.
+__device__ __forceinline__ void unpack_again(u32x4& r) { asm volatile("" : "+v"(r.x), "+v"(r.y), "+v"(r.z), "+v"(r.w)); }
+template <typename R> __device__ __forceinline__ void unpack_again(R&) {}
+
 // how a row of V elements that starts at `base` splits into single elements, aligned vectors, single elements
 template <typename T, int VEC>
 struct RowParts {
@@ -94,8 +99,10 @@ struct SharedRows {
     float* stats;             // [kSharedParts, 4]
     unsigned long long* keys; // [kSharedParts, AGRAD_MAX_TOP]
     uint32_t* tickets;        // [kSharedParts]
+    float* sums;              // [kSumRows, 4], what a first pass over a row leaves for a second one of the same call
 };
-constexpr uint64_t kSharedRowsBytes = (uint64_t)kSharedParts * (16 + 8 * AGRAD_MAX_TOP + 4);
+constexpr uint64_t kSumRows = 65536;
+constexpr uint64_t kSharedRowsBytes = (uint64_t)kSharedParts * (16 + 8 * AGRAD_MAX_TOP + 4) + kSumRows * 16;
 
 template <typename V>
 __device__ __forceinline__ void put_shared(V* to, V value) { __hip_atomic_store(to, value, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }

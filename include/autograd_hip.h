@@ -537,9 +537,9 @@ int agrad_token_logprobs_backward(agrad_ctx* ctx, int dtype, const void* logits,
  * and counts as unused.  A value of -inf is a slot of probability 0.  A row without used slots, or whose logits are
  * all -inf, has loss 0 and a zero gradient; a class at -inf that the teacher gives mass to makes the loss +inf (its
  * gradient is finite); NaN or +inf makes a row NaN.
- *   forward   loss, and stats[rows, 4], fp32, for the backward call (may be NULL): the lse of z (-inf: no
- *             gradient), the lse of the teacher's side (RENORM) or of z outside the ids (TAIL), W, and the factor
- *             of the classes outside the ids: W, or W p_rest - q_rest
+ *   forward   loss, and stats[rows, 4], fp32, for the backward call (may be NULL): the row's largest logit (-inf:
+ *             no gradient), the logarithm of the sum of exp(z) about it, the teacher's lse (RENORM) or log p_rest
+ *             (TAIL; -inf: no class outside), sum q
  *   backward  dlogits (+)= the gradient * dloss[r]
  *   fused     loss (may be NULL) and dlogits = the gradient * (row_scale[r], or grad_scale if row_scale is NULL)
  *             in one launch that reads the logits once where a row fits a workgroup's registers
