@@ -300,7 +300,7 @@ __device__ __forceinline__ void ds_store(T* to, float (&d)[VEC], uint32_t accumu
 #pragma unroll
         for (int k = 0; k < VEC; ++k) d[k] = old[k] + d[k];
     }
-    VecIO<T, VEC>::store(to, d);
+    store_grad<T, VEC>(to, d);
 }
 
 template <typename T, int VEC, bool TAIL>
@@ -405,7 +405,7 @@ distill_bwd_kernel(const T* x, T* dx, const DsArgs a, const float* dloss, const 
 template <typename T, int VEC, int NV, int BLOCK, bool TAIL>
 __global__ void __launch_bounds__(BLOCK)
 distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
-    __shared__ __align__(16) uint32_t map[TAIL ? (NV * BLOCK * VEC + 31) / 32 + 4 : 4];
+    __shared__ __align__(16) uint32_t map[TAIL ? NV * BLOCK * VEC / 32 : 4];
     __shared__ Slots slots;
     __shared__ float lds[BLOCK / kWave];
     __shared__ RowStat lds_stat[BLOCK / kWave];
@@ -432,7 +432,7 @@ distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
     const int32_t id = slot_id(a, row, tid, true);
     float at[1];
     VecIO<T, 1>::load(base + (id >= 0 ? id : 0), at);
-    if (TAIL) clear_map<BLOCK>(map, parts.nvec * VEC);
+    if (TAIL) clear_map<BLOCK>(map, (uint32_t)(NV * BLOCK * VEC));
     const bool used = __syncthreads_or(id >= 0) != 0;
     if (TAIL) mark(map, id, parts.head, parts.nvec * VEC);
     const Teacher teach = teacher_row<BLOCK, TAIL>(a, row, id, lds);
@@ -447,53 +447,42 @@ distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
         if (tid < parts.extra)
             for (uint32_t j = 0; j < a.top; ++j)
                 if (slots.id[j] == (int32_t)e) xe = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const uint32_t vec = (uint32_t)i * BLOCK + tid;
-            const uint32_t bits = vec < parts.nvec ? bits_of<VEC>(map, vec) : 0u;
-            if (bits != 0) mask_raw(raw[i], bits);
-            unpack_again(raw[i]);
-        }
     }
 
-    float m = xe;
+    // One pass in the order of the loads, so that its exponentials are computed while the later vectors are on their way: the
+    // maximum first and the exponentials after it would leave the memory idle for a third of a long row's time.
+    RowStat t = empty_stat();
+    uint32_t bits = TAIL ? bits_of<VEC>(map, tid) : 0u;            // (the map covers all NV vectors of a thread)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        float v[VEC];
-        Raw::unpack(raw[i], v);
-        if ((uint32_t)i * BLOCK + tid < parts.nvec) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) m = fmaxf(m, v[j]);
+        const uint32_t vec = (uint32_t)i * BLOCK + tid;
+        uint32_t next = 0;
+        if (TAIL && i + 1 < NV) {
+            next = bits_of<VEC>(map, vec + BLOCK);
+            asm volatile("" ::: "memory");                         // (one vector's bits ahead, not all of them)
         }
-    }
-    m = block_largest<BLOCK>(m, lds);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) unpack_again(raw[i]);
-    const float shift = m > -INFINITY ? m : 0.0f;
-    float sum = tid < parts.extra ? __builtin_amdgcn_exp2f((xe - shift) * a.c) : 0.0f;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        float v[VEC];
-        Raw::unpack(raw[i], v);
-        float some = 0.0f;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            v[j] = __builtin_amdgcn_exp2f((v[j] - shift) * a.c);
-            some = some + v[j];
+        if (vec < parts.nvec) {
+            if (TAIL && bits != 0) mask_raw(raw[i], bits);
+            float v[VEC];
+            Raw::unpack(raw[i], v);
+            absorb_stat<false, VEC>(t, v, a.c);
         }
-        if ((uint32_t)i * BLOCK + tid < parts.nvec) sum = sum + some;
-        if constexpr (sizeof(T) == 4) raw[i] = typename Raw::type{v[0], v[1], v[2], v[3]};      // keeps the exponentials
+        unpack_again(raw[i]);
+        bits = next;
     }
-    sum = block_total<BLOCK>(sum, lds);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) unpack_again(raw[i]);
+    {
+        float v[1] = {xe};
+        absorb_stat<false, 1>(t, v, a.c);
+    }
+    t = block_stat<BLOCK, false>(t, a.c, lds_stat);
     float loss;
-    const RowSums s = finish_row<BLOCK, TAIL>(a, RowStat{m, sum, 0.0f}, teach, id, q, at[0], own.first, used, lds, lds_stat, loss);
+    const RowSums s = finish_row<BLOCK, TAIL>(a, t, teach, id, q, at[0], own.first, used, lds, lds_stat, loss);
     if (tid == 0 && o.loss != nullptr) o.loss[row] = loss;
     const RowGrad g = row_grad<TAIL>(s);
     const float mul = a.scale * (o.row_scale != nullptr ? o.row_scale[row] : o.grad_scale);
     const bool none = g.m == -INFINITY;
-    // the exponentials are about the largest logit outside the ids (RENORM: of all), whose sum is `sum`
+    // exponentials about the largest logit outside the ids (RENORM: of all)
+    const float shift = t.m > -INFINITY ? t.m : 0.0f;
     if (none) {                                                  // (zeros, whatever the logits hold)
         float v[VEC] = {};
         float d[1] = {0.0f};
@@ -501,7 +490,7 @@ distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
         for (uint32_t vec = tid; vec < parts.nvec; vec += BLOCK) VecIO<T, VEC>::store(out + parts.head + (uint64_t)vec * VEC, v);
         return;
     }
-    const float k = sum == 0.0f ? 0.0f : g.out * mul / sum;
+    const float k = t.s == 0.0f ? 0.0f : g.out * mul / t.s;
     if (tid < parts.extra) {
         float d[1] = {__builtin_amdgcn_exp2f((xe - shift) * a.c) * k};
         VecIO<T, 1>::store(out + e, d);
@@ -515,13 +504,9 @@ distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
         const uint32_t vec = (uint32_t)i * BLOCK + again;
         float v[VEC];
         Raw::unpack(raw[i], v);
-        if constexpr (sizeof(T) != 4) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) v[j] = __builtin_amdgcn_exp2f((v[j] - shift) * a.c);
-        }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = v[j] * k;
-        if (vec < parts.nvec) VecIO<T, VEC>::store(out + parts.head + (uint64_t)vec * VEC, v);
+        for (int j = 0; j < VEC; ++j) v[j] = __builtin_amdgcn_exp2f((v[j] - shift) * a.c) * k;
+        if (vec < parts.nvec) store_grad<T, VEC>(out + parts.head + (uint64_t)vec * VEC, v);
     }
     // the classes among the ids, over what the vectors' threads stored: every wave waits for its stores before the barrier
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");

@@ -491,7 +491,7 @@ __device__ __forceinline__ void lp_store(T* to, float (&d)[VEC], uint32_t accumu
 #pragma unroll
         for (int k = 0; k < VEC; ++k) d[k] = old[k] + d[k];
     }
-    VecIO<T, VEC>::store(to, d);
+    store_grad<T, VEC>(to, d);
 }
 
 template <typename T, int VEC>

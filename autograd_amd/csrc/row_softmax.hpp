@@ -39,6 +39,22 @@ __device__ __forceinline__ RowStat merge_stat(const RowStat& a, const RowStat& b
     return RowStat{M, x.s + y.s, ENT ? x.d + y.d : 0.0f};
 }
 
+// A vector of a gradient to memory.  bf16: the hardware's pair conversion alone (a NaN comes out as the hardware's quiet NaN, not
+// with its payload; the two compares a pair that keep it are a tenth of such a kernel's instructions).
+template <typename T, int VEC>
+__device__ __forceinline__ void store_grad(T* p, const float (&v)[VEC]) { VecIO<T, VEC>::store(p, v); }
+template <>
+__device__ __forceinline__ void store_grad<bf16_t, 8>(bf16_t* p, const float (&v)[8]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const f32x2_hw pair = {v[2 * i], v[2 * i + 1]};
+        w[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, bf16x2_hw));
+    }
+    u32x4 t; t.x = w[0]; t.y = w[1]; t.z = w[2]; t.w = w[3];
+    __builtin_nontemporal_store(t, reinterpret_cast<u32x4*>(p));
+}
+
 // one group of N values into a running part
 // (returns the largest of them, -inf if none is a number)
 template <bool ENT, int N>
@@ -139,7 +155,7 @@ struct Stretch {
 SharedRows shared_rows(void* scratch);                         // the three arrays in that memory
 uint32_t row_parts(uint64_t rows, uint32_t vectors);           // how many workgroups take a row
 
-// ---- workgroup reductions: the lanes of a wave, then the waves in order; every thread gets the result ----
+// ---- workgroup reductions: the lanes of a wave, then the waves, in a fixed order; every thread gets the result ----
 __device__ __forceinline__ float wave_max(float v) {
     v = fmaxf(v, dpp_move<kDppQuadXor1>(v));
     v = fmaxf(v, dpp_move<kDppQuadXor2>(v));
@@ -162,6 +178,15 @@ __device__ __forceinline__ RowStat block_stat(RowStat a, float c, RowStat* lds) 
     if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = a;
     __syncthreads();
     constexpr int W = BLOCK / kWave;
+    if constexpr (W > 4) {                       // (sixteen waves' sums at once would be 48 registers of each thread)
+        const uint32_t lane = threadIdx.x % kWave;
+        a = lane < (uint32_t)W ? lds[lane] : empty_stat();
+        a = about<ENT>(a, wave_max(a.m), c);
+        if constexpr (ENT) wave_sum2(a.s, a.d);
+        else a.s = wave_sum(a.s);
+        __syncthreads();
+        return a;
+    }
     RowStat each[W];
     float M = -INFINITY;
 #pragma unroll
