@@ -220,25 +220,37 @@ distill_fwd_kernel(const T* __restrict__ x, const DsArgs a, const DsOut o) {
     const RowParts<T, VEC> parts(base, a.V);
     const Stretch part(parts.nvec, nth, o.parts);
     const T* body = base + parts.head;
-    const int32_t id = slot_id(a, row, k, nth == 0);
-    float at[1];
-    VecIO<T, 1>::load(base + (id >= 0 ? id : 0), at);
-    if (k < AGRAD_MAX_TOP) slots.id[k] = id;
-    if (TAIL) {
-        const uint32_t classes = (part.hi - part.lo) * VEC;
-        clear_map<kDsBlock>(map, classes);
-        __syncthreads();
-        mark(map, id, parts.head + part.lo * VEC, classes);
-        __syncthreads();
-    }
-    RowStat t = empty_stat();
-    for (uint32_t i0 = part.lo + k; i0 < part.hi; i0 += kDsBlock * kDsUnroll) {
-        typename Raw::type raw[kDsUnroll];
+    // a slot's class and value, then the first vectors, then the slot's logit: the teacher's side is done while they come
+    const uint64_t slot_at = (uint64_t)row * a.top + (k < a.top ? k : 0u);
+    const int32_t asked = a.ids[slot_at];
+    const float given = a.values[slot_at];
+    typename Raw::type raw[kDsUnroll];
+    auto read = [&](uint32_t i0) {
 #pragma unroll
         for (int u = 0; u < kDsUnroll; ++u) {
             const uint32_t i = i0 + u * kDsBlock;
             raw[u] = Raw::load(body + (uint64_t)(i < part.hi ? i : part.lo) * VEC);
         }
+    };
+    uint32_t i0 = part.lo + k;
+    if (i0 < part.hi) read(i0);
+    const int32_t id = k < a.top && asked >= 0 && (uint32_t)asked < a.V ? asked : -1;
+    if (nth == 0 && k < a.top && id != asked && asked != -1) *a.err_flag = 1;
+    float at[1];
+    VecIO<T, 1>::load(base + (id >= 0 ? id : 0), at);
+    if (k < AGRAD_MAX_TOP) slots.id[k] = id;
+    const uint32_t classes = (part.hi - part.lo) * VEC;
+    if (TAIL) clear_map<kDsBlock>(map, classes);
+    const bool used = __syncthreads_or(id >= 0) != 0;
+    if (TAIL) mark(map, id, parts.head + part.lo * VEC, classes);
+    const Teacher teach = teacher_row<kDsBlock, TAIL>(a, id >= 0 ? given : -INFINITY, id, lds);
+    const float q = expf(teach.log_q);
+    bool first = id >= 0;
+    if (TAIL && first)
+        for (uint32_t j = 0; j < k; ++j) first = first && slots.id[j] != id;
+    __syncthreads();
+    RowStat t = empty_stat();
+    while (i0 < part.hi) {
 #pragma unroll
         for (int u = 0; u < kDsUnroll; ++u) {
             const uint32_t i = i0 + u * kDsBlock;
@@ -251,6 +263,8 @@ distill_fwd_kernel(const T* __restrict__ x, const DsArgs a, const DsOut o) {
             Raw::unpack(raw[u], v);
             absorb_stat<false, VEC>(t, v, a.c);
         }
+        i0 += kDsBlock * kDsUnroll;
+        if (i0 < part.hi) read(i0);
     }
     if (nth == 0 && k < parts.extra) {
         const uint32_t e = parts.extra_at(k);
@@ -276,12 +290,6 @@ distill_fwd_kernel(const T* __restrict__ x, const DsArgs a, const DsOut o) {
         }
         t = block_stat<kDsBlock, false>(t, a.c, lds_stat);
     }
-    const bool used = __syncthreads_or(id >= 0) != 0;
-    const Teacher teach = teacher_row<kDsBlock, TAIL>(a, id >= 0 ? a.values[(uint64_t)row * a.top + k] : -INFINITY, id, lds);
-    const float q = expf(teach.log_q);
-    bool first = id >= 0;
-    if (TAIL && first)
-        for (uint32_t j = 0; j < k; ++j) first = first && slots.id[j] != id;
     float base_own, term, loss;
     const RowStat own = ids_side<kDsBlock, TAIL>(a, teach, id, q, at[0], first, base_own, term, lds);
     const RowSums s = finish_row<TAIL>(a, t, own, base_own, term, teach, used, loss);
@@ -294,7 +302,7 @@ distill_fwd_kernel(const T* __restrict__ x, const DsArgs a, const DsOut o) {
     }
 }
 
-// ---- backward: a workgroup a chunk of a row ------------------------------------------------------------------
+// ---- backward ----------------------------------------------------------------------------------------------
 template <typename T, int VEC>
 __device__ __forceinline__ void ds_store(T* to, float (&d)[VEC], uint32_t accumulate) {
     if (accumulate) {
@@ -306,100 +314,101 @@ __device__ __forceinline__ void ds_store(T* to, float (&d)[VEC], uint32_t accumu
     store_grad<T, VEC>(to, d);
 }
 
-template <typename T, int VEC, bool TAIL>
+// A wave takes 64 * U neighbouring vectors of a row and needs no other: it looks through the row's ids for those of its classes,
+// writes its vectors as if there were none, and stores over them, by the lane that stored the vector (in order).  One
+// vector a lane is best where a wave's share of looking is small: 64 ids, 8192 rows of 151936 bf16 802 us (two: 818, four:
+// 872); with 128 ids of 32768 classes two are, 454 us (one: 503), and with 1000 fp32 classes, 108 us (118).  A workgroup that
+// collects the ids of its 16 KB in LDS took 908, 491 and 143 us.
+template <typename T, int VEC, int U, bool TAIL>
 __global__ void __launch_bounds__(kDsBlock)
 distill_bwd_kernel(const T* x, T* dx, const DsArgs a, const float* dloss, const float* row_scale, float grad_scale, const float* stats,
-                   uint32_t accumulate, const FastDiv32 chunks) {
-    // the chunk's ids in slot order, then what is stored over their classes, and by which thread: the one that stores the vector
-    __shared__ Slots here;
-    __shared__ float value[AGRAD_MAX_TOP];
-    __shared__ uint32_t owner[AGRAD_MAX_TOP];
-    __shared__ uint32_t in_wave[kDsBlock / kWave];
+                   uint32_t accumulate, const FastDiv32 chunks, uint32_t waves) {
     typedef RawVec<T, VEC> Raw;
-    const uint32_t row = chunks.div(blockIdx.x), chunk = blockIdx.x - row * chunks.d, tid = threadIdx.x;
+    const uint32_t lane = threadIdx.x % kWave;
+    const uint32_t wave = blockIdx.x * (kDsBlock / kWave) + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
+    if (wave >= waves) return;
+    const uint32_t row = chunks.div(wave), chunk = wave - row * chunks.d;
     const T* base = x + (uint64_t)row * a.ld;
     T* out = dx + (uint64_t)row * a.ld;
     const RowParts<T, VEC> parts(base, a.V);
-    constexpr uint32_t span = kDsBlock * kDsUnroll;                  // vectors of a chunk
-    const uint32_t i0 = chunk * span + tid;
-    typename Raw::type raw[kDsUnroll];
+    constexpr uint32_t span = kWave * U;
+    const uint32_t lo = chunk * span;
+    // slots lane and lane + 64
+    static_assert(AGRAD_MAX_TOP == 2 * kWave, "");
+    const int32_t* ids = a.ids + (uint64_t)row * a.top;
+    const int32_t id0 = lane < a.top ? ids[lane] : -1, id1 = lane + kWave < a.top ? ids[lane + kWave] : -1;
+    typename Raw::type raw[U];
 #pragma unroll
-    for (int u = 0; u < kDsUnroll; ++u) {
-        const uint32_t i = i0 + u * kDsBlock;
+    for (int u = 0; u < U; ++u) {
+        const uint32_t i = lo + u * kWave + lane;
         raw[u] = Raw::load(base + parts.head + (uint64_t)(i < parts.nvec ? i : 0u) * VEC);
     }
-    const uint32_t extra = chunk == 0 ? parts.extra : 0u, e = parts.extra_at(tid);
+    const uint32_t extra = chunk == 0 ? parts.extra : 0u, e = parts.extra_at(lane);
     float xe[1];
-    VecIO<T, 1>::load(base + (tid < extra ? e : 0u), xe);
+    VecIO<T, 1>::load(base + (lane < extra ? e : 0u), xe);
     const float* st = stats + (uint64_t)row * 4;
     const RowGrad g = row_grad<TAIL>(RowSums{st[0], st[1], TAIL ? st[2] : -INFINITY, st[3]});
     const float mul = a.scale * (dloss != nullptr ? dloss[row] : row_scale != nullptr ? row_scale[row] : grad_scale);
     const bool none = g.m == -INFINITY;
 
-    const int32_t id = slot_id(a, row, tid, chunk == 0 && dloss != nullptr);
-    const uint32_t vec = id >= (int32_t)parts.head ? ((uint32_t)id - parts.head) / VEC : 0xffffffffu;
-    const bool in_vectors = vec < parts.nvec;
-    const bool mine = !none && id >= 0 && (in_vectors ? vec / span == chunk : chunk == 0);
-    const uint64_t lanes = __ballot(mine);
-    if (tid % kWave == 0) in_wave[tid / kWave] = (uint32_t)__popcll(lanes);
-    if (tid < AGRAD_MAX_TOP) here.id[tid] = -1;
-    __syncthreads();
-    const uint32_t n = in_wave[0] + in_wave[1];
-    if (n != 0) {                                                   // (uniform)
-        uint32_t place = 0;
-        float at[1], old[1], q = 0.0f;
-        if (mine) {
-            place = (tid >= kWave ? in_wave[0] : 0u) + (uint32_t)__popcll(lanes & ((1ull << (tid % kWave)) - 1));
-            const float u = a.values[(uint64_t)row * a.top + tid];
+    // who stores the class, if this wave does
+    auto owner = [&](int32_t id) {
+        const uint32_t v = (uint32_t)id;
+        if (id < 0 || v >= a.V) return 0xffffffffu;
+        const uint32_t vec = v >= parts.head ? (v - parts.head) / VEC : 0xffffffffu;
+        if (vec < parts.nvec) return vec - lo < span ? vec % kWave : 0xffffffffu;
+        return chunk == 0 ? (v < parts.head ? v : parts.head + (v - parts.tail_start)) : 0xffffffffu;
+    };
+    if (chunk == 0 && dloss != nullptr && ((id0 != -1 && (uint32_t)id0 >= a.V) || (id1 != -1 && (uint32_t)id1 >= a.V))) *a.err_flag = 1;
+    const uint32_t who0 = none ? 0xffffffffu : owner(id0), who1 = none ? 0xffffffffu : owner(id1);
+    const uint64_t mine0 = __ballot(who0 != 0xffffffffu), mine1 = __ballot(who1 != 0xffffffffu);
+    float at0[1] = {0.0f}, at1[1] = {0.0f}, old0[1] = {0.0f}, old1[1] = {0.0f}, q0 = 0.0f, q1 = 0.0f;
+    if ((mine0 | mine1) != 0) {
+        auto ask = [&](bool has, int32_t id, uint32_t slot, float (&at)[1], float (&old)[1], float& q) {
+            if (!has) return;
+            const float u = a.values[(uint64_t)row * a.top + slot];
             VecIO<T, 1>::load(base + id, at);
             if (accumulate) VecIO<T, 1>::load(out + id, old);
             q = TAIL ? expf(u) : expf(u * a.teacher_scale - st[2]);
-            here.id[place] = id;
-            here.q[place] = q;
-        }
-        __syncthreads();
-        if (mine) {
-            const Own own = own_slot(here, n, place, id);
-            float d = own_grad(g, a, at[0], own.taken, mul);
-            if (accumulate) d = old[0] + d;
-            value[place] = d;
-            const uint32_t who = in_vectors ? vec % kDsBlock : ((uint32_t)id < parts.head ? (uint32_t)id : parts.head + ((uint32_t)id - parts.tail_start));
-            owner[place] = own.first ? who : 0xffffffffu;
-        }
+        };
+        ask(who0 != 0xffffffffu, id0, lane, at0, old0, q0);
+        ask(who1 != 0xffffffffu, id1, lane + kWave, at1, old1, q1);
     }
-    __syncthreads();
 
-    if (none) {                                                  // (zeros, whatever the logits hold)
-        if (accumulate) return;
-        float v[VEC] = {};
-        float d[1] = {0.0f};
-        if (tid < extra) VecIO<T, 1>::store(out + e, d);
-#pragma unroll
-        for (int u = 0; u < kDsUnroll; ++u)
-            if (i0 + u * kDsBlock < parts.nvec) VecIO<T, VEC>::store(out + parts.head + (uint64_t)(i0 + u * kDsBlock) * VEC, v);
-        return;
-    }
-    const float k = g.out * mul, b = -g.out_log * kLog2eHi;
-    if (tid < extra) {
-        float d[1] = {__builtin_amdgcn_exp2f(__builtin_fmaf(xe[0] - g.m, a.c, b)) * k};
+    const float k = none ? 0.0f : g.out * mul, b = -g.out_log * kLog2eHi;
+    if (none && accumulate) return;
+    if (lane < extra) {
+        float d[1] = {none ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(xe[0] - g.m, a.c, b)) * k};
         ds_store<T, 1>(out + e, d, accumulate);
     }
 #pragma unroll
-    for (int u = 0; u < kDsUnroll; ++u) {
-        const uint32_t i = i0 + u * kDsBlock;
+    for (int u = 0; u < U; ++u) {
+        const uint32_t i = lo + u * kWave + lane;
         if (i >= parts.nvec) continue;
         float v[VEC];
         Raw::unpack(raw[u], v);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(v[j] - g.m, a.c, b)) * k;
+        for (int j = 0; j < VEC; ++j) v[j] = none ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(v[j] - g.m, a.c, b)) * k;
         ds_store<T, VEC>(out + parts.head + (uint64_t)i * VEC, v, accumulate);
     }
-    // (a later store of the same thread to the same place: in order)
-    for (uint32_t j = 0; j < n; ++j) {
-        if (owner[j] != tid) continue;
-        float d[1] = {value[j]};
-        VecIO<T, 1>::store(out + here.id[j], d);
-    }
+    auto of_lane = [](float v, int l) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), l)); };
+    auto put = [&](uint64_t these, int32_t id, uint32_t who, const float (&at)[1], const float (&old)[1], bool upper) {
+        for (; these != 0; these &= these - 1) {
+            const int l = (int)__builtin_ctzll(these);
+            const int32_t which = __builtin_amdgcn_readlane(id, l);
+            const uint64_t same0 = __ballot(id0 == which), same1 = __ballot(id1 == which);
+            // a class that the row names twice: its first slot stores it
+            if (upper ? same0 != 0 || __builtin_ctzll(same1) != l : __builtin_ctzll(same0) != l) continue;
+            float taken = 0.0f;
+            for (uint64_t w = same0; w != 0; w &= w - 1) taken = taken + of_lane(q0, (int)__builtin_ctzll(w));
+            for (uint64_t w = same1; w != 0; w &= w - 1) taken = taken + of_lane(q1, (int)__builtin_ctzll(w));
+            float d[1] = {own_grad(g, a, of_lane(at[0], l), taken, mul)};
+            if (accumulate) d[0] = of_lane(old[0], l) + d[0];
+            if (lane == (uint32_t)__builtin_amdgcn_readlane((int)who, l)) VecIO<T, 1>::store(out + which, d);
+        }
+    };
+    put(mine0, id0, who0, at0, old0, false);
+    put(mine1, id1, who1, at1, old1, true);
 }
 
 // ---- loss and gradient in one launch, the row in registers in between ------------------------------------------
@@ -583,21 +592,23 @@ int ds_bwd_typed(hipStream_t s, const T* x, T* dx, const DsArgs& a, const float*
                  const float* stats, uint32_t accumulate, uint64_t rows, bool tail) {
     constexpr int WIDE = WideVec<T>::value;
     const bool wide = a.V >= 4 * WIDE && one_alignment(x, dx);
-    const uint32_t vec = wide ? WIDE : 1, span = kDsBlock * kDsUnroll;
+    const bool two = a.top > kWave || a.V / (wide ? WIDE : 1) <= 8 * kWave;
+    const uint32_t vec = wide ? WIDE : 1, span = kWave * (two ? 2 : 1);
     const uint32_t chunks = (a.V / vec + span - 1) / span;
-    uint64_t max_rows = 0x00ffffffull / chunks;                  // workgroups of a launch: 2^32 threads
+    uint64_t max_rows = 0x03ffffffull / chunks;                  // waves of a launch: 2^32 threads
     if (max_rows == 0) max_rows = 1;
     for (uint64_t r0 = 0; r0 < rows; r0 += max_rows) {
         const uint64_t n = rows - r0 < max_rows ? rows - r0 : max_rows;
         DsArgs b = a;
         b.ids += r0 * a.top;
         b.values += r0 * a.top;
-        const dim3 grid((uint32_t)(n * chunks)), block(kDsBlock);
-#define AGRAD_DS(VEC, TAIL) hipLaunchKernelGGL((distill_bwd_kernel<T, VEC, TAIL>), grid, block, 0, s, x + r0 * a.ld, dx + r0 * a.ld, b, dloss ? dloss + r0 : nullptr, row_scale ? row_scale + r0 : nullptr, grad_scale, stats + 4 * r0, accumulate, FastDiv32(chunks))
-        if (wide && tail) AGRAD_DS(WIDE, true);
-        else if (wide) AGRAD_DS(WIDE, false);
-        else if (tail) AGRAD_DS(1, true);
-        else AGRAD_DS(1, false);
+        const uint32_t waves = (uint32_t)(n * chunks);
+        const dim3 grid((waves + kDsBlock / kWave - 1) / (kDsBlock / kWave)), block(kDsBlock);
+#define AGRAD_DS(VEC, U, TAIL) hipLaunchKernelGGL((distill_bwd_kernel<T, VEC, U, TAIL>), grid, block, 0, s, x + r0 * a.ld, dx + r0 * a.ld, b, dloss ? dloss + r0 : nullptr, row_scale ? row_scale + r0 : nullptr, grad_scale, stats + 4 * r0, accumulate, FastDiv32(chunks), waves)
+        if (wide && two) { if (tail) AGRAD_DS(WIDE, 2, true); else AGRAD_DS(WIDE, 2, false); }
+        else if (wide) { if (tail) AGRAD_DS(WIDE, 1, true); else AGRAD_DS(WIDE, 1, false); }
+        else if (two) { if (tail) AGRAD_DS(1, 2, true); else AGRAD_DS(1, 2, false); }
+        else { if (tail) AGRAD_DS(1, 1, true); else AGRAD_DS(1, 1, false); }
 #undef AGRAD_DS
     }
     return check_hip(hipGetLastError(), "top-k distillation backward launch");
