@@ -32,6 +32,7 @@ constexpr int kDsBlock = 256;
 constexpr int kDsUnroll = 4;                       // vectors a thread keeps in flight
 constexpr uint32_t kMapWords = 5120;               // of the bit map: 163840 classes of a row, or of a part of one
 constexpr uint32_t kMapBits = kMapWords * 32;
+constexpr uint32_t kShortMap = 2048;               // words: 65536 classes
 static_assert(AGRAD_MAX_TOP <= kDsBlock && AGRAD_MAX_TOP == 2 * kWave, "a thread a teacher slot, the slots of two waves");
 
 struct DsArgs {
@@ -206,10 +207,13 @@ __device__ __forceinline__ RowStat ids_side(const DsArgs& a, const Teacher& t, i
 }
 
 // ---- forward: a workgroup a row, or a part of one ----------------------------------------------------------
-template <typename T, int VEC, bool TAIL>
+// WORDS: of the bit map, 0 in RENORM.  (A map for the longest part costs a CU its eighth workgroup, which 2048 rows of 50257 bf16
+// classes feel: 46 against 41 us.)
+template <typename T, int VEC, uint32_t WORDS>
 __global__ void __launch_bounds__(kDsBlock)
 distill_fwd_kernel(const T* __restrict__ x, const DsArgs a, const DsOut o) {
-    __shared__ __align__(16) uint32_t map[TAIL ? kMapWords : 4];
+    constexpr bool TAIL = WORDS != 0;
+    __shared__ __align__(16) uint32_t map[TAIL ? WORDS : 4];
     __shared__ Slots slots;
     __shared__ float lds[kDsBlock / kWave];
     __shared__ RowStat lds_stat[kDsBlock / kWave];
@@ -569,6 +573,7 @@ int ds_fwd_typed(hipStream_t s, const T* x, const DsArgs& a, DsOut o, uint64_t r
         if (o.parts > kMaxParts) return set_error(AGRAD_EINVAL, "top-k distillation with a tail: %u classes are too many", a.V);
         slab = kSharedParts / o.parts;
     }
+    const uint32_t longest = ((vectors + o.parts - 1) / o.parts) * (wide ? WIDE : 1);        // classes of a part's vectors, at most
     for (uint64_t r0 = 0; r0 < rows; r0 += slab) {
         const uint64_t n = rows - r0 < slab ? rows - r0 : slab;
         DsArgs b = a;
@@ -579,10 +584,11 @@ int ds_fwd_typed(hipStream_t s, const T* x, const DsArgs& a, DsOut o, uint64_t r
         if (p.stats) p.stats += 4 * r0;
         const dim3 grid((uint32_t)n * o.parts), block(kDsBlock);
         const T* from = x + r0 * a.ld;
-        if (wide && tail) hipLaunchKernelGGL((distill_fwd_kernel<T, WIDE, true>), grid, block, 0, s, from, b, p);
-        else if (wide) hipLaunchKernelGGL((distill_fwd_kernel<T, WIDE, false>), grid, block, 0, s, from, b, p);
-        else if (tail) hipLaunchKernelGGL((distill_fwd_kernel<T, 1, true>), grid, block, 0, s, from, b, p);
-        else hipLaunchKernelGGL((distill_fwd_kernel<T, 1, false>), grid, block, 0, s, from, b, p);
+        if (wide && tail && longest <= kShortMap * 32) hipLaunchKernelGGL((distill_fwd_kernel<T, WIDE, kShortMap>), grid, block, 0, s, from, b, p);
+        else if (wide && tail) hipLaunchKernelGGL((distill_fwd_kernel<T, WIDE, kMapWords>), grid, block, 0, s, from, b, p);
+        else if (wide) hipLaunchKernelGGL((distill_fwd_kernel<T, WIDE, 0>), grid, block, 0, s, from, b, p);
+        else if (tail) hipLaunchKernelGGL((distill_fwd_kernel<T, 1, kShortMap>), grid, block, 0, s, from, b, p);
+        else hipLaunchKernelGGL((distill_fwd_kernel<T, 1, 0>), grid, block, 0, s, from, b, p);
     }
     return check_hip(hipGetLastError(), "top-k distillation launch");
 }
@@ -627,13 +633,16 @@ bool ds_held_launch(hipStream_t s, const T* x, T* dx, const DsArgs& a, const DsO
     return false;
 }
 
-// Rows that no workgroup's registers hold (fp32 beyond 81920 classes, bf16 beyond 163840), rows of a few classes, and logits and
-// gradient at different places within 16 bytes: the forward pass, then the backward pass, over as many rows at a time as the
+// Rows that no workgroup's registers hold (fp32 beyond 81920 classes, bf16 beyond 163840), a few long rows, rows of a few classes,
+// and logits and gradient at different places within 16 bytes: the forward pass, then the backward pass, over as many rows at a time as the
 // context's memory holds sums for.
 template <typename T>
 int ds_fused_typed(hipStream_t s, const T* x, T* dx, const DsArgs& a, const DsOut& o, uint64_t rows, bool tail) {
     constexpr int WIDE = WideVec<T>::value;
-    if (a.V >= 4 * WIDE && one_alignment(x, dx)) {
+    // (a CU reads a long row in 20 us: some tens of them are faster shared out, one row of 151936 bf16 11.8 against 23 us, 64 rows 23
+    // against 27, 128 rows 32 against 28; shorter rows never are by more than a microsecond)
+    const bool few = rows <= 96 && a.V / WIDE > 20 * 512;
+    if (a.V >= 4 * WIDE && one_alignment(x, dx) && !few) {
         if (tail ? ds_held_launch<T, true>(s, x, dx, a, o, rows) : ds_held_launch<T, false>(s, x, dx, a, o, rows))
             return check_hip(hipGetLastError(), "top-k distillation step launch");
     }
