@@ -417,7 +417,7 @@ distill_bwd_kernel(const T* x, T* dx, const DsArgs a, const float* dloss, const 
 
 // ---- loss and gradient in one launch, the row in registers in between ------------------------------------------
 // A workgroup a row, which it holds in registers between the sums and the gradient: 20 vectors a thread leave two 512-thread
-// workgroups to a CU, longer rows take one of 1024 threads.  Sums are taken in the order of the loads, with the running
+// workgroups to a CU, longer rows of fp32 take one of 1024 threads.  Sums are taken in the order of the loads, with the running
 // maximum of each thread, while later vectors are on their way; what a row needs besides its vectors is asked for before
 // them (waits are in order: behind them it would wait for the whole row).  The classes among the ids are stored a second time, by
 // the thread that stored their vector: in order, without a wait for the stores.  x and dx may be the same memory.
@@ -429,10 +429,14 @@ struct HeldSlots {
     uint32_t next[AGRAD_MAX_TOP];           // a list a wave: the slots whose vectors its threads store
 };
 
+// With NV = 0 the row is read twice instead: the first pass reads with ordinary loads, which leave the rows that are being worked
+// on (one or two a CU, some 100 to 260 MB) in the memory-side cache, the second with loads that pass by it.  (Reading and writing
+// 2048 rows of 128256 fp32 like this takes a kernel without arithmetic 432 us, with both passes passing by the cache 583.)
 template <typename T, int VEC, int NV, int BLOCK, bool TAIL>
 __global__ void __launch_bounds__(BLOCK)
 distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
-    __shared__ __align__(16) uint32_t map[TAIL ? NV * BLOCK * VEC / 32 : 4];
+    constexpr int U = NV != 0 ? NV : kDsUnroll;                   // vectors a thread has in registers
+    __shared__ __align__(16) uint32_t map[!TAIL ? 4 : NV != 0 ? NV * BLOCK * VEC / 32 : kMapWords];
     __shared__ HeldSlots slots;
     __shared__ uint32_t heads[BLOCK / kWave];
     __shared__ float lds[BLOCK / kWave];
@@ -448,13 +452,18 @@ distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
     const float given = a.values[slot_at];
     float at[1], xe[1];
     VecIO<T, 1>::load(base + (tid < parts.extra ? parts.extra_at(tid) : 0u), xe);
-    typename Raw::type raw[NV];
+    typename Raw::type raw[U];
+    auto read = [&](uint32_t from) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const uint32_t vec = (uint32_t)i * BLOCK + tid;
-        raw[i] = Raw::load(base + parts.head + (uint64_t)(vec < parts.nvec ? vec : 0u) * VEC);
-    }
-    if (TAIL) clear_map<BLOCK>(map, (uint32_t)(NV * BLOCK * VEC));
+        for (int i = 0; i < U; ++i) {
+            const uint32_t vec = from + (uint32_t)i * BLOCK + tid;
+            const T* at_ = base + parts.head + (uint64_t)(vec < parts.nvec ? vec : 0u) * VEC;
+            if constexpr (NV != 0) raw[i] = Raw::load(at_);
+            else raw[i] = *reinterpret_cast<const typename Raw::type*>(at_);
+        }
+    };
+    read(0);
+    if (TAIL) clear_map<BLOCK>(map, NV != 0 ? (uint32_t)(NV * BLOCK * VEC) : parts.nvec * VEC);
     if (tid < BLOCK / kWave) heads[tid] = 0xffffffffu;
     const int32_t id = tid < a.top && asked >= 0 && (uint32_t)asked < a.V ? asked : -1;
     if (tid < a.top && id != asked && asked != -1) *a.err_flag = 1;
@@ -479,30 +488,34 @@ distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
 
     RowStat t = empty_stat();
     absorb_stat<false, 1>(t, xe, a.c);
-    // (the map covers all NV vectors of a thread; a step of BLOCK vectors is whole words)
+    // (with NV the map covers all vectors of a thread; a step of BLOCK vectors is whole words)
     static_assert(BLOCK * VEC % 32 == 0, "");
-    const uint32_t* words = map + (TAIL ? tid * VEC / 32 : 0u);
     const uint32_t shift_bits = tid * VEC % 32;
-    uint32_t bits = TAIL ? words[0] : 0u;
+    for (uint32_t from = 0; from < parts.nvec; from += U * BLOCK) {
+        if (NV == 0 && from != 0) read(from);
+        const uint32_t* words = map + (TAIL ? (from + tid) * VEC / 32 : 0u);
+        uint32_t bits = TAIL && from + tid < parts.nvec ? words[0] : 0u;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const uint32_t vec = (uint32_t)i * BLOCK + tid;
-        uint32_t ahead = 0;
-        if (TAIL && i + 1 < NV) {
-            ahead = words[(i + 1) * (BLOCK * VEC / 32)];
-            asm volatile("" ::: "memory");                         // (one vector's bits ahead, not all of them)
-        }
-        if (vec < parts.nvec) {
-            if (TAIL) {
-                bits = (bits >> shift_bits) & ((1u << VEC) - 1u);
-                if (bits != 0) mask_raw(raw[i], bits);
+        for (int i = 0; i < U; ++i) {
+            const uint32_t vec = from + (uint32_t)i * BLOCK + tid;
+            uint32_t ahead = 0;
+            if (TAIL && i + 1 < U && (NV != 0 || vec + BLOCK < parts.nvec)) {
+                ahead = words[(i + 1) * (BLOCK * VEC / 32)];
+                asm volatile("" ::: "memory");                     // (one vector's bits ahead, not all of them)
             }
-            float v[VEC];
-            Raw::unpack(raw[i], v);
-            absorb_stat<false, VEC>(t, v, a.c);
+            if (vec < parts.nvec) {
+                if (TAIL) {
+                    bits = (bits >> shift_bits) & ((1u << VEC) - 1u);
+                    if (bits != 0) mask_raw(raw[i], bits);
+                }
+                float v[VEC];
+                Raw::unpack(raw[i], v);
+                absorb_stat<false, VEC>(t, v, a.c);
+            }
+            if constexpr (NV != 0) unpack_again(raw[i]);
+            bits = ahead;
         }
-        unpack_again(raw[i]);
-        bits = ahead;
+        if constexpr (NV != 0) break;
     }
     t = block_stat<BLOCK, false>(t, a.c, lds_stat);
 
@@ -539,14 +552,27 @@ distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
     // longest rows their last registers)
     uint32_t again = tid;
     asm volatile("" : "+v"(again));
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const uint32_t vec = (uint32_t)i * BLOCK + again;
+    auto rewrite = [&](const typename Raw::type& r, uint32_t vec) {
         float v[VEC];
-        Raw::unpack(raw[i], v);
+        Raw::unpack(r, v);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) v[j] = __builtin_amdgcn_exp2f((v[j] - shift) * a.c) * k;
         if (vec < parts.nvec) store_grad<T, VEC>(out + parts.head + (uint64_t)vec * VEC, v);
+    };
+    if constexpr (NV != 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) rewrite(raw[i], (uint32_t)i * BLOCK + again);
+    } else {
+        for (uint32_t from = again; from < parts.nvec; from += 2 * BLOCK) {
+            typename Raw::type two[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t vec = from + (uint32_t)i * BLOCK;
+                two[i] = Raw::load(base + parts.head + (uint64_t)(vec < parts.nvec ? vec : from) * VEC);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) rewrite(two[i], from + (uint32_t)i * BLOCK);
+        }
     }
     for (uint32_t j = heads[tid / kWave]; j != 0xffffffffu; j = slots.next[j & 0xffffu]) {
         if (tid % kWave != j >> 16) continue;
@@ -625,17 +651,24 @@ bool ds_held_launch(hipStream_t s, const T* x, T* dx, const DsArgs& a, const DsO
     constexpr int WIDE = WideVec<T>::value;
     const uint32_t vectors = a.V / WIDE;
     const dim3 grid((uint32_t)rows);
+    // Held rows of two 512-thread workgroups a CU are faster than rows read twice (2048 x 50257 bf16 177 against 184 us, 4096 x 32768
+    // fp32 424 against 431).  Beyond them a CU holds 1024 threads at a time: fp32 still gains (512 x 70000 63 against 73 us, 4096 x
+    // 80000 516 against 570, though 4096 x 50257 378 against 365), bf16, with twice the arithmetic a byte and no second workgroup to
+    // fill its waits, loses (1024 x 110000 120 against 106 us, 8192 x 151936 1096 against 1071).
 #define AGRAD_DS(N, BLOCK) \
     if (vectors <= (uint32_t)(N) * BLOCK) { hipLaunchKernelGGL((distill_held_kernel<T, WIDE, N, BLOCK, TAIL>), grid, dim3(BLOCK), 0, s, x, dx, a, o); return true; }
     AGRAD_DS(1, 256) AGRAD_DS(4, 256) AGRAD_DS(4, 512) AGRAD_DS(8, 512) AGRAD_DS(12, 512) AGRAD_DS(16, 512) AGRAD_DS(20, 512)
-    AGRAD_DS(12, 1024) AGRAD_DS(16, 1024) AGRAD_DS(20, 1024)
+    if constexpr (sizeof(T) == 4) {
+        AGRAD_DS(12, 1024) AGRAD_DS(16, 1024) AGRAD_DS(20, 1024)
+    }
 #undef AGRAD_DS
-    return false;
+    if (TAIL && vectors + 1 > kMapBits / WIDE) return false;
+    hipLaunchKernelGGL((distill_held_kernel<T, WIDE, 0, 1024, TAIL>), grid, dim3(1024), 0, s, x, dx, a, o);
+    return true;
 }
 
-// Rows that no workgroup's registers hold (fp32 beyond 81920 classes, bf16 beyond 163840), a few long rows, rows of a few classes,
-// and logits and gradient at different places within 16 bytes: the forward pass, then the backward pass, over as many rows at a time as the
-// context's memory holds sums for.
+// A few long rows, rows with a tail whose ids' bit map is more than LDS, rows of a few classes, and logits and gradient at different
+// places within 16 bytes: the forward pass, then the backward pass, over as many rows at a time as the context's memory holds sums for.
 template <typename T>
 int ds_fused_typed(hipStream_t s, const T* x, T* dx, const DsArgs& a, const DsOut& o, uint64_t rows, bool tail) {
     constexpr int WIDE = WideVec<T>::value;
