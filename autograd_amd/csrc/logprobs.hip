@@ -494,6 +494,46 @@ __device__ __forceinline__ void lp_store(T* to, float (&d)[VEC], uint32_t accumu
     store_grad<T, VEC>(to, d);
 }
 
+// A row whose lse is so large that fp32 holds little of the logarithm beside the offset (all classes at a mask's lowest value:
+// nothing of it, p would be 1 each; with a scale above 1 the lse is -inf like that of a row without classes).  The row's
+// first workgroup takes all of it and sums it up again about its largest logit; it has read the row before it writes, so dx
+// may be x here too.
+constexpr float kLargeLse = 256.0f;          // (an error of 2^-17 in log p)
+template <typename T, int VEC>
+__device__ void lp_bwd_row(const T* base, T* out, const RowParts<T, VEC>& parts, LpRow r, uint32_t accumulate) {
+    __shared__ RowStat lds[kLpBlock / kWave];
+    const float c = r.scale * kLog2eHi;
+    RowStat t = empty_stat();
+    float e[1] = {-INFINITY};
+    if (threadIdx.x < parts.extra) VecIO<T, 1>::load(base + parts.extra_at(threadIdx.x), e);
+    absorb_stat<false, 1>(t, e, c);
+    for (uint32_t i = threadIdx.x; i < parts.nvec; i += kLpBlock) {
+        float v[VEC];
+        VecIO<T, VEC>::load(base + parts.head + (uint64_t)i * VEC, v);
+        absorb_stat<false, VEC>(t, v, c);
+    }
+    t = block_stat<kLpBlock, false>(t, c, lds);
+    r.lse = logf(t.s);
+    if (t.m == -INFINITY && t.s == 0.0f) {                 // no class: no gradient
+        t.m = 0.0f;
+        r.lse = INFINITY;
+        r.a = r.h = r.g = 0.0f;
+    }
+    if (threadIdx.x < parts.extra) {
+        const uint32_t at = parts.extra_at(threadIdx.x);
+        e[0] = lp_grad(e[0] - t.m, r, at);
+        lp_store<T, 1>(out + at, e, accumulate);
+    }
+    for (uint32_t i = threadIdx.x; i < parts.nvec; i += kLpBlock) {
+        const uint32_t first = parts.head + i * VEC;
+        float v[VEC];
+        VecIO<T, VEC>::load(base + first, v);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[k] = lp_grad(v[k] - t.m, r, first + k);
+        lp_store<T, VEC>(out + first, v, accumulate);
+    }
+}
+
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kLpBlock)
 logprobs_bwd_kernel(const T* x, T* dx, const LpBwdArgs a, const FastDiv32 chunks) {
@@ -506,13 +546,15 @@ logprobs_bwd_kernel(const T* x, T* dx, const LpBwdArgs a, const FastDiv32 chunks
     if (!asked && token != -1 && chunk == 0 && threadIdx.x == 0) *a.err_flag = 1;
     r.scale = a.scale;
     r.lse = a.lse[row];
-    const bool empty = r.lse == -INFINITY;
-    r.token = asked && !empty ? (uint32_t)token : 0xffffffffu;
+    r.token = asked ? (uint32_t)token : 0xffffffffu;
     r.g = asked && a.dlogp != nullptr ? a.scale * a.dlogp[row] : 0.0f;
     r.h = a.dentropy != nullptr ? a.scale * a.dentropy[row] : 0.0f;
     r.a = a.dentropy != nullptr ? __builtin_fmaf(r.h, a.entropy[row], r.g) : r.g;
-    if (empty) { r.lse = INFINITY; r.a = r.h = r.g = 0.0f; }
     const RowParts<T, VEC> parts(base, a.V);
+    if (fabsf(r.lse) > kLargeLse) {
+        if (chunk == 0) lp_bwd_row<T, VEC>(base, out, parts, r, a.accumulate);
+        return;
+    }
     if (chunk == 0 && threadIdx.x < parts.extra) {
         const uint32_t e = parts.extra_at(threadIdx.x);
         float v[1];

@@ -222,6 +222,49 @@ def test_backward_strides_offsets_accumulate_and_in_place(ctx, V, ld, offset, dx
         np.testing.assert_array_equal(same, got)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [70, 5003, 70000])
+def test_backward_of_rows_far_from_zero(ctx, V, dtype):
+    """rows of which fp32 holds no lse: all at a mask's lowest value, or shifted as a whole"""
+    rng = np.random.default_rng(V)
+    low = float(np.finfo(np.float32).min) if dtype == "f32" else -3.3895313892515355e38
+    x = np.tile(L.logits(rng, 1, V, dtype), (7, 1))
+    x[0, :] = low
+    x[1, V // 2:] = low
+    x[2] = L.rounded(x[2] + 60000.0, dtype)
+    x[3] = L.rounded(x[3] - 60000.0, dtype)
+    x[4, :] = -np.inf
+    x[5, :] = -np.inf
+    x[5, 3] = low
+    t = np.array([2, 3, int(x[2].argmax()), int(x[3].argmin()), 1, 3, -1], np.int32)
+    g, h = rng.standard_normal(7).astype(np.float32), rng.standard_normal(7).astype(np.float32)
+    bits = L.store(x, dtype)
+    for scale in (1.0, 1.5):
+        f = L.forward(ctx, bits, t, 0, scale)
+        p, logp, _ = cf._softmax_rows(cf.f64(x) * scale)
+        l = np.abs(np.where(p > 0, logp, 0.0))
+        want = cf.token_logprobs_grad(x, t, g, h, scale)
+        # distances to the largest logit, which is taken off exactly or with half a step, and their product with the scale
+        delta = U * (6 * l + 16) + 2 * L.sum_error(V)
+        size = p * (np.abs(g)[:, None] + np.abs(h)[:, None] * (l + (p * l).sum(-1, keepdims=True) + 1))
+        bound = scale * (size * 2 * delta + np.abs(h)[:, None] * p * L.sum_error(V) * (2 + 2 * np.log(V + 1)))
+        bound = bound + scale * 8 * U * np.abs(g)[:, None] * (np.arange(V) == t[:, None]) + 1e-37
+        for r in (1, 6):                                   # (ordinary ones, whose lse is rounded)
+            one = slice(r, r + 1)
+            bound[r] = backward_bound(cf.f64(x[one]), t[one], g[one], h[one], scale, "f32", want[one])[0]
+        bound = bound + (np.abs(want) + bound) * 2.0 ** -8 if dtype == "bf16" else bound
+        got = L.backward(ctx, bits, t, f["lse"], f["entropy"], g, h, scale)
+        L.assert_within(L.value(got), want, bound, f"scale {scale}")
+        assert not L.value(got)[4].any()
+        same = L.backward(ctx, bits, t, f["lse"], f["entropy"], g, h, scale, in_place=True)
+        np.testing.assert_array_equal(same, got)
+        base = L.rounded(rng.standard_normal((7, V)), dtype)
+        acc = L.value(L.backward(ctx, bits, t, f["lse"], f["entropy"], g, h, scale, flags=capi.ACC_INPUT_GRAD, init=L.store(base, dtype)))
+        half = 2.0 ** -8 if dtype == "bf16" else U
+        L.assert_within(acc, base + want, bound + 2 * half * (np.abs(base + want) + bound), f"accumulated, scale {scale}")
+        np.testing.assert_array_equal(acc[4], base[4])
+
+
 def test_backward_against_differences(ctx):
     """d(dlogp . logp + dentropy . entropy) along single logits, central differences of the float64 form"""
     rng = np.random.default_rng(5)
