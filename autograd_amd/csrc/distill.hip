@@ -28,6 +28,7 @@ namespace agrad {
 
 namespace {
 
+typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
 constexpr int kDsBlock = 256;
 constexpr int kDsUnroll = 4;                       // vectors a thread keeps in flight
 constexpr uint32_t kMapWords = 5120;               // of the bit map: 163840 classes of a row, or of a part of one
@@ -60,10 +61,14 @@ __device__ __forceinline__ void clear_map(uint32_t* map, uint32_t classes) {
     const uint32_t n = (classes + 127) / 128;
     for (uint32_t i = threadIdx.x; i < n; i += BLOCK) reinterpret_cast<u32x4*>(map)[i] = u32x4{0u, 0u, 0u, 0u};
 }
-// (first: the class of bit 0)
-__device__ __forceinline__ void mark(uint32_t* map, int32_t id, uint32_t first, uint32_t classes) {
+// (the bits of a stretch of the row's vectors, and a word for the elements outside the vectors)
+template <typename P>
+__device__ __forceinline__ void mark(uint32_t* map, uint32_t& outside, const P& parts, int32_t id, uint32_t first, uint32_t classes) {
+    if (id < 0) return;
     const uint32_t at = (uint32_t)id - first;
-    if (id >= 0 && at < classes) atomicOr(&map[at / 32], 1u << (at % 32));
+    if (at < classes) atomicOr(&map[at / 32], 1u << (at % 32));
+    else if ((uint32_t)id < parts.head) atomicOr(&outside, 1u << id);
+    else if ((uint32_t)id >= parts.tail_start) atomicOr(&outside, 1u << (parts.head + ((uint32_t)id - parts.tail_start)));
 }
 // the bits of the vec-th vector
 template <int VEC>
@@ -119,26 +124,57 @@ __device__ __forceinline__ Teacher teacher_row(const DsArgs& a, float u, int32_t
 
 // Slots in LDS.  A class that a row names twice counts with both its q; only its first slot stands for it.
 struct Slots {
-    int32_t id[AGRAD_MAX_TOP];
-    float q[AGRAD_MAX_TOP];
+    __align__(16) int32_t id[AGRAD_MAX_TOP];         // (unused slots, and those past the row's: -1)
+    __align__(16) float q[AGRAD_MAX_TOP];
 };
 struct Own {
     bool first;
     float taken;              // sum of the q of this slot's class, in slot order
 };
+// (every slot against all: four at a time and without a branch, so that the reads follow one another without a wait.  One slot at
+// a time, leaving early, took 4 us of a row's latency with 64 ids.)
+template <bool TAKEN>
 __device__ __forceinline__ Own own_slot(const Slots& s, uint32_t n, uint32_t k, int32_t id) {
-    Own o{id >= 0, 0.0f};
-    if (id < 0) return o;
-    for (uint32_t j = 0; j < n; j += 4) {            // (slots past n hold -1)
+    uint32_t at = 0xffffffffu;
+    float taken = 0.0f;
+    if (__ballot(id >= 0) != 0)
+#pragma unroll 4
+        for (uint32_t j = 0; j < n; j += 4) {
+            const i32x4 ids = *reinterpret_cast<const i32x4*>(s.id + j);
+            f32x4 q = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (TAKEN) q = *reinterpret_cast<const f32x4*>(s.q + j);
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            if (s.id[j + i] != id) continue;
-            o.taken = o.taken + s.q[j + i];
-            if (j + i < k) o.first = false;
+            for (int i = 0; i < 4; ++i) {
+                const bool same = ids[i] == id;
+                if constexpr (TAKEN) taken = taken + (same ? q[i] : 0.0f);
+                at = same && j + i < at ? j + i : at;
+            }
+        }
+    return Own{id >= 0 && at == k, taken};
+}
+
+// Who stores a class: a list of slots for each thread of a group, which stores them after its vectors.  The slots of one class are
+// in one thread's list; the order of a list, which atomics decide, does not matter.
+template <int THREADS>
+struct PatchLists {
+    uint32_t head[THREADS];
+    uint32_t next[AGRAD_MAX_TOP];
+    int32_t id[AGRAD_MAX_TOP];
+    float value[AGRAD_MAX_TOP];
+    static constexpr uint32_t kNone = 0xffffffffu;
+    __device__ __forceinline__ void add(uint32_t slot, uint32_t thread, int32_t cls, float v) {
+        id[slot] = cls;
+        value[slot] = v;
+        next[slot] = atomicExch(&head[thread], slot);
+    }
+    template <typename T>
+    __device__ __forceinline__ void store(T* out, uint32_t thread) const {
+        for (uint32_t j = head[thread]; j != kNone; j = next[j]) {
+            float d[1] = {value[j]};
+            VecIO<T, 1>::store(out + id[j], d);
         }
     }
-    return o;
-}
+};
 
 // ---- what a row's gradient is made of --------------------------------------------------------------------
 // all: log of the student's whole sum about m, the largest logit (m = -inf: no gradient); log_rest: log of p_rest (TAIL;
@@ -209,14 +245,15 @@ __device__ __forceinline__ RowStat ids_side(const DsArgs& a, const Teacher& t, i
 // ---- forward: a workgroup a row, or a part of one ----------------------------------------------------------
 // WORDS: of the bit map, 0 in RENORM.  (A map for the longest part costs a CU its eighth workgroup, which 2048 rows of 50257 bf16
 // classes feel: 46 against 41 us.)
-template <typename T, int VEC, uint32_t WORDS>
-__global__ void __launch_bounds__(kDsBlock)
+template <typename T, int VEC, uint32_t WORDS, int BLOCK>
+__global__ void __launch_bounds__(BLOCK)
 distill_fwd_kernel(const T* __restrict__ x, const DsArgs a, const DsOut o) {
     constexpr bool TAIL = WORDS != 0;
     __shared__ __align__(16) uint32_t map[TAIL ? WORDS : 4];
+    __shared__ uint32_t outside;
     __shared__ Slots slots;
-    __shared__ float lds[kDsBlock / kWave];
-    __shared__ RowStat lds_stat[kDsBlock / kWave];
+    __shared__ float lds[BLOCK / kWave];
+    __shared__ RowStat lds_stat[BLOCK / kWave];
     __shared__ uint32_t word;
     typedef RawVec<T, VEC> Raw;
     const uint32_t row = blockIdx.x / o.parts, nth = blockIdx.x - row * o.parts, k = threadIdx.x;
@@ -232,7 +269,7 @@ distill_fwd_kernel(const T* __restrict__ x, const DsArgs a, const DsOut o) {
     auto read = [&](uint32_t i0) {
 #pragma unroll
         for (int u = 0; u < kDsUnroll; ++u) {
-            const uint32_t i = i0 + u * kDsBlock;
+            const uint32_t i = i0 + u * BLOCK;
             raw[u] = Raw::load(body + (uint64_t)(i < part.hi ? i : part.lo) * VEC);
         }
     };
@@ -244,20 +281,19 @@ distill_fwd_kernel(const T* __restrict__ x, const DsArgs a, const DsOut o) {
     VecIO<T, 1>::load(base + (id >= 0 ? id : 0), at);
     if (k < AGRAD_MAX_TOP) slots.id[k] = id;
     const uint32_t classes = (part.hi - part.lo) * VEC;
-    if (TAIL) clear_map<kDsBlock>(map, classes);
+    if (TAIL) clear_map<BLOCK>(map, classes);
+    if (TAIL && k == 0) outside = 0u;
     const bool used = __syncthreads_or(id >= 0) != 0;
-    if (TAIL) mark(map, id, parts.head + part.lo * VEC, classes);
-    const Teacher teach = teacher_row<kDsBlock, TAIL>(a, id >= 0 ? given : -INFINITY, id, lds);
+    if (TAIL) mark(map, outside, parts, id, parts.head + part.lo * VEC, classes);
+    const Teacher teach = teacher_row<BLOCK, TAIL>(a, id >= 0 ? given : -INFINITY, id, lds);
     const float q = expf(teach.log_q);
-    bool first = id >= 0;
-    if (TAIL && first)
-        for (uint32_t j = 0; j < k; ++j) first = first && slots.id[j] != id;
+    const bool first = TAIL && k < AGRAD_MAX_TOP && own_slot<false>(slots, a.top, k, id).first;
     __syncthreads();
     RowStat t = empty_stat();
     while (i0 < part.hi) {
 #pragma unroll
         for (int u = 0; u < kDsUnroll; ++u) {
-            const uint32_t i = i0 + u * kDsBlock;
+            const uint32_t i = i0 + u * BLOCK;
             if (i >= part.hi) continue;
             if (TAIL) {
                 const uint32_t bits = bits_of<VEC>(map, i - part.lo);
@@ -267,20 +303,18 @@ distill_fwd_kernel(const T* __restrict__ x, const DsArgs a, const DsOut o) {
             Raw::unpack(raw[u], v);
             absorb_stat<false, VEC>(t, v, a.c);
         }
-        i0 += kDsBlock * kDsUnroll;
+        i0 += BLOCK * kDsUnroll;
         if (i0 < part.hi) read(i0);
     }
     if (nth == 0 && k < parts.extra) {
         const uint32_t e = parts.extra_at(k);
         float v[1];
         VecIO<T, 1>::load(base + e, v);
-        if (TAIL)
-            for (uint32_t j = 0; j < a.top; ++j)
-                if (slots.id[j] == (int32_t)e) v[0] = -INFINITY;
+        if (TAIL && (outside >> k & 1u)) v[0] = -INFINITY;
         absorb_stat<false, 1>(t, v, a.c);
     }
-    t = block_stat<kDsBlock, false>(t, a.c, lds_stat);
-    if (o.parts > 1) {
+    t = block_stat<BLOCK, false>(t, a.c, lds_stat);
+    if constexpr (BLOCK == kDsBlock) if (o.parts > 1) {
         if (k == 0) {
             float* to = o.shared.stats + 4 * (uint64_t)blockIdx.x;
             put_shared(to, t.m);
@@ -292,10 +326,10 @@ distill_fwd_kernel(const T* __restrict__ x, const DsArgs a, const DsOut o) {
             const float* from = o.shared.stats + 4 * ((uint64_t)row * o.parts + k);
             t = RowStat{get_shared(from), get_shared(from + 1), 0.0f};
         }
-        t = block_stat<kDsBlock, false>(t, a.c, lds_stat);
+        t = block_stat<BLOCK, false>(t, a.c, lds_stat);
     }
     float base_own, term, loss;
-    const RowStat own = ids_side<kDsBlock, TAIL>(a, teach, id, q, at[0], first, base_own, term, lds);
+    const RowStat own = ids_side<BLOCK, TAIL>(a, teach, id, q, at[0], first, base_own, term, lds);
     const RowSums s = finish_row<TAIL>(a, t, own, base_own, term, teach, used, loss);
     if (k == 0) {
         if (o.loss != nullptr) o.loss[row] = loss;
@@ -318,16 +352,29 @@ __device__ __forceinline__ void ds_store(T* to, float (&d)[VEC], uint32_t accumu
     store_grad<T, VEC>(to, d);
 }
 
-// A wave takes 64 * U neighbouring vectors of a row and needs no other: it looks through the row's ids for those of its classes,
-// writes its vectors as if there were none, and stores over them, by the lane that stored the vector (in order).  One
-// vector a lane is best where a wave's share of looking is small: 64 ids, 8192 rows of 151936 bf16 802 us (two: 818, four:
-// 872); with 128 ids of 32768 classes two are, 454 us (one: 503), and with 1000 fp32 classes, 108 us (118).  A workgroup that
-// collects the ids of its 16 KB in LDS took 908, 491 and 143 us.
-template <typename T, int VEC, int U, bool TAIL>
+// A wave takes 128 neighbouring vectors of a row, two a lane, and needs no other: it looks through the row's ids for those of its
+// classes, writes its vectors as if there were none, and stores over them, each by the lane that stored its vector (in
+// order).  Two vectors a lane halve the looking: 8192 rows of 32768 bf16 with 64 ids 195 us, of 8192 with 20 ids 50 us (one
+// vector: 210, 57; 8192 rows of 151936 with 64 ids are 861 and 839).  A workgroup that collected the ids of its 16 KB in LDS took
+// a fifth longer.
+constexpr int kBwdVectors = 2;
+template <int CLASSES>
+struct WaveSlots {
+    PatchLists<kWave> patches;
+    uint32_t seen[CLASSES / 32 + 1];
+};
+// LDS instructions of a wave are carried out in their order; this keeps the compiler to it too
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+template <typename T, int VEC, bool TAIL>
 __global__ void __launch_bounds__(kDsBlock)
 distill_bwd_kernel(const T* x, T* dx, const DsArgs a, const float* dloss, const float* row_scale, float grad_scale, const float* stats,
                    uint32_t accumulate, const FastDiv32 chunks, uint32_t waves) {
     typedef RawVec<T, VEC> Raw;
+    constexpr int U = kBwdVectors;
+    __shared__ WaveSlots<kWave * U * VEC> lists[kDsBlock / kWave];
     const uint32_t lane = threadIdx.x % kWave;
     const uint32_t wave = blockIdx.x * (kDsBlock / kWave) + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave));
     if (wave >= waves) return;
@@ -395,24 +442,44 @@ distill_bwd_kernel(const T* x, T* dx, const DsArgs a, const float* dloss, const 
         for (int j = 0; j < VEC; ++j) v[j] = none ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(v[j] - g.m, a.c, b)) * k;
         ds_store<T, VEC>(out + parts.head + (uint64_t)i * VEC, v, accumulate);
     }
-    auto of_lane = [](float v, int l) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), l)); };
-    auto put = [&](uint64_t these, int32_t id, uint32_t who, const float (&at)[1], const float (&old)[1], bool upper) {
-        for (; these != 0; these &= these - 1) {
-            const int l = (int)__builtin_ctzll(these);
-            const int32_t which = __builtin_amdgcn_readlane(id, l);
-            const uint64_t same0 = __ballot(id0 == which), same1 = __ballot(id1 == which);
-            // a class that the row names twice: its first slot stores it
-            if (upper ? same0 != 0 || __builtin_ctzll(same1) != l : __builtin_ctzll(same0) != l) continue;
-            float taken = 0.0f;
-            for (uint64_t w = same0; w != 0; w &= w - 1) taken = taken + of_lane(q0, (int)__builtin_ctzll(w));
-            for (uint64_t w = same1; w != 0; w &= w - 1) taken = taken + of_lane(q1, (int)__builtin_ctzll(w));
-            float d[1] = {own_grad(g, a, of_lane(at[0], l), taken, mul)};
-            if (accumulate) d[0] = of_lane(old[0], l) + d[0];
-            if (lane == (uint32_t)__builtin_amdgcn_readlane((int)who, l)) VecIO<T, 1>::store(out + which, d);
-        }
+    if ((mine0 | mine1) == 0) return;
+    // A class that the row names twice counts with both its q and is stored for its first slot: slots whose bit is there already
+    // have the wave look for such classes, which otherwise has nothing to compare.
+    auto& w = lists[threadIdx.x / kWave];
+    w.patches.head[lane] = w.patches.kNone;
+    if (lane < sizeof(w.seen) / 4) w.seen[lane] = 0u;
+    wave_lds_order();
+    auto seen = [&](bool has, int32_t id, uint32_t who) {
+        const uint32_t v = (uint32_t)id - parts.head - lo * VEC;                // (outside the vectors: the bits behind theirs)
+        const uint32_t bit = (uint32_t)id >= parts.head && (uint32_t)id < parts.tail_start ? v : span * VEC + who;
+        return has && (atomicOr(&w.seen[bit / 32], 1u << (bit % 32)) >> (bit % 32) & 1u) != 0;
     };
-    put(mine0, id0, who0, at0, old0, false);
-    put(mine1, id1, who1, at1, old1, true);
+    bool first0 = who0 != 0xffffffffu, first1 = who1 != 0xffffffffu;
+    float taken0 = q0, taken1 = q1;
+    const bool again0 = seen(first0, id0, who0), again1 = seen(first1, id1, who1);
+    if (__ballot(again0 || again1) != 0) {
+        auto of_lane = [](float v, int l) { return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), l)); };
+        auto gather = [&](uint64_t these, int32_t id, bool upper) {
+            for (; these != 0; these &= these - 1) {
+                const int l = (int)__builtin_ctzll(these);
+                const int32_t which = __builtin_amdgcn_readlane(id, l);
+                const uint64_t same0 = __ballot(id0 == which), same1 = __ballot(id1 == which);
+                float taken = 0.0f;
+                for (uint64_t m = same0; m != 0; m &= m - 1) taken = taken + of_lane(q0, (int)__builtin_ctzll(m));
+                for (uint64_t m = same1; m != 0; m &= m - 1) taken = taken + of_lane(q1, (int)__builtin_ctzll(m));
+                const bool first = upper ? same0 == 0 && (int)__builtin_ctzll(same1) == l : (int)__builtin_ctzll(same0) == l;
+                const bool me = lane == (uint32_t)l;
+                if (upper) { taken1 = me ? taken : taken1; first1 = me ? first : first1; }
+                else { taken0 = me ? taken : taken0; first0 = me ? first : first0; }
+            }
+        };
+        gather(mine0, id0, false);
+        gather(mine1, id1, true);
+    }
+    if (first0) w.patches.add(lane, who0, id0, own_grad(g, a, at0[0], taken0, mul) + old0[0]);
+    if (first1) w.patches.add(lane + kWave, who1, id1, own_grad(g, a, at1[0], taken1, mul) + old1[0]);
+    wave_lds_order();
+    w.patches.store(out, lane);
 }
 
 // ---- loss and gradient in one launch, the row in registers in between ------------------------------------------
@@ -423,12 +490,6 @@ distill_bwd_kernel(const T* x, T* dx, const DsArgs a, const float* dloss, const 
 // the thread that stored their vector: in order, without a wait for the stores.  x and dx may be the same memory.
 // (Workgroups that stay and ask for their next row's vectors as they store this one's were slower by 4 to 20 %, with no
 // register spilled: 424 against 400 us for 8192 rows of 32768 fp32.)
-struct HeldSlots {
-    Slots s;
-    float value[AGRAD_MAX_TOP];
-    uint32_t next[AGRAD_MAX_TOP];           // a list a wave: the slots whose vectors its threads store
-};
-
 // With NV = 0 the row is read twice instead: the first pass reads with ordinary loads, which leave the rows that are being worked
 // on (one or two a CU, some 100 to 260 MB) in the memory-side cache, the second with loads that pass by it.  (Reading and writing
 // 2048 rows of 128256 fp32 like this takes a kernel without arithmetic 432 us, with both passes passing by the cache 583.)
@@ -437,8 +498,9 @@ __global__ void __launch_bounds__(BLOCK)
 distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
     constexpr int U = NV != 0 ? NV : kDsUnroll;                   // vectors a thread has in registers
     __shared__ __align__(16) uint32_t map[!TAIL ? 4 : NV != 0 ? NV * BLOCK * VEC / 32 : kMapWords];
-    __shared__ HeldSlots slots;
-    __shared__ uint32_t heads[BLOCK / kWave];
+    __shared__ uint32_t outside;
+    __shared__ Slots slots;
+    __shared__ PatchLists<BLOCK> patches;
     __shared__ float lds[BLOCK / kWave];
     __shared__ RowStat lds_stat[BLOCK / kWave];
     typedef RawVec<T, VEC> Raw;
@@ -464,7 +526,8 @@ distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
     };
     read(0);
     if (TAIL) clear_map<BLOCK>(map, NV != 0 ? (uint32_t)(NV * BLOCK * VEC) : parts.nvec * VEC);
-    if (tid < BLOCK / kWave) heads[tid] = 0xffffffffu;
+    if (TAIL && tid == 0) outside = 0u;
+    patches.head[tid] = patches.kNone;
     const int32_t id = tid < a.top && asked >= 0 && (uint32_t)asked < a.V ? asked : -1;
     if (tid < a.top && id != asked && asked != -1) *a.err_flag = 1;
     const float u = id >= 0 ? given : -INFINITY;
@@ -472,18 +535,14 @@ distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
     const bool used = __syncthreads_or(id >= 0) != 0;
 
     // the teacher's side, and what the student says of the ids' classes
-    if (tid < AGRAD_MAX_TOP) slots.s.id[tid] = id;
-    if (TAIL) mark(map, id, parts.head, parts.nvec * VEC);
+    if (tid < AGRAD_MAX_TOP) slots.id[tid] = id;
+    if (TAIL) mark(map, outside, parts, id, parts.head, parts.nvec * VEC);
     const Teacher teach = teacher_row<BLOCK, TAIL>(a, u, id, lds);
     const float q = expf(teach.log_q);
-    if (tid < AGRAD_MAX_TOP) slots.s.q[tid] = q;
+    if (tid < AGRAD_MAX_TOP) slots.q[tid] = q;
     __syncthreads();
-    const Own own = own_slot(slots.s, a.top, tid, id);
-    if (TAIL && tid < parts.extra) {
-        const int32_t e = (int32_t)parts.extra_at(tid);
-        for (uint32_t j = 0; j < a.top; ++j)
-            if (slots.s.id[j] == e) xe[0] = -INFINITY;
-    }
+    const Own own = own_slot<true>(slots, a.top, tid, id);
+    if (TAIL && (outside >> (tid % 32) & 1u)) xe[0] = -INFINITY;       // (at most 15 of them; the others' are not looked at)
     if (tid >= parts.extra) xe[0] = -INFINITY;
 
     RowStat t = empty_stat();
@@ -532,12 +591,11 @@ distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
         for (uint32_t vec = tid; vec < parts.nvec; vec += BLOCK) VecIO<T, VEC>::store(out + parts.head + (uint64_t)vec * VEC, v);
         return;
     }
-    // hand the ids' gradients to the waves that store their vectors
+    // hand the ids' gradients to the threads that store their vectors
     if (own.first) {
         const uint32_t vec = (uint32_t)id >= parts.head ? ((uint32_t)id - parts.head) / VEC : 0xffffffffu;
         const uint32_t who = vec < parts.nvec ? vec % BLOCK : ((uint32_t)id < parts.head ? (uint32_t)id : parts.head + ((uint32_t)id - parts.tail_start));
-        slots.value[tid] = own_grad(g, a, at[0], own.taken, mul);
-        slots.next[tid] = atomicExch(&heads[who / kWave], tid | (who % kWave) << 16);
+        patches.add(tid, who, id, own_grad(g, a, at[0], own.taken, mul));
     }
     __syncthreads();
 
@@ -574,12 +632,7 @@ distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
             for (int i = 0; i < 2; ++i) rewrite(two[i], from + (uint32_t)i * BLOCK);
         }
     }
-    for (uint32_t j = heads[tid / kWave]; j != 0xffffffffu; j = slots.next[j & 0xffffu]) {
-        if (tid % kWave != j >> 16) continue;
-        const uint32_t slot = j & 0xffffu;
-        float d[1] = {slots.value[slot]};
-        VecIO<T, 1>::store(out + slots.s.id[slot], d);
-    }
+    patches.store(out, tid);
 }
 
 inline bool one_alignment(const void* x, const void* dx) {
@@ -608,13 +661,21 @@ int ds_fwd_typed(hipStream_t s, const T* x, const DsArgs& a, DsOut o, uint64_t r
         b.values += r0 * a.top;
         if (p.loss) p.loss += r0;
         if (p.stats) p.stats += 4 * r0;
-        const dim3 grid((uint32_t)n * o.parts), block(kDsBlock);
+        const dim3 grid((uint32_t)n * o.parts);
         const T* from = x + r0 * a.ld;
-        if (wide && tail && longest <= kShortMap * 32) hipLaunchKernelGGL((distill_fwd_kernel<T, WIDE, kShortMap>), grid, block, 0, s, from, b, p);
-        else if (wide && tail) hipLaunchKernelGGL((distill_fwd_kernel<T, WIDE, kMapWords>), grid, block, 0, s, from, b, p);
-        else if (wide) hipLaunchKernelGGL((distill_fwd_kernel<T, WIDE, 0>), grid, block, 0, s, from, b, p);
-        else if (tail) hipLaunchKernelGGL((distill_fwd_kernel<T, 1, kShortMap>), grid, block, 0, s, from, b, p);
-        else hipLaunchKernelGGL((distill_fwd_kernel<T, 1, 0>), grid, block, 0, s, from, b, p);
+#define AGRAD_DS(VEC, WORDS, BLOCK) hipLaunchKernelGGL((distill_fwd_kernel<T, VEC, WORDS, BLOCK>), grid, dim3(BLOCK), 0, s, from, b, p)
+        // (short rows as below: 32768 of 257 fp32 with 10 slots 19 us in 64 threads, 37 in 128, 71 in 256)
+        if (wide && o.parts == 1 && longest <= 128u * kDsUnroll * WIDE) {
+            if (a.top <= 64 && longest <= 64u * kDsUnroll * WIDE) {
+                if (tail) AGRAD_DS(WIDE, 64 * kDsUnroll * WIDE / 32, 64); else AGRAD_DS(WIDE, 0, 64);
+            }
+            else if (tail) AGRAD_DS(WIDE, 128 * kDsUnroll * WIDE / 32, 128); else AGRAD_DS(WIDE, 0, 128);
+        } else if (wide && tail && longest <= kShortMap * 32) AGRAD_DS(WIDE, kShortMap, kDsBlock);
+        else if (wide && tail) AGRAD_DS(WIDE, kMapWords, kDsBlock);
+        else if (wide) AGRAD_DS(WIDE, 0, kDsBlock);
+        else if (tail) AGRAD_DS(1, kShortMap, kDsBlock);
+        else AGRAD_DS(1, 0, kDsBlock);
+#undef AGRAD_DS
     }
     return check_hip(hipGetLastError(), "top-k distillation launch");
 }
@@ -624,8 +685,7 @@ int ds_bwd_typed(hipStream_t s, const T* x, T* dx, const DsArgs& a, const float*
                  const float* stats, uint32_t accumulate, uint64_t rows, bool tail) {
     constexpr int WIDE = WideVec<T>::value;
     const bool wide = a.V >= 4 * WIDE && one_alignment(x, dx);
-    const bool two = a.top > kWave || a.V / (wide ? WIDE : 1) <= 8 * kWave;
-    const uint32_t vec = wide ? WIDE : 1, span = kWave * (two ? 2 : 1);
+    const uint32_t vec = wide ? WIDE : 1, span = kWave * kBwdVectors;
     const uint32_t chunks = (a.V / vec + span - 1) / span;
     uint64_t max_rows = 0x03ffffffull / chunks;                  // waves of a launch: 2^32 threads
     if (max_rows == 0) max_rows = 1;
@@ -636,11 +696,10 @@ int ds_bwd_typed(hipStream_t s, const T* x, T* dx, const DsArgs& a, const float*
         b.values += r0 * a.top;
         const uint32_t waves = (uint32_t)(n * chunks);
         const dim3 grid((waves + kDsBlock / kWave - 1) / (kDsBlock / kWave)), block(kDsBlock);
-#define AGRAD_DS(VEC, U, TAIL) hipLaunchKernelGGL((distill_bwd_kernel<T, VEC, U, TAIL>), grid, block, 0, s, x + r0 * a.ld, dx + r0 * a.ld, b, dloss ? dloss + r0 : nullptr, row_scale ? row_scale + r0 : nullptr, grad_scale, stats + 4 * r0, accumulate, FastDiv32(chunks), waves)
-        if (wide && two) { if (tail) AGRAD_DS(WIDE, 2, true); else AGRAD_DS(WIDE, 2, false); }
-        else if (wide) { if (tail) AGRAD_DS(WIDE, 1, true); else AGRAD_DS(WIDE, 1, false); }
-        else if (two) { if (tail) AGRAD_DS(1, 2, true); else AGRAD_DS(1, 2, false); }
-        else { if (tail) AGRAD_DS(1, 1, true); else AGRAD_DS(1, 1, false); }
+#define AGRAD_DS(VEC, TAIL) hipLaunchKernelGGL((distill_bwd_kernel<T, VEC, TAIL>), grid, block, 0, s, x + r0 * a.ld, dx + r0 * a.ld, b, dloss ? dloss + r0 : nullptr, row_scale ? row_scale + r0 : nullptr, grad_scale, stats + 4 * r0, accumulate, FastDiv32(chunks), waves)
+        if (wide) { if (tail) AGRAD_DS(WIDE, true); else AGRAD_DS(WIDE, false); }
+        else if (tail) AGRAD_DS(1, true);
+        else AGRAD_DS(1, false);
 #undef AGRAD_DS
     }
     return check_hip(hipGetLastError(), "top-k distillation backward launch");
@@ -657,7 +716,11 @@ bool ds_held_launch(hipStream_t s, const T* x, T* dx, const DsArgs& a, const DsO
     // fill its waits, loses (1024 x 110000 120 against 106 us, 8192 x 151936 1096 against 1071).
 #define AGRAD_DS(N, BLOCK) \
     if (vectors <= (uint32_t)(N) * BLOCK) { hipLaunchKernelGGL((distill_held_kernel<T, WIDE, N, BLOCK, TAIL>), grid, dim3(BLOCK), 0, s, x, dx, a, o); return true; }
-    AGRAD_DS(1, 256) AGRAD_DS(4, 256) AGRAD_DS(4, 512) AGRAD_DS(8, 512) AGRAD_DS(12, 512) AGRAD_DS(16, 512) AGRAD_DS(20, 512)
+    // Short rows take the smallest workgroup that has four vectors a thread and a thread a slot, as the reductions of its waves are
+    // most of their time (32768 rows of 257 fp32: 10 slots 26 us in 64 threads, 46 in 128, 83 in 256; 100 slots 84 in 128, 137 in
+    // 256; 8192 rows of 4000 bf16, 10 slots: 28 in 128, 36 in 256).
+    if (a.top <= 64) { AGRAD_DS(2, 64) AGRAD_DS(4, 64) }
+    AGRAD_DS(2, 128) AGRAD_DS(4, 128) AGRAD_DS(4, 256) AGRAD_DS(4, 512) AGRAD_DS(8, 512) AGRAD_DS(12, 512) AGRAD_DS(16, 512) AGRAD_DS(20, 512)
     if constexpr (sizeof(T) == 4) {
         AGRAD_DS(12, 1024) AGRAD_DS(16, 1024) AGRAD_DS(20, 1024)
     }

@@ -20,10 +20,8 @@ namespace {
 constexpr int kLpBlock = 256;
 constexpr int kLpUnroll = 4;         // vectors a thread keeps in flight
 static_assert(AGRAD_MAX_TOP <= kLpBlock, "a thread an alternative");
-constexpr int kCandidates = 1024;    // candidates of a row's alternatives that LDS holds
 constexpr int kLine = 8;             // vectors of a line
 constexpr int kLines = 8192;         // lines that LDS holds
-constexpr int kListed = 512;         // lines with candidates
 struct Nothing {};
 constexpr int kMaxShared = 4096;     // keys that the parts of a row leave
 
@@ -52,16 +50,19 @@ __device__ __forceinline__ uint32_t key_index(uint64_t key) { return 0xffffffffu
 
 // What a workgroup finds.  A line is kLine neighbouring vectors (128 bytes); of each the row's one pass leaves the upper half
 // of its largest logit, which is done with before the first key is written.
+template <int BLOCK>
 struct Candidates {
+    static constexpr int kCandidates = 4 * BLOCK;    // of a row's alternatives
+    static constexpr int kListed = 2 * BLOCK;        // lines with candidates
     union {
         struct {
             uint64_t key[kCandidates];
             u32x4 raw[kListed];     // vectors that hold candidates (of threads that kept theirs)
         };
-        uint16_t line[kLines];
+        uint16_t line[BLOCK == kLpBlock ? kLines : 8];
     };
     uint32_t list[kListed];         // lines, or those vectors, that hold candidates
-    uint32_t shares[kLpBlock];
+    uint32_t shares[BLOCK];
     uint32_t count, listed, bound;
 };
 
@@ -90,16 +91,17 @@ __device__ __forceinline__ uint32_t take_places(uint32_t& count, uint32_t mine) 
     if (threadIdx.x % kWave == 0) at = atomicAdd(&count, total);
     return (uint32_t)__builtin_amdgcn_readfirstlane((int)at) + before;
 }
-__device__ __forceinline__ void append(Candidates& q, bool has, uint64_t key) {
+template <int BLOCK>
+__device__ __forceinline__ void append(Candidates<BLOCK>& q, bool has, uint64_t key) {
     const uint32_t at = take_place(q.count, has);
-    if (at < (uint32_t)kCandidates) q.key[at] = key;
+    if (at < (uint32_t)q.kCandidates) q.key[at] = key;
 }
 
 // Keeps the largest `top` of the candidates, in descending order at the front: a key's place is the number of larger
 // keys, counted (each key against all n: a tenth of the barriers of a sorting network, and faster up to some hundred
 // keys, which is what a row leaves).  All threads call it after a barrier; it ends with one.
 template <int BLOCK, int EACH>
-__device__ __forceinline__ void prune_each(Candidates& q, uint32_t n, uint32_t top) {
+__device__ __forceinline__ void prune_each(Candidates<BLOCK>& q, uint32_t n, uint32_t top) {
     uint64_t mine[EACH];
     uint32_t larger[EACH];
 #pragma unroll
@@ -124,10 +126,11 @@ __device__ __forceinline__ void prune_each(Candidates& q, uint32_t n, uint32_t t
     __syncthreads();
 }
 template <int BLOCK>
-__device__ __forceinline__ void prune(Candidates& q, uint32_t top) {
-    const uint32_t n = q.count < (uint32_t)kCandidates ? q.count : (uint32_t)kCandidates;
+__device__ __forceinline__ void prune(Candidates<BLOCK>& q, uint32_t top) {
+    const uint32_t n = q.count < (uint32_t)q.kCandidates ? q.count : (uint32_t)q.kCandidates;
     if (n <= (uint32_t)BLOCK) prune_each<BLOCK, 1>(q, n, top);
-    else prune_each<BLOCK, kCandidates / BLOCK>(q, n, top);
+    else if (n <= 2u * BLOCK) prune_each<BLOCK, 2>(q, n, top);
+    else prune_each<BLOCK, 4>(q, n, top);
 }
 
 // The upper half of a bound that at least `top` of the threads' values reach, as high as such a bound can be; 0 if fewer
@@ -135,7 +138,7 @@ __device__ __forceinline__ void prune(Candidates& q, uint32_t top) {
 // among the 256 halves up to the highest -- two octaves of the logit -- or, where that is not enough, bit by bit among
 // all; it ends with a barrier.
 template <int BLOCK>
-__device__ __forceinline__ uint32_t bound_of(Candidates& q, uint32_t mine, uint32_t highest, uint32_t top) {
+__device__ __forceinline__ uint32_t bound_of(Candidates<BLOCK>& q, uint32_t mine, uint32_t highest, uint32_t top) {
     constexpr int EACH = BLOCK / kWave;
     q.shares[threadIdx.x] = mine;
     if (threadIdx.x == 0) q.count = q.listed = 0;
@@ -178,7 +181,7 @@ __device__ __forceinline__ uint32_t ordered_half(uint32_t h) { return (h & 0x800
 
 // The largest of n keys, one a thread and step: right whatever they are, and slow.
 template <int BLOCK, typename KeyAt>
-__device__ __forceinline__ void top_by_steps(uint32_t n, uint32_t top, Candidates& q, KeyAt key_at) {
+__device__ __forceinline__ void top_by_steps(uint32_t n, uint32_t top, Candidates<BLOCK>& q, KeyAt key_at) {
     if (threadIdx.x == 0) q.count = 0;
     __syncthreads();
     uint64_t floor_key = 0;
@@ -187,7 +190,7 @@ __device__ __forceinline__ void top_by_steps(uint32_t n, uint32_t top, Candidate
         const uint64_t key = i < n ? key_at(i) : 0ull;
         append(q, key > floor_key, key);
         __syncthreads();
-        const bool full = q.count > (uint32_t)(kCandidates - BLOCK);
+        const bool full = q.count > (uint32_t)(q.kCandidates - BLOCK);
         __syncthreads();
         if (full) {
             prune<BLOCK>(q, top);
@@ -209,7 +212,7 @@ __device__ __forceinline__ void top_by_steps(uint32_t n, uint32_t top, Candidate
 template <typename T, int VEC, int BLOCK, bool HELD>
 __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& parts, const Stretch& part, uint32_t top, float best, float largest,
                                         const typename RawVec<T, VEC>::type (&held)[kLpUnroll], const float (&tops)[kLpUnroll],
-                                        Candidates& q) {
+                                        Candidates<BLOCK>& q) {
     typedef RawVec<T, VEC> Raw;
     const uint32_t extra = part.lo == 0 ? parts.extra : 0u, vectors = part.hi - part.lo;
     const uint32_t bound = bound_of<BLOCK>(q, (uint32_t)(class_key(best, 0u) >> 32), ordered(largest) >> 16, top);
@@ -227,7 +230,7 @@ __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& p
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
             if (!(v[k] >= least)) continue;
-            if (at < (uint32_t)kCandidates) q.key[at] = class_key(v[k], parts.head + number * VEC + k);
+            if (at < (uint32_t)q.kCandidates) q.key[at] = class_key(v[k], parts.head + number * VEC + k);
             ++at;
         }
     };
@@ -240,7 +243,7 @@ __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& p
 #pragma unroll
         for (int u = 0; u < kLpUnroll; ++u) {
             if (!(tops[u] >= least)) continue;
-            if (at < (uint32_t)kListed) {
+            if (at < (uint32_t)q.kListed) {
                 reinterpret_cast<typename Raw::type*>(q.raw)[at] = held[u];
                 q.list[at] = part.lo + u * BLOCK + threadIdx.x;
             }
@@ -248,7 +251,7 @@ __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& p
         }
         __syncthreads();
         const uint32_t n = q.listed;
-        fits = n <= (uint32_t)kListed;
+        fits = n <= (uint32_t)q.kListed;
         const uint32_t classes = fits ? n * VEC : 0u;
         for (uint32_t i = threadIdx.x; i / kWave * kWave < classes; i += BLOCK) {
             float v[1];
@@ -270,11 +273,11 @@ __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& p
             }
             uint32_t at = take_places(q.listed, (uint32_t)__popc(reach));
             for (; reach != 0; reach &= reach - 1u, ++at)
-                if (at < (uint32_t)kListed) q.list[at] = j + (uint32_t)__builtin_ctz(reach);
+                if (at < (uint32_t)q.kListed) q.list[at] = j + (uint32_t)__builtin_ctz(reach);
         }
         __syncthreads();
         const uint32_t n = q.listed;
-        fits = n <= (uint32_t)kListed && lines == all_lines;
+        fits = n <= (uint32_t)q.kListed && lines == all_lines;
         const uint32_t again = fits ? n * kLine : 0u;
         constexpr int U = 2;
         for (uint32_t i0 = threadIdx.x; i0 / kWave * kWave < again; i0 += BLOCK * U) {
@@ -297,7 +300,7 @@ __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& p
         append(q, x[0] >= least, class_key(x[0], e));
     }
     __syncthreads();
-    if (!fits || q.count > (uint32_t)kCandidates) {
+    if (!fits || q.count > (uint32_t)q.kCandidates) {
         __syncthreads();
         const uint32_t in_vectors = vectors * VEC;
         top_by_steps<BLOCK>(in_vectors + extra, top, q, [&](uint32_t i) {
@@ -326,7 +329,7 @@ struct KeyList {
     }
 };
 template <int BLOCK>
-__device__ __forceinline__ void join_tops(const KeyList& mine, const unsigned long long* keys, uint32_t n, uint32_t top, float largest, Candidates& q) {
+__device__ __forceinline__ void join_tops(const KeyList& mine, const unsigned long long* keys, uint32_t n, uint32_t top, float largest, Candidates<BLOCK>& q) {
     constexpr int EACH = kMaxShared / BLOCK;
     uint32_t best = 0;
 #pragma unroll
@@ -336,7 +339,7 @@ __device__ __forceinline__ void join_tops(const KeyList& mine, const unsigned lo
     for (int i = 0; i < EACH; ++i)
         if (i * (uint32_t)BLOCK < n) append(q, mine.key[i] != 0ull && (uint32_t)(mine.key[i] >> 48) >= bound, mine.key[i]);
     __syncthreads();
-    if (q.count > (uint32_t)kCandidates) {
+    if (q.count > (uint32_t)q.kCandidates) {
         __syncthreads();
         top_by_steps<BLOCK>(n, top, q, [&](uint32_t i) { return (uint64_t)get_shared(keys + i); });
     } else {
@@ -348,11 +351,11 @@ __device__ __forceinline__ void join_tops(const KeyList& mine, const unsigned lo
 // A workgroup reads a row, or a part of it, once, kLpUnroll vectors a thread in flight.  With HELD the part is no longer than
 // those, and they stay in registers for the alternatives; with LINES the pass leaves every line's largest logit for them.
 enum LpMode { PLAIN, LINES, HELD };
-template <typename T, int VEC, bool ENT, LpMode MODE>
-__global__ void __launch_bounds__(kLpBlock)
+template <typename T, int VEC, bool ENT, LpMode MODE, int BLOCK>
+__global__ void __launch_bounds__(BLOCK)
 logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
-    __shared__ RowStat lds[kLpBlock / kWave];
-    __shared__ std::conditional_t<MODE == PLAIN, Nothing, Candidates> found;
+    __shared__ RowStat lds[BLOCK / kWave];
+    __shared__ std::conditional_t<MODE == PLAIN, Nothing, Candidates<BLOCK>> found;
     __shared__ uint32_t word;
     typedef RawVec<T, VEC> Raw;
     const uint32_t row = blockIdx.x / a.parts, nth = blockIdx.x - row * a.parts;
@@ -366,7 +369,7 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
     auto read = [&](uint32_t i0) {
 #pragma unroll
         for (int u = 0; u < kLpUnroll; ++u) {
-            const uint32_t i = i0 + u * kLpBlock;
+            const uint32_t i = i0 + u * BLOCK;
             raw[u] = Raw::load(body + (uint64_t)(i < part.hi ? i : part.lo) * VEC);
         }
     };
@@ -374,7 +377,7 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
 #pragma unroll
         for (int u = 0; u < kLpUnroll; ++u) {
             tops[u] = -INFINITY;
-            if (i0 + u * kLpBlock < part.hi) {
+            if (i0 + u * BLOCK < part.hi) {
                 float v[VEC];
                 Raw::unpack(raw[u], v);
                 tops[u] = absorb_stat<ENT, VEC>(t, v, a.c);
@@ -396,7 +399,7 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
         absorb(part.lo + threadIdx.x);
     } else {
         const uint32_t lane = threadIdx.x % kWave;
-        for (uint32_t i0 = part.lo + (threadIdx.x - lane); i0 < part.hi; i0 += kLpBlock * kLpUnroll) {     // (whole waves)
+        for (uint32_t i0 = part.lo + (threadIdx.x - lane); i0 < part.hi; i0 += BLOCK * kLpUnroll) {     // (whole waves)
             read(i0 + lane);
             absorb(i0 + lane);
             if constexpr (MODE == LINES) {
@@ -406,17 +409,17 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
                     float m = fmaxf(tops[u], dpp_move<kDppQuadXor1>(tops[u]));
                     m = fmaxf(m, dpp_move<kDppQuadXor2>(m));
                     m = fmaxf(m, dpp_move<kDppRowHalfMirror>(m));
-                    const uint32_t line = (i0 - part.lo + u * kLpBlock + lane) / kLine;
+                    const uint32_t line = (i0 - part.lo + u * BLOCK + lane) / kLine;
                     if (lane % kLine == 0 && line < (uint32_t)kLines) found.line[line] = (uint16_t)(__float_as_uint(m) >> 16);
                 }
             }
         }
     }
     const float best = t.m;
-    t = block_stat<kLpBlock, ENT>(t, a.c, lds);
+    t = block_stat<BLOCK, ENT>(t, a.c, lds);
     if constexpr (MODE != PLAIN)
-        if (a.top != 0) row_top<T, VEC, kLpBlock, MODE == HELD>(base, parts, part, a.top, best, t.m, raw, tops, found);
-    if (a.parts > 1) {
+        if (a.top != 0) row_top<T, VEC, BLOCK, MODE == HELD>(base, parts, part, a.top, best, t.m, raw, tops, found);
+    if constexpr (BLOCK == kLpBlock) if (a.parts > 1) {
         if (threadIdx.x == 0) {
             float* to = a.shared.stats + 4 * (uint64_t)blockIdx.x;
             put_shared(to, t.m);
@@ -435,10 +438,10 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
         }
         if constexpr (MODE != PLAIN) {
             const KeyList mine(keys, a.parts * a.top);                // (asked for before the statistics are put together)
-            t = block_stat<kLpBlock, ENT>(t, a.c, lds);
-            if (a.top != 0) join_tops<kLpBlock>(mine, keys, a.parts * a.top, a.top, t.m, found);
+            t = block_stat<BLOCK, ENT>(t, a.c, lds);
+            if (a.top != 0) join_tops<BLOCK>(mine, keys, a.parts * a.top, a.top, t.m, found);
         } else {
-            t = block_stat<kLpBlock, ENT>(t, a.c, lds);
+            t = block_stat<BLOCK, ENT>(t, a.c, lds);
         }
     }
     const bool empty = t.m == -INFINITY && t.s == 0.0f;
@@ -499,20 +502,20 @@ __device__ __forceinline__ void lp_store(T* to, float (&d)[VEC], uint32_t accumu
 // first workgroup takes all of it and sums it up again about its largest logit; it has read the row before it writes, so dx
 // may be x here too.
 constexpr float kLargeLse = 256.0f;          // (an error of 2^-17 in log p)
-template <typename T, int VEC>
+template <typename T, int VEC, int BLOCK>
 __device__ void lp_bwd_row(const T* base, T* out, const RowParts<T, VEC>& parts, LpRow r, uint32_t accumulate) {
-    __shared__ RowStat lds[kLpBlock / kWave];
+    __shared__ RowStat lds[BLOCK / kWave];
     const float c = r.scale * kLog2eHi;
     RowStat t = empty_stat();
     float e[1] = {-INFINITY};
     if (threadIdx.x < parts.extra) VecIO<T, 1>::load(base + parts.extra_at(threadIdx.x), e);
     absorb_stat<false, 1>(t, e, c);
-    for (uint32_t i = threadIdx.x; i < parts.nvec; i += kLpBlock) {
+    for (uint32_t i = threadIdx.x; i < parts.nvec; i += BLOCK) {
         float v[VEC];
         VecIO<T, VEC>::load(base + parts.head + (uint64_t)i * VEC, v);
         absorb_stat<false, VEC>(t, v, c);
     }
-    t = block_stat<kLpBlock, false>(t, c, lds);
+    t = block_stat<BLOCK, false>(t, c, lds);
     r.lse = logf(t.s);
     if (t.m == -INFINITY && t.s == 0.0f) {                 // no class: no gradient
         t.m = 0.0f;
@@ -524,7 +527,7 @@ __device__ void lp_bwd_row(const T* base, T* out, const RowParts<T, VEC>& parts,
         e[0] = lp_grad(e[0] - t.m, r, at);
         lp_store<T, 1>(out + at, e, accumulate);
     }
-    for (uint32_t i = threadIdx.x; i < parts.nvec; i += kLpBlock) {
+    for (uint32_t i = threadIdx.x; i < parts.nvec; i += BLOCK) {
         const uint32_t first = parts.head + i * VEC;
         float v[VEC];
         VecIO<T, VEC>::load(base + first, v);
@@ -534,8 +537,8 @@ __device__ void lp_bwd_row(const T* base, T* out, const RowParts<T, VEC>& parts,
     }
 }
 
-template <typename T, int VEC>
-__global__ void __launch_bounds__(kLpBlock)
+template <typename T, int VEC, int BLOCK>
+__global__ void __launch_bounds__(BLOCK)
 logprobs_bwd_kernel(const T* x, T* dx, const LpBwdArgs a, const FastDiv32 chunks) {
     const uint32_t row = chunks.div(blockIdx.x), chunk = blockIdx.x - row * chunks.d;
     const T* base = x + (uint64_t)row * a.ld;
@@ -552,7 +555,7 @@ logprobs_bwd_kernel(const T* x, T* dx, const LpBwdArgs a, const FastDiv32 chunks
     r.a = a.dentropy != nullptr ? __builtin_fmaf(r.h, a.entropy[row], r.g) : r.g;
     const RowParts<T, VEC> parts(base, a.V);
     if (fabsf(r.lse) > kLargeLse) {
-        if (chunk == 0) lp_bwd_row<T, VEC>(base, out, parts, r, a.accumulate);
+        if (chunk == 0) lp_bwd_row<T, VEC, BLOCK>(base, out, parts, r, a.accumulate);
         return;
     }
     if (chunk == 0 && threadIdx.x < parts.extra) {
@@ -562,7 +565,7 @@ logprobs_bwd_kernel(const T* x, T* dx, const LpBwdArgs a, const FastDiv32 chunks
         v[0] = lp_grad(v[0], r, e);
         lp_store<T, 1>(out + e, v, a.accumulate);
     }
-    const uint32_t i = chunk * kLpBlock + threadIdx.x;
+    const uint32_t i = chunk * BLOCK + threadIdx.x;
     if (i >= parts.nvec) return;
     const uint32_t first = parts.head + i * VEC;
     float v[VEC];
@@ -572,21 +575,37 @@ logprobs_bwd_kernel(const T* x, T* dx, const LpBwdArgs a, const FastDiv32 chunks
     lp_store<T, VEC>(out + first, v, a.accumulate);
 }
 
-template <typename T, int VEC, LpMode MODE>
+template <typename T, int VEC, LpMode MODE, int BLOCK = kLpBlock>
 void lp_fwd_launch(hipStream_t s, const T* x, const LpArgs& a, uint64_t rows) {
-    const dim3 grid((uint32_t)rows * a.parts), block(kLpBlock);
-    if (a.entropy) hipLaunchKernelGGL((logprobs_fwd_kernel<T, VEC, true, MODE>), grid, block, 0, s, x, a);
-    else hipLaunchKernelGGL((logprobs_fwd_kernel<T, VEC, false, MODE>), grid, block, 0, s, x, a);
+    const dim3 grid((uint32_t)rows * a.parts), block(BLOCK);
+    if (a.entropy) hipLaunchKernelGGL((logprobs_fwd_kernel<T, VEC, true, MODE, BLOCK>), grid, block, 0, s, x, a);
+    else hipLaunchKernelGGL((logprobs_fwd_kernel<T, VEC, false, MODE, BLOCK>), grid, block, 0, s, x, a);
+}
+
+// Rows of up to kLpUnroll vectors a thread, in the smallest workgroup that holds one: with many rows the reductions of its waves
+// are most of the time (32768 rows of 257 fp32 in 64 threads and in 256: 15 and 40 us without alternatives, 26 and 87 with 5).
+// The alternatives need four threads each, for a useful bound.
+template <typename T, int VEC>
+int lp_fwd_short(hipStream_t s, const T* x, const LpArgs& a, uint64_t rows) {
+    const uint32_t vectors = a.V / VEC;
+    auto fits = [&](uint32_t block) { return vectors <= block * kLpUnroll && 4 * a.top <= block; };
+    if (a.top == 0 && fits(64)) lp_fwd_launch<T, VEC, PLAIN, 64>(s, x, a, rows);
+    else if (a.top == 0 && fits(128)) lp_fwd_launch<T, VEC, PLAIN, 128>(s, x, a, rows);
+    else if (fits(64)) lp_fwd_launch<T, VEC, HELD, 64>(s, x, a, rows);
+    else if (fits(128)) lp_fwd_launch<T, VEC, HELD, 128>(s, x, a, rows);
+    else lp_fwd_launch<T, VEC, HELD>(s, x, a, rows);
+    return check_hip(hipGetLastError(), "token log probabilities launch");
 }
 
 template <typename T>
 int lp_fwd_typed(hipStream_t s, const T* x, LpArgs a, uint64_t rows) {
     constexpr int WIDE = WideVec<T>::value;
-    if (a.V < 4 * WIDE) {
-        lp_fwd_launch<T, 1, HELD>(s, x, a, rows);
-        return check_hip(hipGetLastError(), "token log probabilities launch");
-    }
     const uint32_t vectors = a.V / WIDE;
+    // Short rows with many alternatives go by single elements: of fewer vectors than twice the alternatives the threads' largest
+    // logits give no useful bound (1000 bf16 classes, 128 alternatives: 28.6 us, all of them candidates; by elements 6.9).
+    const bool many = a.V <= (uint32_t)kLpBlock * kLpUnroll && vectors < 2 * a.top;
+    if (a.V < 4 * WIDE || many) return lp_fwd_short<T, 1>(s, x, a, rows);
+    if (vectors <= (uint32_t)kLpBlock / 2 * kLpUnroll) return lp_fwd_short<T, WIDE>(s, x, a, rows);
     a.parts = row_parts(rows, vectors);
     uint64_t slab = rows;
     if (a.top != 0) {
@@ -621,7 +640,10 @@ int lp_bwd_typed(hipStream_t s, const T* x, T* dx, LpBwdArgs a, uint64_t rows) {
     // rows are realigned by their first elements, which needs both tensors at one offset within 16 bytes
     const bool wide = a.V >= 4 * WIDE && ((reinterpret_cast<uintptr_t>(x) ^ reinterpret_cast<uintptr_t>(dx)) & 15u) == 0;
     const uint32_t vec = wide ? WIDE : 1;
-    const uint32_t chunks = (a.V / vec + kLpBlock - 1) / kLpBlock;
+    // (short rows leave most of a larger workgroup's threads idle: 32768 rows of 257 fp32 16.4 against 24.8 us, of 2048 bf16 42.5
+    // against 45.0; longer rows are the same in both)
+    const uint32_t block = a.V / vec <= 256u ? 64u : kLpBlock;
+    const uint32_t chunks = (a.V / vec + block - 1) / block;
     uint64_t max_rows = 0x00ffffffull / chunks;                  // workgroups of a launch: 2^32 threads
     if (max_rows == 0) max_rows = 1;
     for (uint64_t r0 = 0; r0 < rows; r0 += max_rows) {
@@ -632,9 +654,13 @@ int lp_bwd_typed(hipStream_t s, const T* x, T* dx, LpBwdArgs a, uint64_t rows) {
         if (b.entropy) b.entropy += r0;
         if (b.dlogp) b.dlogp += r0;
         if (b.dentropy) b.dentropy += r0;
-        const dim3 grid((uint32_t)(n * chunks)), block(kLpBlock);
-        if (wide) hipLaunchKernelGGL((logprobs_bwd_kernel<T, WIDE>), grid, block, 0, s, x + r0 * a.ld, dx + r0 * a.ld, b, FastDiv32(chunks));
-        else hipLaunchKernelGGL((logprobs_bwd_kernel<T, 1>), grid, block, 0, s, x + r0 * a.ld, dx + r0 * a.ld, b, FastDiv32(chunks));
+        const dim3 grid((uint32_t)(n * chunks));
+#define AGRAD_LP(VEC, BLOCK) hipLaunchKernelGGL((logprobs_bwd_kernel<T, VEC, BLOCK>), grid, dim3(BLOCK), 0, s, x + r0 * a.ld, dx + r0 * a.ld, b, FastDiv32(chunks))
+        if (wide && block == 64) AGRAD_LP(WIDE, 64);
+        else if (wide) AGRAD_LP(WIDE, kLpBlock);
+        else if (block == 64) AGRAD_LP(1, 64);
+        else AGRAD_LP(1, kLpBlock);
+#undef AGRAD_LP
     }
     return check_hip(hipGetLastError(), "token log probabilities backward launch");
 }
@@ -651,13 +677,16 @@ SharedRows shared_rows(void* scratch) {
 }
 
 // Parts of a row: as many as make 512 workgroups of all rows, or 1024 where the parts stay longer than 4096 vectors, but
-// none shorter than 512, two vectors a thread (a part costs its workgroup's reductions, and the parts are put together one
-// after the other).  48 rows of 18992 vectors, with 8 alternatives: 10 parts each 17.2 us, 21 parts 18.4, 5 parts 18.6, 2
-// parts 27.4; 256 rows of 16032: 4 parts 24.8, 2 parts 26.9, 1 part 31.9; one row: parts of 518 11.8, of 1069 13.2.
+// none shorter than 1024, four vectors a thread, which stay in its registers for the alternatives (a part costs its
+// workgroup's reductions, and the parts are put together one after the other).  Up to 2048 vectors one workgroup is as fast:
+// what one leaves for another takes 2 us to arrive (one row of 8192 fp32 with 20 alternatives 7.8 us, in two parts 9.4, in
+// eight 9.2; of 16384 10.0, in four parts 9.5; of 65536 26, in eight 12.1, in sixteen 9.8).  48 rows of 18992 vectors, with
+// 8 alternatives: 10 parts each 16.2 us, 7 parts 17.0, 21 parts 16.5; 37 rows of 12564: 13 parts 12.5, 7 parts 13.3, 19 parts 14.3.
 uint32_t row_parts(uint64_t rows, uint32_t vectors) {
+    if (vectors <= 2048u) return 1u;
     uint64_t parts = 512 / rows;
     if (parts == 0 || vectors / parts > 4096) parts = kSharedParts / rows;
-    if (parts > vectors / 512u) parts = vectors / 512u;
+    if (parts > (vectors + 1023u) / 1024u) parts = (vectors + 1023u) / 1024u;
     if (parts > kMaxParts) parts = kMaxParts;
     return parts < 1 ? 1u : (uint32_t)parts;
 }
