@@ -131,14 +131,15 @@ struct Own {
     bool first;
     float taken;              // sum of the q of this slot's class, in slot order
 };
-// (every slot against all: four at a time and without a branch, so that the reads follow one another without a wait.  One slot at
-// a time, leaving early, took 4 us of a row's latency with 64 ids.)
+// (every slot against all: eight at a time and without a branch, so that the reads follow one another without a wait.  One slot at
+// a time, leaving early, took 4 us of a row's latency with 64 ids; sixteen at a time take a workgroup of 1024 threads more than
+// 64 registers, and a CU its second one.)
 template <bool TAKEN>
 __device__ __forceinline__ Own own_slot(const Slots& s, uint32_t n, uint32_t k, int32_t id) {
     uint32_t at = 0xffffffffu;
     float taken = 0.0f;
     if (__ballot(id >= 0) != 0)
-#pragma unroll 4
+#pragma unroll 2
         for (uint32_t j = 0; j < n; j += 4) {
             const i32x4 ids = *reinterpret_cast<const i32x4*>(s.id + j);
             f32x4 q = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -494,7 +495,7 @@ distill_bwd_kernel(const T* x, T* dx, const DsArgs a, const float* dloss, const 
 // on (one or two a CU, some 100 to 260 MB) in the memory-side cache, the second with loads that pass by it.  (Reading and writing
 // 2048 rows of 128256 fp32 like this takes a kernel without arithmetic 432 us, with both passes passing by the cache 583.)
 template <typename T, int VEC, int NV, int BLOCK, bool TAIL>
-__global__ void __launch_bounds__(BLOCK)
+__global__ void __launch_bounds__(BLOCK, NV == 0 ? 8 : 1)
 distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
     constexpr int U = NV != 0 ? NV : kDsUnroll;                   // vectors a thread has in registers
     __shared__ __align__(16) uint32_t map[!TAIL ? 4 : NV != 0 ? NV * BLOCK * VEC / 32 : kMapWords];

@@ -19,6 +19,7 @@ namespace {
 
 constexpr int kLpBlock = 256;
 constexpr int kLpUnroll = 4;         // vectors a thread keeps in flight
+constexpr uint32_t kMostHeld = 16;   // and of a row that it keeps for its alternatives
 static_assert(AGRAD_MAX_TOP <= kLpBlock, "a thread an alternative");
 constexpr int kLine = 8;             // vectors of a line
 constexpr int kLines = 8192;         // lines that LDS holds
@@ -209,9 +210,9 @@ __device__ __forceinline__ void top_by_steps(uint32_t n, uint32_t top, Candidate
 // logits).  (Reading the shares again instead of lines reads the whole row: eight threads have a part in each 128 bytes.
 // 8192 rows of 128256 bf16, top 64: 595 us.)  A row whose largest logits are equal in great number, or crowd into few
 // shares, can leave more than LDS holds and goes the slow way.
-template <typename T, int VEC, int BLOCK, bool HELD>
+template <typename T, int VEC, int BLOCK, bool HELD, int U>
 __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& parts, const Stretch& part, uint32_t top, float best, float largest,
-                                        const typename RawVec<T, VEC>::type (&held)[kLpUnroll], const float (&tops)[kLpUnroll],
+                                        const typename RawVec<T, VEC>::type (&held)[U], const float (&tops)[U],
                                         Candidates<BLOCK>& q) {
     typedef RawVec<T, VEC> Raw;
     const uint32_t extra = part.lo == 0 ? parts.extra : 0u, vectors = part.hi - part.lo;
@@ -238,10 +239,10 @@ __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& p
         // first whole vectors, then classes, an element a thread: a place for each class of four vectors costs more
         uint32_t reach = 0;
 #pragma unroll
-        for (int u = 0; u < kLpUnroll; ++u) reach += tops[u] >= least ? 1u : 0u;
+        for (int u = 0; u < U; ++u) reach += tops[u] >= least ? 1u : 0u;
         uint32_t at = take_places(q.listed, reach);
 #pragma unroll
-        for (int u = 0; u < kLpUnroll; ++u) {
+        for (int u = 0; u < U; ++u) {
             if (!(tops[u] >= least)) continue;
             if (at < (uint32_t)q.kListed) {
                 reinterpret_cast<typename Raw::type*>(q.raw)[at] = held[u];
@@ -279,18 +280,18 @@ __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& p
         const uint32_t n = q.listed;
         fits = n <= (uint32_t)q.kListed && lines == all_lines;
         const uint32_t again = fits ? n * kLine : 0u;
-        constexpr int U = 2;
-        for (uint32_t i0 = threadIdx.x; i0 / kWave * kWave < again; i0 += BLOCK * U) {
-            typename Raw::type raw[U];
-            uint32_t number[U];
+        constexpr int AHEAD = 2;
+        for (uint32_t i0 = threadIdx.x; i0 / kWave * kWave < again; i0 += BLOCK * AHEAD) {
+            typename Raw::type raw[AHEAD];
+            uint32_t number[AHEAD];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
+            for (int u = 0; u < AHEAD; ++u) {
                 const uint32_t i = i0 + u * BLOCK;
                 number[u] = i < again ? q.list[i / kLine] * kLine + i % kLine : vectors;
                 raw[u] = Raw::load(body + (uint64_t)(part.lo + (number[u] < vectors ? number[u] : 0u)) * VEC);
             }
 #pragma unroll
-            for (int u = 0; u < U; ++u) append_vector(number[u] < vectors, part.lo + number[u], raw[u]);
+            for (int u = 0; u < AHEAD; ++u) append_vector(number[u] < vectors, part.lo + number[u], raw[u]);
         }
     }
     if (threadIdx.x < extra) {
@@ -348,10 +349,10 @@ __device__ __forceinline__ void join_tops(const KeyList& mine, const unsigned lo
 }
 
 // ---- forward -----------------------------------------------------------------------------------------
-// A workgroup reads a row, or a part of it, once, kLpUnroll vectors a thread in flight.  With HELD the part is no longer than
-// those, and they stay in registers for the alternatives; with LINES the pass leaves every line's largest logit for them.
+// A workgroup reads a row, or a part of it, once, U vectors a thread in flight.  With HELD the part is no longer than those, and
+// they stay in registers for the alternatives; with LINES the pass leaves every line's largest logit for them.
 enum LpMode { PLAIN, LINES, HELD };
-template <typename T, int VEC, bool ENT, LpMode MODE, int BLOCK>
+template <typename T, int VEC, bool ENT, LpMode MODE, int BLOCK, int U>
 __global__ void __launch_bounds__(BLOCK)
 logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
     __shared__ RowStat lds[BLOCK / kWave];
@@ -363,19 +364,19 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
     const RowParts<T, VEC> parts(base, a.V);
     const Stretch part(parts.nvec, nth, a.parts);
     const T* body = base + parts.head;
-    typename Raw::type raw[kLpUnroll];
-    float tops[kLpUnroll];
+    typename Raw::type raw[U];
+    float tops[U];
     RowStat t = empty_stat();
     auto read = [&](uint32_t i0) {
 #pragma unroll
-        for (int u = 0; u < kLpUnroll; ++u) {
+        for (int u = 0; u < U; ++u) {
             const uint32_t i = i0 + u * BLOCK;
             raw[u] = Raw::load(body + (uint64_t)(i < part.hi ? i : part.lo) * VEC);
         }
     };
     auto absorb = [&](uint32_t i0) {
 #pragma unroll
-        for (int u = 0; u < kLpUnroll; ++u) {
+        for (int u = 0; u < U; ++u) {
             tops[u] = -INFINITY;
             if (i0 + u * BLOCK < part.hi) {
                 float v[VEC];
@@ -399,13 +400,13 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
         absorb(part.lo + threadIdx.x);
     } else {
         const uint32_t lane = threadIdx.x % kWave;
-        for (uint32_t i0 = part.lo + (threadIdx.x - lane); i0 < part.hi; i0 += BLOCK * kLpUnroll) {     // (whole waves)
+        for (uint32_t i0 = part.lo + (threadIdx.x - lane); i0 < part.hi; i0 += BLOCK * U) {     // (whole waves)
             read(i0 + lane);
             absorb(i0 + lane);
             if constexpr (MODE == LINES) {
                 static_assert(kLine == 8, "the lanes of half a DPP row");
 #pragma unroll
-                for (int u = 0; u < kLpUnroll; ++u) {
+                for (int u = 0; u < U; ++u) {
                     float m = fmaxf(tops[u], dpp_move<kDppQuadXor1>(tops[u]));
                     m = fmaxf(m, dpp_move<kDppQuadXor2>(m));
                     m = fmaxf(m, dpp_move<kDppRowHalfMirror>(m));
@@ -418,7 +419,7 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
     const float best = t.m;
     t = block_stat<BLOCK, ENT>(t, a.c, lds);
     if constexpr (MODE != PLAIN)
-        if (a.top != 0) row_top<T, VEC, BLOCK, MODE == HELD>(base, parts, part, a.top, best, t.m, raw, tops, found);
+        if (a.top != 0) row_top<T, VEC, BLOCK, MODE == HELD, U>(base, parts, part, a.top, best, t.m, raw, tops, found);
     if constexpr (BLOCK == kLpBlock) if (a.parts > 1) {
         if (threadIdx.x == 0) {
             float* to = a.shared.stats + 4 * (uint64_t)blockIdx.x;
@@ -575,11 +576,11 @@ logprobs_bwd_kernel(const T* x, T* dx, const LpBwdArgs a, const FastDiv32 chunks
     lp_store<T, VEC>(out + first, v, a.accumulate);
 }
 
-template <typename T, int VEC, LpMode MODE, int BLOCK = kLpBlock>
+template <typename T, int VEC, LpMode MODE, int BLOCK = kLpBlock, int U = kLpUnroll>
 void lp_fwd_launch(hipStream_t s, const T* x, const LpArgs& a, uint64_t rows) {
     const dim3 grid((uint32_t)rows * a.parts), block(BLOCK);
-    if (a.entropy) hipLaunchKernelGGL((logprobs_fwd_kernel<T, VEC, true, MODE, BLOCK>), grid, block, 0, s, x, a);
-    else hipLaunchKernelGGL((logprobs_fwd_kernel<T, VEC, false, MODE, BLOCK>), grid, block, 0, s, x, a);
+    if (a.entropy) hipLaunchKernelGGL((logprobs_fwd_kernel<T, VEC, true, MODE, BLOCK, U>), grid, block, 0, s, x, a);
+    else hipLaunchKernelGGL((logprobs_fwd_kernel<T, VEC, false, MODE, BLOCK, U>), grid, block, 0, s, x, a);
 }
 
 // Rows of up to kLpUnroll vectors a thread, in the smallest workgroup that holds one: with many rows the reductions of its waves
@@ -606,7 +607,9 @@ int lp_fwd_typed(hipStream_t s, const T* x, LpArgs a, uint64_t rows) {
     const bool many = a.V <= (uint32_t)kLpBlock * kLpUnroll && vectors < 2 * a.top;
     if (a.V < 4 * WIDE || many) return lp_fwd_short<T, 1>(s, x, a, rows);
     if (vectors <= (uint32_t)kLpBlock / 2 * kLpUnroll) return lp_fwd_short<T, WIDE>(s, x, a, rows);
-    a.parts = row_parts(rows, vectors);
+    // (with alternatives a row is shared from where a workgroup cannot hold it: 4096 vectors in one, one row 8.4 us, 256 rows 9.6; in
+    // four parts 9.5 and 13.2)
+    a.parts = a.top != 0 && vectors <= kLpBlock * kMostHeld ? 1u : row_parts(rows, vectors);
     uint64_t slab = rows;
     if (a.top != 0) {
         if (a.parts * a.top > (uint32_t)kMaxShared) a.parts = kMaxShared / a.top;
@@ -618,7 +621,9 @@ int lp_fwd_typed(hipStream_t s, const T* x, LpArgs a, uint64_t rows) {
             slab = kSharedParts / a.parts;
         }
     }
-    const bool held = (vectors + a.parts - 1) / a.parts <= (uint32_t)kLpBlock * kLpUnroll;
+    const uint32_t longest = (vectors + a.parts - 1) / a.parts;
+    // (held against read again by lines: 8192 rows of 8192 fp32 with 20 alternatives 45.7 against 60.3 us, of 16384 88 against 94)
+    auto held = [&](uint32_t each) { return a.top != 0 && longest <= kLpBlock * each; };
     for (uint64_t r0 = 0; r0 < rows; r0 += slab) {
         const uint64_t n = rows - r0 < slab ? rows - r0 : slab;
         LpArgs b = a;
@@ -627,7 +632,9 @@ int lp_fwd_typed(hipStream_t s, const T* x, LpArgs a, uint64_t rows) {
         if (b.lse) b.lse += r0;
         if (b.top) { b.top_ids += r0 * b.top; b.top_logp += r0 * b.top; }
         const T* from = x + r0 * a.ld;
-        if (held) lp_fwd_launch<T, WIDE, HELD>(s, from, b, n);
+        if (held(4)) lp_fwd_launch<T, WIDE, HELD, kLpBlock, 4>(s, from, b, n);
+        else if (held(8)) lp_fwd_launch<T, WIDE, HELD, kLpBlock, 8>(s, from, b, n);
+        else if (held(kMostHeld)) lp_fwd_launch<T, WIDE, HELD, kLpBlock, kMostHeld>(s, from, b, n);
         else if (a.top != 0) lp_fwd_launch<T, WIDE, LINES>(s, from, b, n);
         else lp_fwd_launch<T, WIDE, PLAIN>(s, from, b, n);
     }
@@ -676,17 +683,19 @@ SharedRows shared_rows(void* scratch) {
                       reinterpret_cast<float*>(at + (16ull + 8ull * AGRAD_MAX_TOP + 4ull) * kSharedParts)};
 }
 
-// Parts of a row: as many as make 512 workgroups of all rows, or 1024 where the parts stay longer than 4096 vectors, but
-// none shorter than 1024, four vectors a thread, which stay in its registers for the alternatives (a part costs its
-// workgroup's reductions, and the parts are put together one after the other).  Up to 2048 vectors one workgroup is as fast:
-// what one leaves for another takes 2 us to arrive (one row of 8192 fp32 with 20 alternatives 7.8 us, in two parts 9.4, in
-// eight 9.2; of 16384 10.0, in four parts 9.5; of 65536 26, in eight 12.1, in sixteen 9.8).  48 rows of 18992 vectors, with
-// 8 alternatives: 10 parts each 16.2 us, 7 parts 17.0, 21 parts 16.5; 37 rows of 12564: 13 parts 12.5, 7 parts 13.3, 19 parts 14.3.
+// Parts of a row: of 1024 vectors, four a thread, or 2048 where that makes 256 workgroups of all rows, but not more than 512
+// workgroups, or 1024 where the parts stay longer than 4096 vectors (a part costs its workgroup's reductions, and the parts
+// are put together one after the other).  Up to 2048 vectors one workgroup is as fast: what one leaves for another takes 2 us to
+// arrive.  One row of 2048 vectors 4.1 us (two parts 4.9), of 4096 5.5 (four parts 4.9), of 16384 18.3 (four parts 7.3, eight 5.7,
+// sixteen 5.2); 64 rows of 8192 without alternatives: two parts 9.4, four 7.7, eight 7.7, sixteen 10.5; 37 rows of 12564 with
+// 5: five parts 12.6, seven 11.7, thirteen 12.4, nineteen 14.3; 48 rows of 18992 with 8: five parts 14.5, ten 14.2, nineteen 15.9.
 uint32_t row_parts(uint64_t rows, uint32_t vectors) {
     if (vectors <= 2048u) return 1u;
-    uint64_t parts = 512 / rows;
-    if (parts == 0 || vectors / parts > 4096) parts = kSharedParts / rows;
-    if (parts > (vectors + 1023u) / 1024u) parts = (vectors + 1023u) / 1024u;
+    uint64_t parts = (vectors + 1023u) / 1024u;
+    if (parts * rows >= 256) parts = (vectors + 2047u) / 2048u;
+    uint64_t most = 512 / rows;
+    if (most == 0 || vectors / most > 4096) most = kSharedParts / rows;
+    if (parts > most) parts = most;
     if (parts > kMaxParts) parts = kMaxParts;
     return parts < 1 ? 1u : (uint32_t)parts;
 }
