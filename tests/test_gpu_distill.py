@@ -95,6 +95,67 @@ def test_loss_and_gradient(ctx, rows, V, K, dtype, tail):
 
 @pytest.mark.parametrize("tail", [False, True])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,V,K", [(70, 40, 33), (70, 257, 64), (70, 600, 65), (9, 1030, 64), (9, 2049, 128), (9, 4100, 7), (9, 8200, 64), (5, 17000, 128)])
+def test_short_rows_and_many_slots(ctx, rows, V, K, dtype, tail):
+    """every size of a workgroup, with a thread a slot"""
+    rng = np.random.default_rng(rows + V + K)
+    x = L.logits(rng, rows, V, dtype)
+    ids, values = L.teacher(rng, rows, V, K, tail)
+    check(ctx, x, ids, values, dtype, scale=1.1, tail=tail)
+    check(ctx, x, ids, values, dtype, tail=tail, ld=V + 9, offset=3)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [45001, 60000, 80003, 90001, 162000, 170000])
+def test_more_rows_than_are_shared(ctx, V, dtype, tail):
+    """a workgroup a row, in registers or read twice; copies of three rows, which have to be copies afterwards where they start
+    at the same place within 16 bytes (elsewhere the vectors hold other classes, and the sums other orders)"""
+    rng = np.random.default_rng(V)
+    x = L.logits(rng, 3, V, dtype)
+    ids, values = L.teacher(rng, 3, V, 70, tail)
+    ids[0, :2] = [0, V - 1]
+    x[2, :V // 2] = -np.inf
+    x[2, ids[2]] = 1.0
+    bits = L.store(x, dtype)
+    loss, dz = cf.topk_distill(x, ids, values, 0.8, tail=tail)
+    w = np.array([1.0, -0.5, 2.0], np.float32)
+    b_loss, b_grad = bounds(x, ids, values, 0.8, 1.0, tail, dtype, w, dz * w[:, None])
+    n = 33
+    got, dx = L.distill_fused(ctx, np.tile(bits, (n, 1)), np.tile(ids, (n, 1)), np.tile(values, (n, 1)), scale=0.8, tail=tail,
+                              row_scale=np.tile(w, n))
+    for r in range(3 * n):
+        if r >= 24:
+            assert got[r] == got[r - 24] and (dx[r] == dx[r - 24]).all(), r
+        else:
+            L.assert_within(got[r], loss[r % 3], b_loss[r % 3], f"loss of row {r}")
+            L.assert_within(L.value(dx[r]), dz[r % 3] * w[r % 3], b_grad[r % 3], f"gradient of row {r}")
+    again, same = L.distill_fused(ctx, np.tile(bits, (n, 1)), np.tile(ids, (n, 1)), np.tile(values, (n, 1)), scale=0.8, tail=tail,
+                                  row_scale=np.tile(w, n), in_place=True)
+    np.testing.assert_array_equal(again, got)
+    np.testing.assert_array_equal(same, dx)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [20, 300, 5003])
+def test_classes_that_are_named_many_times(ctx, V, dtype, tail):
+    rng = np.random.default_rng(V)
+    rows, K = 6, 128
+    x = L.logits(rng, rows, V, dtype)
+    ids, values = L.teacher(rng, rows, V, K, tail, ragged=False)
+    ids[0, :] = 17                                   # one class, 128 times
+    ids[1, :] = rng.integers(0, V, K)
+    ids[2, :] = rng.integers(0, 10, K)
+    ids[3, 64:] = ids[3, :64]
+    ids[4, :] = np.where(np.arange(K) % 2, V - 1, 0)
+    ids[5, ::3] = -1
+    check(ctx, x, ids, values, dtype, tail=tail)
+    check(ctx, x, ids, values, dtype, tail=tail, ld=V + 3, offset=1)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("V,ld,offset", [(1003, 1003, 1), (1003, 1088, 3), (50257, 50304, 0), (37, 40, 5), (4096, 4100, 7), (16385, 16400, 2)])
 def test_strides_and_offsets(ctx, V, ld, offset, dtype, tail):
     rng = np.random.default_rng(V + offset)

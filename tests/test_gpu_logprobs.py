@@ -61,6 +61,21 @@ def test_forward(ctx, rows, V, dtype):
         check_forward(got, x, tokens, scale, top, f"top {top}")
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,V", [(70, 40), (70, 257), (70, 600), (9, 1030), (9, 2049), (9, 3001), (9, 7001), (9, 9001), (3, 16003), (3, 30011), (40, 50257)])
+def test_forward_of_rows_that_are_kept(ctx, rows, V, dtype):
+    """rows and parts of every length that stays in registers, in every size of a workgroup"""
+    rng = np.random.default_rng(V + rows)
+    few = L.logits(rng, min(rows, 9), V, dtype)
+    few[0, rng.random(V) < 0.7] = -np.inf
+    few[0, 5] = 1.0
+    x, tokens = np.tile(few, (-(-rows // len(few)), 1))[:rows], rng.integers(0, V, rows).astype(np.int32)
+    x[np.arange(rows), tokens] = 2.0
+    for top in (0, 3, 16, 32, 100):
+        got = L.forward(ctx, L.store(x, dtype), tokens, top, 0.9)
+        check_forward(got, x, tokens, 0.9, top, f"top {top}")
+
+
 def test_forward_outputs_on_their_own_and_together_have_the_same_bits(ctx):
     rng = np.random.default_rng(1)
     for V, dtype in ((777, "f32"), (50257, "bf16")):
@@ -171,6 +186,18 @@ def test_alternatives_come_in_order(ctx, V, dtype):
             np.testing.assert_array_equal(got["top_ids"][r], want[r][:top], err_msg=f"{name}, top {top}")
     many = L.forward(ctx, L.store(np.tile(x, (40, 1)), dtype), None, 64, entropy=False)     # (many rows: another split)
     np.testing.assert_array_equal(many["top_ids"], np.tile(want[:, :64], (40, 1)))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [300, 700, 1500, 7001, 15001, 30011])
+def test_alternatives_of_rows_that_are_kept_come_in_order(ctx, V, dtype):
+    names, xs = zip(*order_cases(V))
+    x = L.rounded(np.stack(xs), dtype)
+    want = cf.token_logprobs(x, np.full(len(x), -1), 1.0, 128)[3]
+    for top in (1, 16, 17, 32, 128):
+        got = L.forward(ctx, L.store(x, dtype), None, top, entropy=False)
+        for r, name in enumerate(names):
+            np.testing.assert_array_equal(got["top_ids"][r], want[r][:top], err_msg=f"{name}, top {top}")
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
