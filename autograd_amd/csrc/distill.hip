@@ -66,8 +66,8 @@ template <typename P>
 __device__ __forceinline__ void mark(uint32_t* map, uint32_t& outside, const P& parts, int32_t id, uint32_t first, uint32_t classes) {
     if (id < 0) return;
     const uint32_t at = (uint32_t)id - first;
-    if (at < classes) atomicOr(&map[at / 32], 1u << (at % 32));
-    else if ((uint32_t)id < parts.head) atomicOr(&outside, 1u << id);
+    if ((uint32_t)id < parts.head) atomicOr(&outside, 1u << id);
+    else if (at < classes) atomicOr(&map[at / 32], 1u << (at % 32));
     else if ((uint32_t)id >= parts.tail_start) atomicOr(&outside, 1u << (parts.head + ((uint32_t)id - parts.tail_start)));
 }
 // the bits of the vec-th vector
@@ -267,21 +267,22 @@ distill_fwd_kernel(const T* __restrict__ x, const DsArgs a, const DsOut o) {
     const int32_t asked = a.ids[slot_at];
     const float given = a.values[slot_at];
     typename Raw::type raw[kDsUnroll];
+    const uint32_t length = part.hi - part.lo, skew = line_skew<VEC>(body + (uint64_t)part.lo * VEC, length, BLOCK * kDsUnroll);
     auto read = [&](uint32_t i0) {
 #pragma unroll
         for (int u = 0; u < kDsUnroll; ++u) {
-            const uint32_t i = i0 + u * BLOCK;
-            raw[u] = Raw::load(body + (uint64_t)(i < part.hi ? i : part.lo) * VEC);
+            const uint32_t i = i0 + u * BLOCK - skew;
+            raw[u] = Raw::load(body + (uint64_t)(part.lo + (i < length ? i : 0u)) * VEC);
         }
     };
-    uint32_t i0 = part.lo + k;
-    if (i0 < part.hi) read(i0);
+    uint32_t i0 = k;
+    if (i0 < length + skew) read(i0);
     const int32_t id = k < a.top && asked >= 0 && (uint32_t)asked < a.V ? asked : -1;
     if (nth == 0 && k < a.top && id != asked && asked != -1) *a.err_flag = 1;
     float at[1];
     VecIO<T, 1>::load(base + (id >= 0 ? id : 0), at);
     if (k < AGRAD_MAX_TOP) slots.id[k] = id;
-    const uint32_t classes = (part.hi - part.lo) * VEC;
+    const uint32_t classes = length * VEC;
     if (TAIL) clear_map<BLOCK>(map, classes);
     if (TAIL && k == 0) outside = 0u;
     const bool used = __syncthreads_or(id >= 0) != 0;
@@ -291,13 +292,13 @@ distill_fwd_kernel(const T* __restrict__ x, const DsArgs a, const DsOut o) {
     const bool first = TAIL && k < AGRAD_MAX_TOP && own_slot<false>(slots, a.top, k, id).first;
     __syncthreads();
     RowStat t = empty_stat();
-    while (i0 < part.hi) {
+    while (i0 < length + skew) {
 #pragma unroll
         for (int u = 0; u < kDsUnroll; ++u) {
-            const uint32_t i = i0 + u * BLOCK;
-            if (i >= part.hi) continue;
+            const uint32_t i = i0 + u * BLOCK - skew;
+            if (i >= length) continue;
             if (TAIL) {
-                const uint32_t bits = bits_of<VEC>(map, i - part.lo);
+                const uint32_t bits = bits_of<VEC>(map, i);
                 if (bits != 0) mask_raw(raw[u], bits);
             }
             float v[VEC];
@@ -305,7 +306,7 @@ distill_fwd_kernel(const T* __restrict__ x, const DsArgs a, const DsOut o) {
             absorb_stat<false, VEC>(t, v, a.c);
         }
         i0 += BLOCK * kDsUnroll;
-        if (i0 < part.hi) read(i0);
+        if (i0 < length + skew) read(i0);
     }
     if (nth == 0 && k < parts.extra) {
         const uint32_t e = parts.extra_at(k);
@@ -383,8 +384,9 @@ distill_bwd_kernel(const T* x, T* dx, const DsArgs a, const float* dloss, const 
     const T* base = x + (uint64_t)row * a.ld;
     T* out = dx + (uint64_t)row * a.ld;
     const RowParts<T, VEC> parts(base, a.V);
+    // (its vectors are lo .. lo + span; of the first wave the first ones are before the row, large numbers)
     constexpr uint32_t span = kWave * U;
-    const uint32_t lo = chunk * span;
+    const uint32_t lo = chunk * span - line_skew<VEC>(base + parts.head);
     // slots lane and lane + 64
     static_assert(AGRAD_MAX_TOP == 2 * kWave, "");
     const int32_t* ids = a.ids + (uint64_t)row * a.top;
@@ -408,7 +410,7 @@ distill_bwd_kernel(const T* x, T* dx, const DsArgs a, const float* dloss, const 
         const uint32_t v = (uint32_t)id;
         if (id < 0 || v >= a.V) return 0xffffffffu;
         const uint32_t vec = v >= parts.head ? (v - parts.head) / VEC : 0xffffffffu;
-        if (vec < parts.nvec) return vec - lo < span ? vec % kWave : 0xffffffffu;
+        if (vec < parts.nvec) return vec - lo < span ? (vec - lo) % kWave : 0xffffffffu;
         return chunk == 0 ? (v < parts.head ? v : parts.head + (v - parts.tail_start)) : 0xffffffffu;
     };
     if (chunk == 0 && dloss != nullptr && ((id0 != -1 && (uint32_t)id0 >= a.V) || (id1 != -1 && (uint32_t)id1 >= a.V))) *a.err_flag = 1;
@@ -516,17 +518,19 @@ distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
     float at[1], xe[1];
     VecIO<T, 1>::load(base + (tid < parts.extra ? parts.extra_at(tid) : 0u), xe);
     typename Raw::type raw[U];
+    // places of vectors count from the 128 bytes in which the first one lies
+    const uint32_t skew = line_skew<VEC>(base + parts.head, parts.nvec, U * BLOCK), places = parts.nvec + skew;
     auto read = [&](uint32_t from) {
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const uint32_t vec = from + (uint32_t)i * BLOCK + tid;
+            const uint32_t vec = from + (uint32_t)i * BLOCK + tid - skew;
             const T* at_ = base + parts.head + (uint64_t)(vec < parts.nvec ? vec : 0u) * VEC;
             if constexpr (NV != 0) raw[i] = Raw::load(at_);
             else raw[i] = *reinterpret_cast<const typename Raw::type*>(at_);
         }
     };
     read(0);
-    if (TAIL) clear_map<BLOCK>(map, NV != 0 ? (uint32_t)(NV * BLOCK * VEC) : parts.nvec * VEC);
+    if (TAIL) clear_map<BLOCK>(map, NV != 0 ? (uint32_t)(NV * BLOCK * VEC) : places * VEC);
     if (TAIL && tid == 0) outside = 0u;
     patches.head[tid] = patches.kNone;
     const int32_t id = tid < a.top && asked >= 0 && (uint32_t)asked < a.V ? asked : -1;
@@ -537,7 +541,7 @@ distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
 
     // the teacher's side, and what the student says of the ids' classes
     if (tid < AGRAD_MAX_TOP) slots.id[tid] = id;
-    if (TAIL) mark(map, outside, parts, id, parts.head, parts.nvec * VEC);
+    if (TAIL) mark(map, outside, parts, id, parts.head - skew * VEC, places * VEC);
     const Teacher teach = teacher_row<BLOCK, TAIL>(a, u, id, lds);
     const float q = expf(teach.log_q);
     if (tid < AGRAD_MAX_TOP) slots.q[tid] = q;
@@ -551,19 +555,19 @@ distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
     // (with NV the map covers all vectors of a thread; a step of BLOCK vectors is whole words)
     static_assert(BLOCK * VEC % 32 == 0, "");
     const uint32_t shift_bits = tid * VEC % 32;
-    for (uint32_t from = 0; from < parts.nvec; from += U * BLOCK) {
+    for (uint32_t from = 0; from < places; from += U * BLOCK) {
         if (NV == 0 && from != 0) read(from);
         const uint32_t* words = map + (TAIL ? (from + tid) * VEC / 32 : 0u);
-        uint32_t bits = TAIL && from + tid < parts.nvec ? words[0] : 0u;
+        uint32_t bits = TAIL && from + tid < places ? words[0] : 0u;
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const uint32_t vec = from + (uint32_t)i * BLOCK + tid;
+            const uint32_t place = from + (uint32_t)i * BLOCK + tid;
             uint32_t ahead = 0;
-            if (TAIL && i + 1 < U && (NV != 0 || vec + BLOCK < parts.nvec)) {
+            if (TAIL && i + 1 < U && (NV != 0 || place + BLOCK < places)) {
                 ahead = words[(i + 1) * (BLOCK * VEC / 32)];
                 asm volatile("" ::: "memory");                     // (one vector's bits ahead, not all of them)
             }
-            if (vec < parts.nvec) {
+            if (place - skew < parts.nvec) {
                 if (TAIL) {
                     bits = (bits >> shift_bits) & ((1u << VEC) - 1u);
                     if (bits != 0) mask_raw(raw[i], bits);
@@ -595,7 +599,7 @@ distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
     // hand the ids' gradients to the threads that store their vectors
     if (own.first) {
         const uint32_t vec = (uint32_t)id >= parts.head ? ((uint32_t)id - parts.head) / VEC : 0xffffffffu;
-        const uint32_t who = vec < parts.nvec ? vec % BLOCK : ((uint32_t)id < parts.head ? (uint32_t)id : parts.head + ((uint32_t)id - parts.tail_start));
+        const uint32_t who = vec < parts.nvec ? (vec + skew) % BLOCK : ((uint32_t)id < parts.head ? (uint32_t)id : parts.head + ((uint32_t)id - parts.tail_start));
         patches.add(tid, who, id, own_grad(g, a, at[0], own.taken, mul));
     }
     __syncthreads();
@@ -620,17 +624,17 @@ distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
     };
     if constexpr (NV != 0) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) rewrite(raw[i], (uint32_t)i * BLOCK + again);
+        for (int i = 0; i < NV; ++i) rewrite(raw[i], (uint32_t)i * BLOCK + again - skew);
     } else {
-        for (uint32_t from = again; from < parts.nvec; from += 2 * BLOCK) {
+        for (uint32_t from = again; from < places; from += 2 * BLOCK) {
             typename Raw::type two[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const uint32_t vec = from + (uint32_t)i * BLOCK;
-                two[i] = Raw::load(base + parts.head + (uint64_t)(vec < parts.nvec ? vec : from) * VEC);
+                const uint32_t vec = from + (uint32_t)i * BLOCK - skew;
+                two[i] = Raw::load(base + parts.head + (uint64_t)(vec < parts.nvec ? vec : 0u) * VEC);
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i) rewrite(two[i], from + (uint32_t)i * BLOCK);
+            for (int i = 0; i < 2; ++i) rewrite(two[i], from + (uint32_t)i * BLOCK - skew);
         }
     }
     patches.store(out, tid);
@@ -687,7 +691,8 @@ int ds_bwd_typed(hipStream_t s, const T* x, T* dx, const DsArgs& a, const float*
     constexpr int WIDE = WideVec<T>::value;
     const bool wide = a.V >= 4 * WIDE && one_alignment(x, dx);
     const uint32_t vec = wide ? WIDE : 1, span = kWave * kBwdVectors;
-    const uint32_t chunks = (a.V / vec + span - 1) / span;
+    const bool lines = ((reinterpret_cast<uintptr_t>(x) | (rows > 1 ? a.ld * sizeof(T) : 0u)) & 127u) == 0;      // every row at 128 bytes
+    const uint32_t chunks = (a.V / vec + (wide && !lines ? 7u : 0u) + span - 1) / span;
     uint64_t max_rows = 0x03ffffffull / chunks;                  // waves of a launch: 2^32 threads
     if (max_rows == 0) max_rows = 1;
     for (uint64_t r0 = 0; r0 < rows; r0 += max_rows) {
@@ -726,7 +731,7 @@ bool ds_held_launch(hipStream_t s, const T* x, T* dx, const DsArgs& a, const DsO
         AGRAD_DS(12, 1024) AGRAD_DS(16, 1024) AGRAD_DS(20, 1024)
     }
 #undef AGRAD_DS
-    if (TAIL && vectors + 1 > kMapBits / WIDE) return false;
+    if (TAIL && vectors + 8 > kMapBits / WIDE) return false;
     hipLaunchKernelGGL((distill_held_kernel<T, WIDE, 0, 1024, TAIL>), grid, dim3(1024), 0, s, x, dx, a, o);
     return true;
 }

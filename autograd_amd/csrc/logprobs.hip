@@ -213,7 +213,7 @@ __device__ __forceinline__ void top_by_steps(uint32_t n, uint32_t top, Candidate
 template <typename T, int VEC, int BLOCK, bool HELD, int U>
 __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& parts, const Stretch& part, uint32_t top, float best, float largest,
                                         const typename RawVec<T, VEC>::type (&held)[U], const float (&tops)[U],
-                                        Candidates<BLOCK>& q) {
+                                        uint32_t skew, Candidates<BLOCK>& q) {
     typedef RawVec<T, VEC> Raw;
     const uint32_t extra = part.lo == 0 ? parts.extra : 0u, vectors = part.hi - part.lo;
     const uint32_t bound = bound_of<BLOCK>(q, (uint32_t)(class_key(best, 0u) >> 32), ordered(largest) >> 16, top);
@@ -260,7 +260,7 @@ __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& p
             append(q, i < classes && v[0] >= least, class_key(v[0], parts.head + q.list[i < classes ? i / VEC : 0u] * VEC + i % VEC));
         }
     } else {
-        const uint32_t all_lines = (vectors + kLine - 1) / kLine, lines = all_lines <= (uint32_t)kLines ? all_lines : 0u;
+        const uint32_t all_lines = (vectors + skew + kLine - 1) / kLine, lines = all_lines <= (uint32_t)kLines ? all_lines : 0u;
         const uint32_t from = bound < 0x80u ? 0x80u : bound;                 // (-inf is 0x7f)
         for (uint32_t j0 = 0; j0 < lines; j0 += BLOCK * 8) {
             const uint32_t j = j0 + threadIdx.x * 8;
@@ -287,7 +287,7 @@ __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& p
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
                 const uint32_t i = i0 + u * BLOCK;
-                number[u] = i < again ? q.list[i / kLine] * kLine + i % kLine : vectors;
+                number[u] = i < again ? q.list[i / kLine] * kLine + i % kLine - skew : vectors;      // (before the first: large)
                 raw[u] = Raw::load(body + (uint64_t)(part.lo + (number[u] < vectors ? number[u] : 0u)) * VEC);
             }
 #pragma unroll
@@ -367,18 +367,21 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
     typename Raw::type raw[U];
     float tops[U];
     RowStat t = empty_stat();
+    // lane 0 of the part's first wave stands before its first vector, where that is not at 128 bytes: whole lines a wave
+    const uint32_t length = part.hi - part.lo, skew = MODE == HELD ? 0u : line_skew<VEC>(body + (uint64_t)part.lo * VEC, length, BLOCK * U);
+    auto inside = [&](uint32_t i) { return MODE == HELD ? i < part.hi : i - part.lo < length; };
     auto read = [&](uint32_t i0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const uint32_t i = i0 + u * BLOCK;
-            raw[u] = Raw::load(body + (uint64_t)(i < part.hi ? i : part.lo) * VEC);
+            raw[u] = Raw::load(body + (uint64_t)(inside(i) ? i : part.lo) * VEC);
         }
     };
     auto absorb = [&](uint32_t i0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             tops[u] = -INFINITY;
-            if (i0 + u * BLOCK < part.hi) {
+            if (inside(i0 + u * BLOCK)) {
                 float v[VEC];
                 Raw::unpack(raw[u], v);
                 tops[u] = absorb_stat<ENT, VEC>(t, v, a.c);
@@ -400,9 +403,10 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
         absorb(part.lo + threadIdx.x);
     } else {
         const uint32_t lane = threadIdx.x % kWave;
-        for (uint32_t i0 = part.lo + (threadIdx.x - lane); i0 < part.hi; i0 += BLOCK * U) {     // (whole waves)
-            read(i0 + lane);
-            absorb(i0 + lane);
+        const uint32_t first = part.lo - skew + lane;                                 // (of wave 0; whole waves)
+        for (uint32_t i0 = threadIdx.x - lane; i0 < length + skew; i0 += BLOCK * U) {
+            read(first + i0);
+            absorb(first + i0);
             if constexpr (MODE == LINES) {
                 static_assert(kLine == 8, "the lanes of half a DPP row");
 #pragma unroll
@@ -410,7 +414,7 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
                     float m = fmaxf(tops[u], dpp_move<kDppQuadXor1>(tops[u]));
                     m = fmaxf(m, dpp_move<kDppQuadXor2>(m));
                     m = fmaxf(m, dpp_move<kDppRowHalfMirror>(m));
-                    const uint32_t line = (i0 - part.lo + u * BLOCK + lane) / kLine;
+                    const uint32_t line = (i0 + u * BLOCK + lane) / kLine;
                     if (lane % kLine == 0 && line < (uint32_t)kLines) found.line[line] = (uint16_t)(__float_as_uint(m) >> 16);
                 }
             }
@@ -419,7 +423,7 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
     const float best = t.m;
     t = block_stat<BLOCK, ENT>(t, a.c, lds);
     if constexpr (MODE != PLAIN)
-        if (a.top != 0) row_top<T, VEC, BLOCK, MODE == HELD, U>(base, parts, part, a.top, best, t.m, raw, tops, found);
+        if (a.top != 0) row_top<T, VEC, BLOCK, MODE == HELD, U>(base, parts, part, a.top, best, t.m, raw, tops, skew, found);
     if constexpr (BLOCK == kLpBlock) if (a.parts > 1) {
         if (threadIdx.x == 0) {
             float* to = a.shared.stats + 4 * (uint64_t)blockIdx.x;
@@ -566,7 +570,7 @@ logprobs_bwd_kernel(const T* x, T* dx, const LpBwdArgs a, const FastDiv32 chunks
         v[0] = lp_grad(v[0], r, e);
         lp_store<T, 1>(out + e, v, a.accumulate);
     }
-    const uint32_t i = chunk * BLOCK + threadIdx.x;
+    const uint32_t i = chunk * BLOCK + threadIdx.x - line_skew<VEC>(base + parts.head);
     if (i >= parts.nvec) return;
     const uint32_t first = parts.head + i * VEC;
     float v[VEC];
@@ -614,7 +618,7 @@ int lp_fwd_typed(hipStream_t s, const T* x, LpArgs a, uint64_t rows) {
     if (a.top != 0) {
         if (a.parts * a.top > (uint32_t)kMaxShared) a.parts = kMaxShared / a.top;
         // a part's lines have to fit LDS: rows of more than kLines lines are cut, so many rows a launch as the parts' memory takes
-        const uint32_t least = vectors / (uint32_t)(kLines * kLine) + 1;
+        const uint32_t least = (vectors + kLine) / (uint32_t)(kLines * kLine) + 1;
         if (least > a.parts) {
             a.parts = least < kMaxShared / a.top ? least : kMaxShared / a.top;
             if (a.parts > kMaxParts) a.parts = kMaxParts;
@@ -650,7 +654,8 @@ int lp_bwd_typed(hipStream_t s, const T* x, T* dx, LpBwdArgs a, uint64_t rows) {
     // (short rows leave most of a larger workgroup's threads idle: 32768 rows of 257 fp32 16.4 against 24.8 us, of 2048 bf16 42.5
     // against 45.0; longer rows are the same in both)
     const uint32_t block = a.V / vec <= 256u ? 64u : kLpBlock;
-    const uint32_t chunks = (a.V / vec + block - 1) / block;
+    const bool lines = ((reinterpret_cast<uintptr_t>(x) | (rows > 1 ? a.ld * sizeof(T) : 0u)) & 127u) == 0;      // every row at 128 bytes
+    const uint32_t chunks = (a.V / vec + (wide && !lines ? 7u : 0u) + block - 1) / block;
     uint64_t max_rows = 0x00ffffffull / chunks;                  // workgroups of a launch: 2^32 threads
     if (max_rows == 0) max_rows = 1;
     for (uint64_t r0 = 0; r0 < rows; r0 += max_rows) {
