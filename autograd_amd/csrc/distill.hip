@@ -741,9 +741,12 @@ bool ds_held_launch(hipStream_t s, const T* x, T* dx, const DsArgs& a, const DsO
 template <typename T>
 int ds_fused_typed(hipStream_t s, const T* x, T* dx, const DsArgs& a, const DsOut& o, uint64_t rows, bool tail) {
     constexpr int WIDE = WideVec<T>::value;
-    // (a CU reads a long row in 20 us: some tens of them are faster shared out, one row of 151936 bf16 11.8 against 23 us, 64 rows 23
-    // against 27, 128 rows 32 against 28; shorter rows never are by more than a microsecond)
-    const bool few = rows <= 96 && a.V / WIDE > 20 * 512;
+    // A CU takes up to 25 us for a long row; few of them are faster shared out in two launches, which are faster up to some number of rows
+    // that grows with the classes beyond 6000 vectors: one row of 151936 bf16 10.9 against 24.4 us, 96 rows 27.7 against 28.3, 160
+    // rows 36.9 against 33.7; of 90000 bf16, 32 rows 14.9 against 18.0, 64 rows 18.3 against 18.1; of 60000 fp32, 32 rows 14.8
+    // against 15.1, 64 rows 19.1 against 16.0; of 40000, 8 rows 11.2 against 11.5, 32 rows 13.2 against 11.9; of 32768 bf16, one
+    // row 10.8 against 9.3.
+    const bool few = a.V > 6000 * WIDE && rows * 900 <= a.V - 6000 * WIDE;
     if (a.V >= 4 * WIDE && one_alignment(x, dx) && !few) {
         if (tail ? ds_held_launch<T, true>(s, x, dx, a, o, rows) : ds_held_launch<T, false>(s, x, dx, a, o, rows))
             return check_hip(hipGetLastError(), "top-k distillation step launch");
