@@ -19,6 +19,7 @@ namespace {
 
 constexpr int kLpBlock = 256;
 constexpr int kLpUnroll = 4;         // vectors a thread keeps in flight
+constexpr uint32_t kManyRows = 1024; // more have their time by throughput, fewer by latency
 constexpr uint32_t kMostHeld = 16;   // and of a row that it keeps for its alternatives
 static_assert(AGRAD_MAX_TOP <= kLpBlock, "a thread an alternative");
 constexpr int kLine = 8;             // vectors of a line
@@ -589,11 +590,12 @@ void lp_fwd_launch(hipStream_t s, const T* x, const LpArgs& a, uint64_t rows) {
 
 // Rows of up to kLpUnroll vectors a thread, in the smallest workgroup that holds one: with many rows the reductions of its waves
 // are most of the time (32768 rows of 257 fp32 in 64 threads and in 256: 15 and 40 us without alternatives, 26 and 87 with 5).
-// The alternatives need four threads each, for a useful bound.
+// The alternatives need some threads each, for a useful bound: two do where there are many rows (32768 rows of 2000 bf16, 64
+// alternatives: 82 us, with four 127), and cost a few rows their latency (512 rows: 8.0 us, with four 7.2).
 template <typename T, int VEC>
 int lp_fwd_short(hipStream_t s, const T* x, const LpArgs& a, uint64_t rows) {
-    const uint32_t vectors = a.V / VEC;
-    auto fits = [&](uint32_t block) { return vectors <= block * kLpUnroll && 4 * a.top <= block; };
+    const uint32_t vectors = a.V / VEC, each = rows > kManyRows ? 2 : 4;
+    auto fits = [&](uint32_t block) { return vectors <= block * kLpUnroll && each * a.top <= block; };
     if (a.top == 0 && fits(64)) lp_fwd_launch<T, VEC, PLAIN, 64>(s, x, a, rows);
     else if (a.top == 0 && fits(128)) lp_fwd_launch<T, VEC, PLAIN, 128>(s, x, a, rows);
     else if (fits(64)) lp_fwd_launch<T, VEC, HELD, 64>(s, x, a, rows);
@@ -606,9 +608,11 @@ template <typename T>
 int lp_fwd_typed(hipStream_t s, const T* x, LpArgs a, uint64_t rows) {
     constexpr int WIDE = WideVec<T>::value;
     const uint32_t vectors = a.V / WIDE;
-    // Short rows with many alternatives go by single elements: of fewer vectors than twice the alternatives the threads' largest
-    // logits give no useful bound (1000 bf16 classes, 128 alternatives: 28.6 us, all of them candidates; by elements 6.9).
-    const bool many = a.V <= (uint32_t)kLpBlock * kLpUnroll && vectors < 2 * a.top;
+    // Short rows with many alternatives go by single elements: of fewer vectors than one and a half times the alternatives the threads'
+    // largest logits give no useful bound (1000 bf16 classes, 128 alternatives: 28.6 us, all of them candidates; by elements 6.9).
+    // Up to twice as many vectors, elements are faster for a few rows (512 rows of 600 bf16, 50 alternatives 6.2 against 6.9 us) and
+    // vectors for many (32768 rows 69 against 105).
+    const bool many = a.V <= (uint32_t)kLpBlock * kLpUnroll && 2 * vectors < (rows > kManyRows ? 3 : 4) * a.top;
     if (a.V < 4 * WIDE || many) return lp_fwd_short<T, 1>(s, x, a, rows);
     if (vectors <= (uint32_t)kLpBlock / 2 * kLpUnroll) return lp_fwd_short<T, WIDE>(s, x, a, rows);
     // (with alternatives a row is shared from where a workgroup cannot hold it: 4096 vectors in one, one row 8.4 us, 256 rows 9.6; in

@@ -201,6 +201,18 @@ def test_alternatives_of_rows_that_are_kept_come_in_order(ctx, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [40, 257, 601, 1000, 2001, 4000])
+def test_alternatives_of_many_short_rows_come_in_order(ctx, V, dtype):
+    xs = [x for _, x in order_cases(V)]
+    x = L.rounded(np.stack(xs), dtype)
+    want = cf.token_logprobs(x, np.full(len(x), -1), 1.0, 128)[3]
+    n = -(-1030 // len(x))
+    for top in (5, 20, 32, 33, 50, 64, 65, 100, 128):
+        got = L.forward(ctx, L.store(np.tile(x, (n, 1)), dtype), None, top, entropy=False)
+        np.testing.assert_array_equal(got["top_ids"], np.tile(want[:, :top], (n, 1)), err_msg=f"top {top}")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("rows,V", [(1, 1), (3, 7), (4, 129), (5, 1000), (3, 4099), (40, 517), (2, 50257), (2, 151936)])
 def test_backward(ctx, rows, V, dtype):
     rng = np.random.default_rng(2000 + V)
