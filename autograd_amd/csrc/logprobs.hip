@@ -351,7 +351,9 @@ __device__ __forceinline__ void join_tops(const KeyList& mine, const unsigned lo
 
 // ---- forward -----------------------------------------------------------------------------------------
 // A workgroup reads a row, or a part of it, once, U vectors a thread in flight.  With HELD the part is no longer than those, and
-// they stay in registers for the alternatives; with LINES the pass leaves every line's largest logit for them.
+// they stay in registers for the alternatives; with LINES the pass leaves every line's largest logit for them.  HBM bounds long
+// batches (4096 rows of 50257 fp32 with entropy 126 us, 6.5 TB/s; 8192 rows of 128256 bf16 with 64 alternatives 346 us, 6.1 TB/s),
+// latency the small ones (one row of 128256 bf16 with 20 alternatives 9.5 us, 5.5 without).
 enum LpMode { PLAIN, LINES, HELD };
 template <typename T, int VEC, bool ENT, LpMode MODE, int BLOCK, int U>
 __global__ void __launch_bounds__(BLOCK)
@@ -472,7 +474,8 @@ logprobs_fwd_kernel(const T* __restrict__ x, const LpArgs a) {
 
 // ---- backward ----------------------------------------------------------------------------------------
 // One vector a thread, a workgroup a chunk of a row (the most independent waves: a stream of one read and one write runs
-// best that way here).  With l = log p:  dx = scale * (g [v == token] - p (g + h entropy + h l)).
+// best that way here: 4096 rows of 128256 fp32 687 us, 2048 rows of 50257 bf16 66 us, 6.1 and 6.3 TB/s).  With l = log p:
+// dx = scale * (g [v == token] - p (g + h entropy + h l)).
 struct LpBwdArgs {
     const int32_t* tokens; const float* lse; const float* entropy; const float* dlogp; const float* dentropy;
     uint64_t ld; uint32_t V; float scale; uint32_t accumulate;
