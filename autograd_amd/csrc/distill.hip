@@ -178,6 +178,10 @@ struct PatchLists {
 };
 
 // ---- what a row's gradient is made of --------------------------------------------------------------------
+// Where p_rest is below fp32's numbers, down to classes at a mask's lowest value, the sums about m say nothing of the classes outside.
+// There a forward call leaves, in place of log p_rest and sum q, their own largest logit and -1 - the log of their sum about it; sum q
+// is negative in no other row.
+constexpr float kFarRest = -100.0f;                    // log p_rest, with fp32's error of 2^-17 in it
 // all: log of the student's whole sum about m, the largest logit (m = -inf: no gradient); log_rest: log of p_rest (TAIL;
 // -inf: no class outside), mass: sum q.  This is what a forward call leaves for its backward call, so that a row of logits
 // far from 0 loses nothing (an lse of 1e6 would have lost log p).
@@ -221,6 +225,7 @@ __device__ __forceinline__ RowSums finish_row(const DsArgs& a, const RowStat& pa
     RowSums s{all.m, log_s, -INFINITY, t.mass};
     if (TAIL && !(pass.m == -INFINITY && pass.s == 0.0f)) {
         s.log_rest = (pass.m - all.m) * a.scale + (logf(pass.s) - log_s);
+        if (s.log_rest == -INFINITY) s.log_rest = -3.4028234663852886e38f;          // (there are classes outside)
         const float q_rest = fmaxf(1.0f - t.mass, 0.0f);
         if (q_rest > 0.0f) loss = loss + q_rest * (logf(q_rest) - s.log_rest);
     }
@@ -340,6 +345,7 @@ distill_fwd_kernel(const T* __restrict__ x, const DsArgs a, const DsOut o) {
         if (o.stats != nullptr) {
             float* to = o.stats + row * 4ull;
             to[0] = s.m; to[1] = s.all; to[2] = TAIL ? s.log_rest : teach.lse; to[3] = s.mass;
+            if (TAIL && s.log_rest < kFarRest && s.log_rest > -INFINITY) { to[2] = t.m; to[3] = -1.0f - logf(t.s); }
         }
     }
 }
@@ -403,7 +409,16 @@ distill_bwd_kernel(const T* x, T* dx, const DsArgs a, const float* dloss, const 
     float xe[1];
     VecIO<T, 1>::load(base + (lane < extra ? e : 0u), xe);
     const float* st = stats + (uint64_t)row * 4;
-    const RowGrad g = row_grad<TAIL>(RowSums{st[0], st[1], TAIL ? st[2] : -INFINITY, st[3]});
+    RowGrad g = row_grad<TAIL>(RowSums{st[0], st[1], TAIL ? st[2] : -INFINITY, st[3]});
+    float from = g.m;                                     // what the exponentials of the classes outside are about
+    if (TAIL && st[3] < 0.0f) {
+        auto q_of = [&](int32_t id, uint32_t slot) { return id >= 0 && (uint32_t)id < a.V ? expf(a.values[(uint64_t)row * a.top + slot]) : 0.0f; };
+        const float mass = wave_sum(q_of(id0, lane) + q_of(id1, lane + kWave)), q_rest = fmaxf(1.0f - mass, 0.0f);
+        from = st[2];
+        g.out_log = -1.0f - st[3];
+        g.out = -q_rest;
+        g.mass = mass + q_rest;
+    }
     const float mul = a.scale * (dloss != nullptr ? dloss[row] : row_scale != nullptr ? row_scale[row] : grad_scale);
     const bool none = g.m == -INFINITY;
 
@@ -434,7 +449,7 @@ distill_bwd_kernel(const T* x, T* dx, const DsArgs a, const float* dloss, const 
     const float k = none ? 0.0f : g.out * mul, b = -g.out_log * kLog2eHi;
     if (none && accumulate) return;
     if (lane < extra) {
-        float d[1] = {none ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(xe[0] - g.m, a.c, b)) * k};
+        float d[1] = {none ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(xe[0] - from, a.c, b)) * k};
         ds_store<T, 1>(out + e, d, accumulate);
     }
 #pragma unroll
@@ -444,7 +459,7 @@ distill_bwd_kernel(const T* x, T* dx, const DsArgs a, const float* dloss, const 
         float v[VEC];
         Raw::unpack(raw[u], v);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = none ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(v[j] - g.m, a.c, b)) * k;
+        for (int j = 0; j < VEC; ++j) v[j] = none ? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(v[j] - from, a.c, b)) * k;
         ds_store<T, VEC>(out + parts.head + (uint64_t)i * VEC, v, accumulate);
     }
     if ((mine0 | mine1) == 0) return;

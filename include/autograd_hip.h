@@ -539,7 +539,8 @@ int agrad_token_logprobs_backward(agrad_ctx* ctx, int dtype, const void* logits,
  * gradient is finite); NaN or +inf makes a row NaN.
  *   forward   loss, and stats[rows, 4], fp32, for the backward call (may be NULL): the row's largest logit (-inf:
  *             no gradient), the logarithm of the sum of exp(z) about it, the teacher's lse (RENORM) or log p_rest
- *             (TAIL; -inf: no class outside), sum q
+ *             (TAIL; -inf: no class outside), sum q; where p_rest is below exp(-100) the last two are the
+ *             largest logit outside the ids and -1 - the logarithm of the sum about it
  *   backward  dlogits (+)= the gradient * dloss[r]
  *   fused     loss (may be NULL) and dlogits = the gradient * (row_scale[r], or grad_scale if row_scale is NULL)
  *             in one launch that reads the logits once where a row fits a workgroup's registers

@@ -229,12 +229,14 @@ def topk_distill(x, ids, values, scale=1.0, teacher_scale=1.0, tail=False):
         outside[[i for i, _ in used]] = False
         q_rest = max(0.0, 1.0 - mass)
         if tail and outside.any() and not np.isneginf(logp[r, outside]).all():
+            # (the classes outside on their own: next to a maximum of -3.4e38 their number would be lost in log_rest)
             m = logp[r, outside].max()
-            log_rest = m + np.log(np.exp(logp[r, outside] - m).sum())
+            e = np.exp(logp[r, outside] - m)
+            log_rest = m + np.log(e.sum())
             if q_rest > 0:
                 loss[r] += q_rest * (np.log(q_rest) - log_rest)
             grad[r] += (mass + q_rest) * p[r]
-            grad[r, outside] -= q_rest * np.exp(logp[r, outside] - log_rest)
+            grad[r, outside] -= q_rest * e / e.sum()
         else:
             grad[r] += mass * p[r]
     return loss, grad * s

@@ -34,10 +34,11 @@ def parts(x, ids, values, scale, teacher_scale, tail):
             out[ids[r, used]] = False
             if out.any() and np.isfinite(logp[r, out]).any():
                 m = logp[r, out].max()
-                log_rest = m + np.log(np.exp(logp[r, out] - m).sum())
+                e = np.exp(logp[r, out] - m)
+                log_rest = m + np.log(e.sum())
                 left = max(1.0 - q.sum(), 1e-9)
                 size[r] += np.abs(np.log(left)) + np.abs(log_rest)
-                rest[r, out] = np.exp(logp[r, out] - log_rest)
+                rest[r, out] = e / e.sum()
     return p, logp, lse, size, q_at, rest
 
 
@@ -247,6 +248,51 @@ def test_in_place_accumulate_and_scales(ctx, dtype):
             want = base + cf.topk_distill(x, ids, values, tail=tail)[1] * w.astype(np.float64)[:, None]
             _, bound = bounds(x, ids, values, 1.0, 1.0, tail, dtype, w, want)
             L.assert_within(L.value(acc), want, bound + 4 * U * np.abs(want) + (2.0 ** -8 * np.abs(want) if dtype == "bf16" else 0.0), "accumulated")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [300, 5003, 70000])
+def test_tail_far_below_the_ids(ctx, V, dtype):
+    """what the student gives to all other classes is below the smallest number: masks of the lowest value, large offsets"""
+    rng = np.random.default_rng(V)
+    rows, K, far = 6, 70, float(np.finfo(np.float32).min) if dtype == "f32" else -3.3895313892515355e38
+    x = L.logits(rng, rows, V, dtype)
+    ids, values = L.teacher(rng, rows, V, K, True, ragged=False)
+    values = (values - 0.5).astype(np.float32)
+    ids[1, 3] = ids[1, 66]
+    out = np.ones((rows, V), bool)
+    for r in range(rows):
+        out[r, ids[r]] = False
+    x[0, out[0]] = far
+    for r, by in ((1, 60000.0), (2, 150.0), (3, 101.0), (4, 90.0)):
+        x[r, out[r]] -= by
+    x[5, out[5]] = np.where(np.arange(out[5].sum()) % 2, far, far / 2)
+    x = L.rounded(x, dtype)
+    w = np.array([1, -0.5, 2, 1, 0.25, -1], np.float32)
+    for scale in (1.0, 0.75):
+        loss, dz = cf.topk_distill(x, ids, values, scale, tail=True)
+        p, logp, lse, size, q_at, rest = parts(x, ids, values, scale, 1.0, True)
+        want = dz * w[:, None]
+        # Distances are taken from the largest of their own kind, so that l is what an exponential's argument is off by in units of U;
+        # log p_rest enters it where it is above -100 (4 roundings); q = exp(u) is off by |u| U.
+        with np.errstate(divide="ignore"):
+            l = np.where(out, np.abs(np.where(rest > 0, np.log(np.where(rest > 0, rest, 1.0)), 0.0)), np.abs(np.where(p > 0, logp, 0.0)))
+        per = L.sum_error(V) + 2 * U * (K + 64) + U * (4 * l + 16 + 400)
+        u_max = np.abs(values).max()
+        bound = np.abs(w)[:, None] * scale * 2 * (per + 2 * U * u_max) * (p + q_at + rest) + 1e-37
+        if dtype == "bf16":
+            bound = bound + (np.abs(want) + bound) * 2.0 ** -8
+        bits = L.store(x, dtype)
+        got, stats = L.distill_forward(ctx, bits, ids, values, scale=scale, tail=True)
+        # (its terms are as large as the largest, with relative errors as above and of q_rest, a difference from 1)
+        b_loss = 2 * (L.sum_error(V) + 2 * U * (K + 64)) * size / np.minimum(1.0, 1.0 - q_at.sum(1))
+        L.assert_within(got, loss, b_loss, "loss")
+        dx = L.distill_backward(ctx, bits, ids, values, w, stats, scale=scale, tail=True)
+        f_loss, f_dx = L.distill_fused(ctx, bits, ids, values, scale=scale, tail=True, row_scale=w)
+        L.assert_within(f_loss, loss, b_loss, "loss of the step")
+        rel_q = (2 * U * (K + 64) / (1.0 - q_at.sum(1)))[:, None] * np.abs(w)[:, None] * scale * (rest + p)      # (q_rest is a difference)
+        L.assert_within(L.value(f_dx), want, bound + rel_q, f"gradient of the step, scale {scale}")
+        L.assert_within(L.value(dx), want, bound + rel_q, f"gradient, scale {scale}")
 
 
 def test_gradient_against_differences(ctx):

@@ -92,6 +92,18 @@ def test_distill_form_is_cross_entropy_at_its_ends():
     assert np.abs(loss).max() < 1e-14 and np.abs(grad).max() < 1e-15
 
 
+def test_distill_form_of_a_student_at_a_masks_lowest_value():
+    """a gradient's row adds up to 0, whatever the offset between the ids and the other classes"""
+    x = np.full((2, 40), float(np.finfo(np.float32).min))
+    x[:, :5] = np.arange(5)
+    x[1, 20:] /= 2
+    loss, grad = cf.topk_distill(x, np.tile(np.arange(5), (2, 1)), np.full((2, 5), np.log(0.15)), tail=True)
+    np.testing.assert_allclose(grad.sum(-1), 0, atol=1e-12)
+    np.testing.assert_allclose(grad[0, 5:], -0.25 / 35, rtol=1e-12)
+    np.testing.assert_allclose(grad[1, 20:], -0.25 / 20, rtol=1e-12)
+    assert not grad[1, 5:20].any()
+
+
 # ---- ops -----------------------------------------------------------------------------------------
 def test_ops_refuse_what_the_kernels_do_not_take():
     assert MAX_TOP == capi.MAX_TOP
