@@ -79,11 +79,15 @@ __device__ __forceinline__ uint32_t take_place(uint32_t& count, bool has) {
     at = (uint32_t)__builtin_amdgcn_readlane((int)at, (int)first);
     return has ? at + __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0u)) : 0xffffffffu;
 }
-// The same for several of a lane's, at most 15: the first of its places.  All lanes of the wave take part.
+// The same for several of a lane's, at most MOST: the first of its places.  All lanes of the wave take part.  A ballot a bit of
+// MOST: a count that has more bits than are balloted would be taken for a smaller one, and lanes would share places.
+template <int MOST>
 __device__ __forceinline__ uint32_t take_places(uint32_t& count, uint32_t mine) {
+    static_assert(MOST > 0 && MOST <= kWave, "a count of a lane");
+    constexpr int BITS = 32 - __builtin_clz((unsigned)MOST);
     uint32_t before = 0, total = 0;
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
+    for (int b = 0; b < BITS; ++b) {
         const uint64_t lanes = __ballot((mine >> b) & 1u);
         before += __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0u)) << b;
         total += (uint32_t)__popcll(lanes) << b;
@@ -227,7 +231,7 @@ __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& p
         uint32_t mine = 0;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) mine += has && v[k] >= least ? 1u : 0u;
-        uint32_t at = take_places(q.count, mine);
+        uint32_t at = take_places<VEC>(q.count, mine);
         if (mine == 0) return;
 #pragma unroll
         for (int k = 0; k < VEC; ++k) {
@@ -241,7 +245,7 @@ __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& p
         uint32_t reach = 0;
 #pragma unroll
         for (int u = 0; u < U; ++u) reach += tops[u] >= least ? 1u : 0u;
-        uint32_t at = take_places(q.listed, reach);
+        uint32_t at = take_places<U>(q.listed, reach);            // (all U vectors of a thread may reach it)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (!(tops[u] >= least)) continue;
@@ -263,17 +267,18 @@ __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& p
     } else {
         const uint32_t all_lines = (vectors + skew + kLine - 1) / kLine, lines = all_lines <= (uint32_t)kLines ? all_lines : 0u;
         const uint32_t from = bound < 0x80u ? 0x80u : bound;                 // (-inf is 0x7f)
-        for (uint32_t j0 = 0; j0 < lines; j0 += BLOCK * 8) {
-            const uint32_t j = j0 + threadIdx.x * 8;
+        constexpr int EACH = 8;                                              // lines a thread looks at: one load
+        for (uint32_t j0 = 0; j0 < lines; j0 += BLOCK * EACH) {
+            const uint32_t j = j0 + threadIdx.x * EACH;
             u32x4 w = *reinterpret_cast<const u32x4*>(q.line + (j < lines ? j : 0u));
             const uint32_t pair[4] = {w.x, w.y, w.z, w.w};
             uint32_t reach = 0;
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
+            for (int k = 0; k < EACH; ++k) {
                 const uint32_t h = k % 2 ? pair[k / 2] >> 16 : pair[k / 2] & 0xffffu;
                 if (j + k < lines && ordered_half(h) >= from) reach |= 1u << k;
             }
-            uint32_t at = take_places(q.listed, (uint32_t)__popc(reach));
+            uint32_t at = take_places<EACH>(q.listed, (uint32_t)__popc(reach));
             for (; reach != 0; reach &= reach - 1u, ++at)
                 if (at < (uint32_t)q.kListed) q.list[at] = j + (uint32_t)__builtin_ctz(reach);
         }

@@ -408,3 +408,51 @@ def test_refusals(ctx):
                 ctx.call("agrad_token_logprobs_backward", *{**back, **over}.values())
             assert e.value.code == capi.EINVAL
     ctx.synchronize()
+
+
+def crowded_cases(V):
+    """order_cases, and rows in which a workgroup's threads find all that they hold among the candidates, or none"""
+    yield from order_cases(V)
+    rng = np.random.default_rng(V + 1)
+    i = np.arange(V)
+    for period in (1024, 2048):
+        yield f"masked but for every {period}th vector", np.where(i % period < 8, 1.0 + i / V, -np.inf)
+    yield "far from zero", 1000.0 + rng.standard_normal(V)               # (few steps of 16 bits)
+    yield "far below zero", -60000.0 + rng.standard_normal(V)
+    yield "one class", np.where(i == V - 3, 1.0, -np.inf)
+
+
+def assert_order(ctx, dtype, V, rows):
+    names, xs = zip(*crowded_cases(V))
+    x = L.rounded(np.stack(xs), dtype)
+    want = cf.token_logprobs(x, np.full(len(x), -1), 1.0, 128)[3]
+    n = -(-rows // len(x)) if rows else 1
+    at = np.arange(n * len(x))[:rows or None] % len(x)
+    bits = L.store(x, dtype)[at]
+    for top in (1, 5, 20, 64, 128):
+        got = L.forward(ctx, bits, None, top, entropy=False)["top_ids"]
+        for r, i in enumerate(at):
+            np.testing.assert_array_equal(got[r], want[i, :top], err_msg=f"row {r}, {names[i]}, top {top}")
+
+
+@pytest.mark.parametrize("dtype,V", [("f32", 4096), ("f32", 8192), ("f32", 15364), ("f32", 16384), ("f32", 16387),
+                                     ("bf16", 8192), ("bf16", 16384), ("bf16", 30728), ("bf16", 32000), ("bf16", 32768), ("bf16", 32775)])
+def test_alternatives_of_rows_that_fill_their_threads(ctx, dtype, V):
+    """rows of 4, 8 and 16 vectors a thread, and next to that: up to all of a thread's vectors are candidates"""
+    assert_order(ctx, dtype, V, 0)
+
+
+@pytest.mark.parametrize("dtype,V,rows", [("f32", 32768, 400), ("f32", 65536, 220), ("bf16", 65536, 200), ("bf16", 65536, 256),
+                                          ("bf16", 131072, 110), ("bf16", 128256, 128)])
+def test_alternatives_of_parts_that_fill_their_threads(ctx, dtype, V, rows):
+    """the same for rows that two or four workgroups share, of 16 vectors a thread each"""
+    assert_order(ctx, dtype, V, rows)
+
+
+@pytest.mark.parametrize("dtype,V", [("f32", 16384), ("bf16", 32768)])
+def test_equal_logits_have_their_alternatives(ctx, dtype, V):
+    """an output head of zeros: every class as likely as another, the lowest ids first"""
+    x = np.zeros((3, V), np.float32)
+    got = L.forward(ctx, L.store(x, dtype), np.array([0, V - 1, -1], np.int32), 9)
+    check_forward(got, x, np.array([0, V - 1, -1]), 1.0, 9)
+    np.testing.assert_array_equal(got["top_ids"], np.tile(np.arange(9), (3, 1)))
