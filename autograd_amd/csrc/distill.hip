@@ -118,7 +118,7 @@ __device__ __forceinline__ Teacher teacher_row(const DsArgs& a, float u, int32_t
     if (total == 0.0f) return Teacher{-INFINITY, 0.0f, INFINITY};
     t.lse = m + logf(total);
     t.log_q = w - t.lse;
-    t.mass = 1.0f;
+    t.mass = total == total ? 1.0f : total;                        // (NaN for a value of NaN or +inf)
     return t;
 }
 
@@ -184,7 +184,8 @@ struct PatchLists {
 constexpr float kFarRest = -100.0f;                    // log p_rest, with fp32's error of 2^-17 in it
 // all: log of the student's whole sum about m, the largest logit (m = -inf: no gradient); log_rest: log of p_rest (TAIL;
 // -inf: no class outside), mass: sum q.  This is what a forward call leaves for its backward call, so that a row of logits
-// far from 0 loses nothing (an lse of 1e6 would have lost log p).
+// far from 0 loses nothing (an lse of 1e6 would have lost log p).  A row whose loss is NaN has NaN in all four, so that its whole
+// gradient is NaN: its largest logit alone may be -inf, which would say that there is none.
 struct RowSums {
     float m, all, log_rest, mass;
 };
@@ -232,6 +233,9 @@ __device__ __forceinline__ RowSums finish_row(const DsArgs& a, const RowStat& pa
     if (!used || t.lse == INFINITY || (all.m == -INFINITY && all.s == 0.0f)) {
         loss = 0.0f;
         s = RowSums{-INFINITY, 0.0f, -INFINITY, 0.0f};
+    } else if (log_s != log_s || !(t.mass < INFINITY)) {           // NaN or +inf among the logits, or the teacher's values
+        loss = NAN;
+        s = RowSums{NAN, NAN, NAN, NAN};
     }
     return s;
 }
@@ -625,7 +629,7 @@ distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
 
     // exponentials about the largest logit outside the ids (RENORM: of all)
     const float shift = t.m > -INFINITY ? t.m : 0.0f;
-    const float k = t.s == 0.0f ? 0.0f : g.out * mul / t.s;
+    const float k = g.out * mul / (t.s == 0.0f ? 1.0f : t.s);            // (without classes outside g.out is 0, or NaN with the row)
     if (tid < parts.extra) {
         float d[1] = {__builtin_amdgcn_exp2f((xe[0] - shift) * a.c) * k};
         VecIO<T, 1>::store(out + parts.extra_at(tid), d);

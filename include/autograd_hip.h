@@ -536,7 +536,8 @@ int agrad_token_logprobs_backward(agrad_ctx* ctx, int dtype, const void* logits,
  * holds twice counts with both its values, its class once.  An id outside [-1, V) sets the deferred index error
  * and counts as unused.  A value of -inf is a slot of probability 0.  A row without used slots, or whose logits are
  * all -inf, has loss 0 and a zero gradient; a class at -inf that the teacher gives mass to makes the loss +inf (its
- * gradient is finite); NaN or +inf makes a row NaN.
+ * gradient is finite); NaN or +inf among the logits or the used slots' values (TAIL: or values whose sum q overflows) makes
+ * the row NaN, loss and whole gradient.
  *   forward   loss, and stats[rows, 4], fp32, for the backward call (may be NULL): the row's largest logit (-inf:
  *             no gradient), the logarithm of the sum of exp(z) about it, the teacher's lse (RENORM) or log p_rest
  *             (TAIL; -inf: no class outside), sum q; where p_rest is below exp(-100) the last two are the

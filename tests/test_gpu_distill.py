@@ -388,3 +388,55 @@ def test_refusals_and_no_rows(ctx):
             none = {k: (None if isinstance(v, C.c_void_p) else v) for k, v in good.items()}
             ctx.call("agrad_topk_distill_" + name, *{**none, "rows": 0}.values())
     ctx.synchronize()
+
+
+def three_ways(ctx, bits, ids, values, w, **kw):
+    """(name, loss, gradient) of forward and backward, of the step, and of a backward call that accumulates"""
+    loss, stats = L.distill_forward(ctx, bits, ids, values, **kw)
+    yield "two calls", loss, L.value(L.distill_backward(ctx, bits, ids, values, w, stats, **kw))
+    f_loss, f_dx = L.distill_fused(ctx, bits, ids, values, row_scale=w, **kw)
+    yield "step", f_loss, L.value(f_dx)
+    acc = L.distill_backward(ctx, bits, ids, values, w, stats, flags=capi.ACC_INPUT_GRAD, init=np.zeros_like(bits), **kw)
+    yield "accumulated", loss, L.value(acc)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V,copies", [(20, 1), (300, 1), (5003, 1), (90000, 1), (90000, 8)])
+def test_rows_with_nan_or_infinity_are_nan(ctx, V, copies, dtype, tail):
+    """loss and whole gradient, also where no class of the row is a number; what is left of other rows is as it was"""
+    rng = np.random.default_rng(V)
+    rows, K = 12, 6
+    x = L.logits(rng, rows, V, dtype)
+    ids, values = L.teacher(rng, rows, V, K, tail, ragged=False)
+    other = [next(v for v in range(V // 2, V) if v not in ids[r]) for r in range(rows)]
+    x[0, :] = np.nan
+    x[1, :] = -np.inf
+    x[1, other[1]] = np.nan
+    x[2, :] = -np.inf
+    x[2, ids[2, 0]] = np.nan
+    x[3, :] = -np.inf
+    x[3, other[3]] = np.inf
+    x[4, ids[4, 3]] = np.nan
+    x[5, other[5]] = np.nan
+    values[6, 1] = np.nan
+    values[7, 2] = np.inf
+    for r, low in ((8, -200.0), (9, -np.inf)):           # the teacher's NaN where the student gives next to nothing, or nothing, to the rest
+        out = np.ones(V, bool)
+        out[ids[r]] = False
+        x[r, out] = low
+        values[r, 0] = np.nan
+    bad = np.arange(rows) < 10
+    bits, at = L.store(x, dtype), np.tile(np.arange(rows), copies)
+    w = np.where(np.arange(rows) % 2, -0.5, 2.0).astype(np.float32)
+    ok = ~bad
+    want_loss, dz = cf.topk_distill(x[ok], ids[ok], values[ok], tail=tail)
+    want = dz * w[ok, None]
+    b_loss, b_grad = bounds(x[ok], ids[ok], values[ok], 1.0, 1.0, tail, dtype, w[ok], want)
+    for name, loss, dx in three_ways(ctx, bits[at], ids[at], values[at], w[at], tail=tail):
+        for r in np.flatnonzero(bad[at]):
+            assert np.isnan(loss[r]) and np.isnan(dx[r]).all(), (name, at[r], loss[r], np.isnan(dx[r]).mean())
+        for r in np.flatnonzero(ok[at]):
+            i = at[r] - 10
+            L.assert_within(loss[r], want_loss[i], b_loss[i], f"{name}: loss of row {r}")
+            L.assert_within(dx[r], want[i], b_grad[i], f"{name}: gradient of row {r}")
