@@ -1,7 +1,7 @@
 // Distillation from a teacher's top logits: the Kullback-Leibler divergence of the student's distribution
 // p = softmax(scale * x) from a teacher's q, of which `top` classes a row are known, and its gradient.
 //
-//   RENORM   q = softmax(teacher_scale * u) over the row's used slots
+//   RENORM   q = softmax(teacher_scale * u) over the row's used slots, about the largest u
 //            loss = sum_k q_k (log q_k - log p[id_k])
 //   TAIL     q_k = exp(u_k), the values are log probabilities; what they leave, q_rest = max(0, 1 - sum q), belongs to
 //            all the other classes together, to which the student gives p_rest = sum of p outside the ids
@@ -97,29 +97,24 @@ __device__ __forceinline__ void mask_raw(float& r, uint32_t bits) { if (bits) r 
 __device__ __forceinline__ void mask_raw(bf16_t& r, uint32_t bits) { if (bits) r = 0xff80; }
 
 // ---- the teacher's side of a row ------------------------------------------------------------------------
-// Thread k has slot k, with the value u (-inf, if unused): log q.  For everyone: sum q, the softmax's denominator (RENORM; +inf: no slots
-// to learn from).
+// Thread k has slot k, with the value u (-inf, if unused): log q.  For everyone: sum q, and of the softmax (RENORM) its largest
+// value and the log of its sum about that (+inf: no slots to learn from).  The two are kept apart: together they would be rounded at the
+// size of the values, whose common offset is no part of q (64 values of 1e6: log q off by 0.03).
 struct Teacher {
-    float log_q, mass, lse;
+    float log_q, mass, top, log_sum;
 };
+// log q of a value: distances to the largest first
+__device__ __forceinline__ float renorm_log_q(float u, float top, float log_sum, float teacher_scale) { return (u - top) * teacher_scale - log_sum; }
 template <int BLOCK, bool TAIL>
-__device__ __forceinline__ Teacher teacher_row(const DsArgs& a, float u, int32_t id, float* lds) {
-    Teacher t;
-    if (TAIL) {
-        t.log_q = u;
-        t.lse = 0.0f;
-        t.mass = block_total<BLOCK>(expf(u), lds);
-        return t;
-    }
-    const float w = id >= 0 ? u * a.teacher_scale : -INFINITY;
-    const float m = block_largest<BLOCK>(w, lds);
-    const float e = m == -INFINITY ? (w != w ? w : 0.0f) : expf(w - m);
+__device__ __forceinline__ Teacher teacher_row(const DsArgs& a, float u, float* lds) {
+    if (TAIL) return Teacher{u, block_total<BLOCK>(expf(u), lds), 0.0f, 0.0f};
+    const float top = block_largest<BLOCK>(u, lds);
+    const float e = top == -INFINITY ? (u != u ? u : 0.0f) : expf((u - top) * a.teacher_scale);
     const float total = block_total<BLOCK>(e, lds);
-    if (total == 0.0f) return Teacher{-INFINITY, 0.0f, INFINITY};
-    t.lse = m + logf(total);
-    t.log_q = w - t.lse;
-    t.mass = total == total ? 1.0f : total;                        // (NaN for a value of NaN or +inf)
-    return t;
+    if (total == 0.0f) return Teacher{-INFINITY, 0.0f, -INFINITY, INFINITY};
+    const float log_sum = logf(total);
+    // (sum q is 1; NaN for a value of NaN or +inf)
+    return Teacher{renorm_log_q(u, top, log_sum, a.teacher_scale), total == total ? 1.0f : total, top, log_sum};
 }
 
 // Slots in LDS.  A class that a row names twice counts with both its q; only its first slot stands for it.
@@ -230,7 +225,7 @@ __device__ __forceinline__ RowSums finish_row(const DsArgs& a, const RowStat& pa
         const float q_rest = fmaxf(1.0f - t.mass, 0.0f);
         if (q_rest > 0.0f) loss = loss + q_rest * (logf(q_rest) - s.log_rest);
     }
-    if (!used || t.lse == INFINITY || (all.m == -INFINITY && all.s == 0.0f)) {
+    if (!used || t.log_sum == INFINITY || (all.m == -INFINITY && all.s == 0.0f)) {
         loss = 0.0f;
         s = RowSums{-INFINITY, 0.0f, -INFINITY, 0.0f};
     } else if (log_s != log_s || !(t.mass < INFINITY)) {           // NaN or +inf among the logits, or the teacher's values
@@ -298,7 +293,7 @@ distill_fwd_kernel(const T* __restrict__ x, const DsArgs a, const DsOut o) {
     if (TAIL && k == 0) outside = 0u;
     const bool used = __syncthreads_or(id >= 0) != 0;
     if (TAIL) mark(map, outside, parts, id, parts.head + part.lo * VEC, classes);
-    const Teacher teach = teacher_row<BLOCK, TAIL>(a, id >= 0 ? given : -INFINITY, id, lds);
+    const Teacher teach = teacher_row<BLOCK, TAIL>(a, id >= 0 ? given : -INFINITY, lds);
     const float q = expf(teach.log_q);
     const bool first = TAIL && k < AGRAD_MAX_TOP && own_slot<false>(slots, a.top, k, id).first;
     __syncthreads();
@@ -348,7 +343,7 @@ distill_fwd_kernel(const T* __restrict__ x, const DsArgs a, const DsOut o) {
         if (o.loss != nullptr) o.loss[row] = loss;
         if (o.stats != nullptr) {
             float* to = o.stats + row * 4ull;
-            to[0] = s.m; to[1] = s.all; to[2] = TAIL ? s.log_rest : teach.lse; to[3] = s.mass;
+            to[0] = s.m; to[1] = s.all; to[2] = TAIL ? s.log_rest : teach.log_sum; to[3] = TAIL ? s.mass : teach.top;
             if (TAIL && s.log_rest < kFarRest && s.log_rest > -INFINITY) { to[2] = t.m; to[3] = -1.0f - logf(t.s); }
         }
     }
@@ -413,7 +408,7 @@ distill_bwd_kernel(const T* x, T* dx, const DsArgs a, const float* dloss, const 
     float xe[1];
     VecIO<T, 1>::load(base + (lane < extra ? e : 0u), xe);
     const float* st = stats + (uint64_t)row * 4;
-    RowGrad g = row_grad<TAIL>(RowSums{st[0], st[1], TAIL ? st[2] : -INFINITY, st[3]});
+    RowGrad g = row_grad<TAIL>(RowSums{st[0], st[1], TAIL ? st[2] : -INFINITY, TAIL ? st[3] : 1.0f});
     float from = g.m;                                     // what the exponentials of the classes outside are about
     if (TAIL && st[3] < 0.0f) {
         auto q_of = [&](int32_t id, uint32_t slot) { return id >= 0 && (uint32_t)id < a.V ? expf(a.values[(uint64_t)row * a.top + slot]) : 0.0f; };
@@ -444,7 +439,7 @@ distill_bwd_kernel(const T* x, T* dx, const DsArgs a, const float* dloss, const 
             const float u = a.values[(uint64_t)row * a.top + slot];
             VecIO<T, 1>::load(base + id, at);
             if (accumulate) VecIO<T, 1>::load(out + id, old);
-            q = TAIL ? expf(u) : expf(u * a.teacher_scale - st[2]);
+            q = expf(TAIL ? u : renorm_log_q(u, st[3], st[2], a.teacher_scale));
         };
         ask(who0 != 0xffffffffu, id0, lane, at0, old0, q0);
         ask(who1 != 0xffffffffu, id1, lane + kWave, at1, old1, q1);
@@ -565,7 +560,7 @@ distill_held_kernel(const T* x, T* dx, const DsArgs a, const DsOut o) {
     // the teacher's side, and what the student says of the ids' classes
     if (tid < AGRAD_MAX_TOP) slots.id[tid] = id;
     if (TAIL) mark(map, outside, parts, id, parts.head - skew * VEC, places * VEC);
-    const Teacher teach = teacher_row<BLOCK, TAIL>(a, u, id, lds);
+    const Teacher teach = teacher_row<BLOCK, TAIL>(a, u, lds);
     const float q = expf(teach.log_q);
     if (tid < AGRAD_MAX_TOP) slots.q[tid] = q;
     __syncthreads();

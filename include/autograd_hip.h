@@ -539,8 +539,9 @@ int agrad_token_logprobs_backward(agrad_ctx* ctx, int dtype, const void* logits,
  * gradient is finite); NaN or +inf among the logits or the used slots' values (TAIL: or values whose sum q overflows) makes
  * the row NaN, loss and whole gradient.
  *   forward   loss, and stats[rows, 4], fp32, for the backward call (may be NULL): the row's largest logit (-inf:
- *             no gradient), the logarithm of the sum of exp(z) about it, the teacher's lse (RENORM) or log p_rest
- *             (TAIL; -inf: no class outside), sum q; where p_rest is below exp(-100) the last two are the
+ *             no gradient), the logarithm of the sum of exp(z) about it, and
+ *             RENORM: the logarithm of the teacher's sum about the largest of the used values, and that value
+ *             TAIL: log p_rest (-inf: no class outside), sum q; where p_rest is below exp(-100) instead of them the
  *             largest logit outside the ids and -1 - the logarithm of the sum about it
  *   backward  dlogits (+)= the gradient * dloss[r]
  *   fused     loss (may be NULL) and dlogits = the gradient * (row_scale[r], or grad_scale if row_scale is NULL)

@@ -440,3 +440,34 @@ def test_rows_with_nan_or_infinity_are_nan(ctx, V, copies, dtype, tail):
             i = at[r] - 10
             L.assert_within(loss[r], want_loss[i], b_loss[i], f"{name}: loss of row {r}")
             L.assert_within(dx[r], want[i], b_grad[i], f"{name}: gradient of row {r}")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V,copies", [(300, 1), (5003, 1), (60000, 1), (60000, 10)])
+def test_teachers_far_from_zero(ctx, V, copies, dtype):
+    """Renormalised values with a common offset, of which q is free.  Their distances to the largest are exact (numbers of one
+    size) and take at most two roundings more with the scale, so that the bound is that of values without the offset."""
+    rng = np.random.default_rng(V)
+    rows, K, low = 8, 64, np.finfo(np.float32).min
+    x = L.logits(rng, rows, V, dtype)
+    ids, values = L.teacher(rng, rows, V, K, False)
+    values[0] += np.float32(1e6)
+    values[1] -= np.float32(1e6)
+    values[2] = 1e6                                  # all equal: q = 1 / 64
+    values[3] = low
+    values[4] = -low
+    values[5, 1:] = low                              # one class and a mask of the lowest value
+    values[6] += np.float32(300.0)
+    values[7] = np.where(np.arange(K) % 2, low, -np.inf)
+    bits, at = L.store(x, dtype), np.tile(np.arange(rows), copies)
+    w = np.where(np.arange(rows) % 2, -0.5, 2.0).astype(np.float32)
+    for teacher_scale in (1.0, 0.5, 1.75):
+        loss_want, dz = cf.topk_distill(x, ids, values, 0.8, teacher_scale)
+        want = dz * w[:, None]
+        top = np.where(ids >= 0, values, -np.inf).max(1, keepdims=True).astype(np.float64)
+        about = np.where(np.isfinite(values), values - top, -np.inf)
+        about = np.where(about < -1e30, -np.inf, about)                    # (q = 0)
+        b_loss, b_grad = bounds(x, ids, about, 0.8, teacher_scale, False, dtype, w, want)
+        for name, loss, dx in three_ways(ctx, bits[at], ids[at], values[at], w[at], scale=0.8, teacher_scale=teacher_scale):
+            L.assert_within(loss, loss_want[at], b_loss[at], f"{name}: loss, {teacher_scale}")
+            L.assert_within(dx, want[at], b_grad[at], f"{name}: gradient, {teacher_scale}")
