@@ -217,7 +217,9 @@ __device__ __forceinline__ RowSums finish_row(const DsArgs& a, const RowStat& pa
     const RowStat all = TAIL ? merge_stat<false>(pass, own, a.c) : pass;
     const float log_s = logf(all.s);
     loss = term;
-    if (t.mass != 0.0f) loss = loss + t.mass * ((all.m - base) * a.scale + log_s);
+    // (base is the largest logit of the ids, so that the distance is not negative; if all of them are at -inf it is 0, term is +inf,
+    // and a distance below 0, down to -inf by the scale, must not take that back)
+    if (t.mass != 0.0f) loss = loss + t.mass * (fmaxf((all.m - base) * a.scale, 0.0f) + log_s);
     RowSums s{all.m, log_s, -INFINITY, t.mass};
     if (TAIL && !(pass.m == -INFINITY && pass.s == 0.0f)) {
         s.log_rest = (pass.m - all.m) * a.scale + (logf(pass.s) - log_s);

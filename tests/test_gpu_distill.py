@@ -471,3 +471,29 @@ def test_teachers_far_from_zero(ctx, V, copies, dtype):
         for name, loss, dx in three_ways(ctx, bits[at], ids[at], values[at], w[at], scale=0.8, teacher_scale=teacher_scale):
             L.assert_within(loss, loss_want[at], b_loss[at], f"{name}: loss, {teacher_scale}")
             L.assert_within(dx, want[at], b_grad[at], f"{name}: gradient, {teacher_scale}")
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V,copies", [(20, 1), (300, 1), (5003, 1), (60000, 1), (60000, 40)])
+def test_masked_ids_among_classes_at_the_lowest_value(ctx, V, copies, dtype, tail):
+    """mass on classes at -inf alone: the loss is +inf, whatever the others' offset times the scale is; the gradient is that of
+    equal classes (p = 1 / n, a sum of ones: exact but for sum_error and a few roundings)"""
+    rng = np.random.default_rng(V)
+    rows, K = 2, 5
+    low = float(np.finfo(np.float32).min) if dtype == "f32" else -3.3895313892515355e38
+    ids, values = L.teacher(rng, rows, V, K, tail, ragged=False)
+    x = np.full((rows, V), low, np.float32)
+    np.put_along_axis(x, ids, -np.inf, 1)
+    at = np.tile(np.arange(rows), copies)
+    w = np.array([1.0, -0.5], np.float32)
+    for scale in (1.0, 1.5):
+        loss_want, dz = cf.topk_distill(x, ids, values, scale, tail=tail)
+        assert np.isposinf(loss_want).all()
+        want = dz * w[:, None]
+        # W <= 1 plus roundings; among the others p W - r q_rest, r = p: terms of 1 / n
+        bound = scale * np.abs(w)[:, None] * (L.sum_error(V) + 2 * U * (K + 64)) * np.where(np.isneginf(x), 1.0, 2.0 / (V - K))
+        bound = bound + (2.0 ** -8 * (np.abs(want) + bound) if dtype == "bf16" else 0.0)
+        for name, loss, dx in three_ways(ctx, L.store(x, dtype)[at], ids[at], values[at], w[at], scale=scale, tail=tail):
+            assert np.isposinf(loss).all(), (name, scale, loss)
+            L.assert_within(dx, want[at], bound[at], f"{name}: gradient, scale {scale}")
