@@ -22,6 +22,7 @@ UNARY_EXP, UNARY_LOG, UNARY_RSQRT = 0, 1, 2
 MUL_SAME, MUL_ROW, MUL_COL, MUL_SCALAR = 0, 1, 2, 3
 DISTILL_RENORM, DISTILL_TAIL = 0, 1
 MAX_TOP = 128
+MAX_TAIL_CLASSES = 5242880
 OK, EINVAL, EHIP, ENOKERNEL, EINDEX, EWORKSPACE = 0, -1, -2, -3, -4, -5
 NOALLOC_SCRATCH_BYTES = 32 << 20
 

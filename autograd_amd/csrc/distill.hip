@@ -34,6 +34,7 @@ constexpr int kDsUnroll = 4;                       // vectors a thread keeps in 
 constexpr uint32_t kMapWords = 5120;               // of the bit map: 163840 classes of a row, or of a part of one
 constexpr uint32_t kMapBits = kMapWords * 32;
 constexpr uint32_t kShortMap = 2048;               // words: 65536 classes
+static_assert(AGRAD_MAX_TAIL_CLASSES == kMaxParts * kMapBits, "a row's parts hold the bits of so many classes");
 static_assert(AGRAD_MAX_TOP <= kDsBlock && AGRAD_MAX_TOP == 2 * kWave, "a thread a teacher slot, the slots of two waves");
 
 struct DsArgs {
@@ -671,10 +672,9 @@ int ds_fwd_typed(hipStream_t s, const T* x, const DsArgs& a, DsOut o, uint64_t r
     const uint32_t vectors = wide ? a.V / WIDE : a.V;
     o.parts = wide ? row_parts(rows, vectors) : 1u;
     uint64_t slab = rows;
-    if (tail && vectors / o.parts + 1 > kMapBits / WIDE) {
+    if (tail && (vectors + o.parts - 1) / o.parts > kMapBits / WIDE) {
         // a part's classes have to fit the bit map: rows longer than it are cut, so many rows a launch as the parts' memory takes
-        o.parts = vectors / (kMapBits / WIDE - 1) + 1;
-        if (o.parts > kMaxParts) return set_error(AGRAD_EINVAL, "top-k distillation with a tail: %u classes are too many", a.V);
+        o.parts = (vectors + kMapBits / WIDE - 1) / (kMapBits / WIDE);             // (at most kMaxParts: the classes are checked)
         slab = kSharedParts / o.parts;
     }
     const uint32_t longest = ((vectors + o.parts - 1) / o.parts) * (wide ? WIDE : 1);        // classes of a part's vectors, at most
@@ -795,6 +795,8 @@ int ds_args(const char* what, int dtype, const void* logits, const int32_t* ids,
         return set_error(AGRAD_EINVAL, "%s: the teacher's scale must be positive and finite", what);
     if (mode == AGRAD_DISTILL_TAIL && teacher_scale != 1.0f)
         return set_error(AGRAD_EINVAL, "%s: log probabilities with a tail are taken as they are (teacher_scale 1)", what);
+    if (mode == AGRAD_DISTILL_TAIL && V > AGRAD_MAX_TAIL_CLASSES)
+        return set_error(AGRAD_EINVAL, "%s: %u classes, at most %u with a tail", what, V, AGRAD_MAX_TAIL_CLASSES);
     if (rows != 0 && (logits == nullptr || ids == nullptr || values == nullptr)) return set_error(AGRAD_EINVAL, "%s: null operand", what);
     const float c = (float)((double)scale * 1.4426950408889634);
     *a = DsArgs{ids, values, ld, V, top, scale, c, teacher_scale, err_flag};

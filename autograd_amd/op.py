@@ -533,6 +533,7 @@ def _inverse_temperature(value, what):
 
 
 MAX_TOP = 128     # classes a row that the operators below take or give (AGRAD_MAX_TOP)
+MAX_TAIL_CLASSES = 5242880     # classes of a row of logits that distillation with a tail takes (AGRAD_MAX_TAIL_CLASSES)
 
 
 class TokenLogprobs(NamedTuple):
@@ -625,6 +626,8 @@ class TopKDistillOp(Op):
                              f"{teacher_values.shape}")
         if not 1 <= teacher_ids.shape[-1] <= MAX_TOP:
             raise ValueError(f"TopKDistill takes 1 to {MAX_TOP} classes a row, got {teacher_ids.shape[-1]}")
+        if self.tail and logits.shape[-1] > MAX_TAIL_CLASSES:
+            raise ValueError(f"TopKDistill: {logits.shape[-1]} classes, at most {MAX_TAIL_CLASSES} with a tail")
         if is_bf16(teacher_ids.dtype) or np.dtype(teacher_ids.dtype) not in INT_DTYPES:
             raise ValueError(f"TopKDistill: teacher ids are int32, got {teacher_ids.dtype}")
         if is_bf16(teacher_values.dtype) or np.dtype(teacher_values.dtype) != np.dtype(np.float32):

@@ -530,7 +530,7 @@ int agrad_token_logprobs_backward(agrad_ctx* ctx, int dtype, const void* logits,
  *                         student's on all other classes, p_rest:
  *                         loss = sum_k q_k (log q_k - log p[id_k]) + q_rest (log q_rest - log p_rest),
  *                         without the last term if q_rest is 0 or no class outside the ids is above -inf.
- *                         teacher_scale must be 1.
+ *                         teacher_scale must be 1, and a row has at most AGRAD_MAX_TAIL_CLASSES classes.
  * The gradient is scale * (p[v] W - sum of q_k with id_k = v) for the classes among the ids and
  * scale * p[v] (W - q_rest / p_rest) for the others, W = sum q + q_rest (RENORM: q_rest = 0).  An id that a row
  * holds twice counts with both its values, its class once.  An id outside [-1, V) sets the deferred index error
@@ -547,6 +547,7 @@ int agrad_token_logprobs_backward(agrad_ctx* ctx, int dtype, const void* logits,
  *   fused     loss (may be NULL) and dlogits = the gradient * (row_scale[r], or grad_scale if row_scale is NULL)
  *             in one launch that reads the logits once where a row fits a workgroup's registers
  * dlogits has the logits' stride and may be the logits (in place). */
+#define AGRAD_MAX_TAIL_CLASSES 5242880
 enum { AGRAD_DISTILL_RENORM = 0, AGRAD_DISTILL_TAIL = 1 };
 int agrad_topk_distill_forward(agrad_ctx* ctx, int dtype, const void* logits, const int32_t* teacher_ids,
                                const float* teacher_values, float* loss, float* stats,

@@ -497,3 +497,48 @@ def test_masked_ids_among_classes_at_the_lowest_value(ctx, V, copies, dtype, tai
         for name, loss, dx in three_ways(ctx, L.store(x, dtype)[at], ids[at], values[at], w[at], scale=scale, tail=tail):
             assert np.isposinf(loss).all(), (name, scale, loss)
             L.assert_within(dx, want[at], bound[at], f"{name}: gradient, scale {scale}")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [capi.MAX_TAIL_CLASSES, capi.MAX_TAIL_CLASSES - 1, 163840, 163841, 2 * 163840 + 3])
+def test_most_classes_with_a_tail(ctx, V, dtype):
+    """rows in as many parts as their bit maps need; the largest fill every part's map"""
+    rng = np.random.default_rng(V)
+    rows = 2 if V > 1000000 else 3
+    x = L.logits(rng, rows, V, dtype)
+    ids, values = L.teacher(rng, rows, V, 40, True)
+    ids[0, :4] = [0, 1, V - 2, V - 1]                # (the first and the last bits)
+    ids[1, :6] = [v for k in (1, 2, 4) for v in (k * (V // 8), k * (V // 8) + 1)]
+    check(ctx, x, ids, values, dtype, tail=True)
+    if V < 1000000:
+        n = 12
+        check(ctx, np.tile(x, (n, 1)), np.tile(ids, (n, 1)), np.tile(values, (n, 1)), dtype, tail=True, ld=V + 3, offset=1)
+
+
+@pytest.mark.parametrize("V", [163840, 163847])
+def test_loss_of_many_rows_as_long_as_a_bit_map(ctx, V):
+    """a workgroup a row, or two where its bits are one map more"""
+    rng = np.random.default_rng(V)
+    rows, n = 3, 344
+    x = L.logits(rng, rows, V, "bf16")
+    ids, values = L.teacher(rng, rows, V, 40, True)
+    ids[0, :4] = [0, 1, V - 2, V - 1]
+    want, dz = cf.topk_distill(x, ids, values, tail=True)
+    bound, _ = bounds(x, ids, values, 1.0, 1.0, True, "bf16", np.ones(rows), dz)
+    got, _ = L.distill_forward(ctx, np.tile(L.store(x, "bf16"), (n, 1)), np.tile(ids, (n, 1)), np.tile(values, (n, 1)), tail=True)
+    L.assert_within(got, np.tile(want, n), np.tile(bound, n), "loss")
+
+
+def test_more_classes_than_a_tail_takes_are_refused(ctx):
+    V = capi.MAX_TAIL_CLASSES + 1
+    with L.Device(ctx) as dev:
+        x, dx = dev.up(np.zeros(V, np.float32)), dev.up(np.zeros(V, np.float32))
+        i, o = dev.up(np.zeros(2, np.int32)), dev.up(np.zeros(16, np.float32))
+        for dtype in (capi.F32, capi.BF16):
+            for name, args in (("forward", (L.p(o), L.p(o), 1, V, V, 2, 1.0, 1.0, 1)), ("backward", (L.p(o), L.p(o), L.p(dx), 1, V, V, 2, 1.0, 1.0, 1, 0)),
+                               ("fused", (L.p(o), None, L.p(dx), 1, V, V, 2, 1.0, 1.0, 1.0, 1))):
+                with pytest.raises(capi.AgradError) as e:
+                    ctx.call("agrad_topk_distill_" + name, dtype, L.p(x), L.p(i), L.p(o), *args)
+                assert e.value.code == capi.EINVAL, name
+        assert not dx.download().any()
+    ctx.synchronize()

@@ -171,3 +171,13 @@ def test_a_student_learns_its_teachers_alternatives_on_the_oracle_device():
         assert before is None or not np.array_equal(value, before)
         before = value
         opt.step()
+
+
+def test_a_tail_takes_so_many_classes():
+    from autograd_amd.op import MAX_TAIL_CLASSES
+    assert MAX_TAIL_CLASSES == capi.MAX_TAIL_CLASSES
+    ids, u = T((1, 2), np.int32, False), T((1, 2), np.float32, False)
+    x, long = (T((1, MAX_TAIL_CLASSES + more), grad=False) for more in (0, 1))
+    assert x.distill_topk(ids, u, tail=True).shape == (1,) and long.distill_topk(ids, u).shape == (1,)
+    with pytest.raises(ValueError):
+        long.distill_topk(ids, u, tail=True)
