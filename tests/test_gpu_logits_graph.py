@@ -280,3 +280,66 @@ def test_buffers_of_another_context_or_too_small_are_refused():
         with pytest.raises(ValueError):
             call(**bad)
     one.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("tail", [False, True])
+def test_step_by_buffer_ids(ctx, dtype, tail):
+    """HipContext.topk_distill_fused: loss and gradient of the C ABI's call, at offsets, in place, without a loss or row scales; operands that
+    are not the context's, or too small, are refused before anything is written"""
+    from autograd_amd import hip_ext
+    rng = np.random.default_rng(21)
+    rows, V, ld, K, lead = 6, 1003, 1024, 9, 32
+    x = L.store(L.logits(rng, rows, V, dtype), dtype)
+    ids, values = L.teacher(rng, rows, V, K, tail)
+    w = rng.standard_normal(rows).astype(np.float32)
+    kw = dict(scale=0.75, teacher_scale=1.0 if tail else 0.5, tail=tail, ld=ld, offset=lead // x.itemsize)
+    want_loss, want = L.distill_fused(ctx, x, ids, values, row_scale=w, **kw)
+    _, flat = L.distill_fused(ctx, x, ids, values, grad_scale=-0.25, **kw)
+    one, other = hip_ext.HipContext(0), hip_ext.HipContext(0)
+    kind, item = (hip_ext.BF16, 2) if dtype == "bf16" else (hip_ext.F32, 4)
+    padded = np.full((rows, ld), L.PAD, x.dtype)
+    padded[:, :V] = x
+
+    def up(context, a):
+        buf = context.alloc(lead + a.nbytes)
+        context.copy_from_host(buf, lead, a)
+        return buf
+
+    def down(buf, like):
+        return one.copy_to_host(buf, lead, list(like.shape), like.dtype.name)
+
+    bx, bi, bv, bw = up(one, padded), up(one, ids), up(one, values), up(one, w)
+    loss0, dx0 = np.full(rows, -7.0, np.float32), np.full((rows, ld), 3, x.dtype)
+    bl, bd = up(one, loss0), up(one, dx0)
+    good = dict(ids=[bx, bi, bv, bl, bw, bd], offs=[lead] * 6, rows=rows, V=V, ld=ld, top=K)
+
+    def call(grad_scale=1.0, **over):
+        a = {**good, **over}
+        one.topk_distill_fused(kind, a["ids"], a["offs"], a["rows"], a["V"], a["ld"], a["top"], kw["scale"], kw["teacher_scale"], grad_scale, int(tail))
+
+    foreign = up(other, padded)
+    for at in range(6):
+        for bad in (foreign, 1):
+            with pytest.raises(ValueError):
+                call(ids=[bad if i == at else b for i, b in enumerate(good["ids"])])
+        with pytest.raises(ValueError):
+            call(offs=[lead + item * (ld - V) + 4 if i == at else lead for i in range(6)])     # (the last row would end behind its buffer)
+    for over in (dict(ids=good["ids"][:5]), dict(offs=[lead] * 5), dict(rows=rows + 1), dict(top=K + 1), dict(ld=ld + 8), dict(ld=V - 1), dict(top=0),
+                 dict(ids=[0, bi, bv, bl, bw, bd]), dict(ids=[bx, 0, bv, bl, bw, bd]), dict(ids=[bx, bi, 0, bl, bw, bd]), dict(ids=[bx, bi, bv, bl, bw, 0])):
+        with pytest.raises(ValueError):
+            call(**over)
+    one.synchronize()
+    np.testing.assert_array_equal(down(bl, loss0), loss0)
+    np.testing.assert_array_equal(down(bd, dx0), dx0)
+    np.testing.assert_array_equal(down(bx, padded), padded)
+
+    call()
+    one.synchronize()
+    np.testing.assert_array_equal(down(bl, loss0), want_loss)
+    np.testing.assert_array_equal(down(bd, dx0)[:, :V], want)
+    assert (down(bd, dx0)[:, V:] == 3).all()
+    call(grad_scale=-0.25, ids=[bx, bi, bv, 0, 0, bx])                 # (no loss, one scale, in place)
+    one.synchronize()
+    np.testing.assert_array_equal(down(bx, padded)[:, :V], flat)
+    np.testing.assert_array_equal(down(bl, loss0), want_loss)
