@@ -48,14 +48,6 @@ struct DsOut {
     SharedRows shared; uint32_t parts;
 };
 
-__device__ __forceinline__ int32_t slot_id(const DsArgs& a, uint64_t row, uint32_t k, bool report) {
-    if (k >= a.top) return -1;
-    const int32_t id = a.ids[row * a.top + k];
-    if (id >= 0 && (uint32_t)id < a.V) return id;
-    if (report && id != -1) *a.err_flag = 1;
-    return -1;
-}
-
 // ---- the bit map of a row's ids -----------------------------------------------------------------------
 template <int BLOCK>
 __device__ __forceinline__ void clear_map(uint32_t* map, uint32_t classes) {
