@@ -343,3 +343,55 @@ def test_step_by_buffer_ids(ctx, dtype, tail):
     one.synchronize()
     np.testing.assert_array_equal(down(bx, padded)[:, :V], flat)
     np.testing.assert_array_equal(down(bl, loss0), want_loss)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, BF16])
+@pytest.mark.parametrize("order", [(0, 1, 2), (2, 0, 1), (1, 2, 0), (2, 1, 0)])
+def test_logits_that_several_operators_read(order, dtype):
+    """cross-entropy, distillation and a policy term of the same logits, whichever writes the gradient first and whichever adds to it"""
+    U = L.U
+    rng = np.random.default_rng(31)
+    B, N, V, K = 2, 7, 259, 5
+    cast = (lambda a: L.rounded(a, "bf16")) if dtype == BF16 else (lambda a: a.astype(np.float32))
+    x_np = cast(2 * rng.standard_normal((B, N, V)))
+    t_np = rng.integers(0, V, (B, N)).astype(np.int32)
+    ids_np, u_np = L.teacher(rng, B * N, V, K, True)
+    adv = rng.standard_normal((B, N)).astype(np.float32)
+    x, t = leaf("hip", x_np.shape, dtype, True, x_np), leaf("hip", t_np.shape, np.int32, False, t_np)
+    ids, u = leaf("hip", (B, N, K), np.int32, False, ids_np.reshape(B, N, K)), leaf("hip", (B, N, K), np.float32, False, u_np.reshape(B, N, K))
+    a = leaf("hip", adv.shape, np.float32, False, adv)
+
+    def policy():
+        said = x.token_logprobs(t, entropy=True, top=3, scale=0.8)
+        return said.logp * a + said.entropy * a
+
+    terms = [lambda: x.cross_entropy(t), lambda: x.distill_topk(ids, u, tail=True, scale=1.25), policy]
+    loss = None
+    for i in order:
+        term = terms[i]()
+        loss = term if loss is None else loss + term
+    rt = compiled("hip", loss)
+    flat, tf = x_np.reshape(-1, V), t_np.reshape(-1)
+    parts = [cf.cross_entropy_grad(flat, tf, np.ones(B * N)), cf.topk_distill(flat, ids_np, u_np, 1.25, tail=True)[1],
+             cf.token_logprobs_grad(flat, tf, adv.reshape(-1), adv.reshape(-1), 0.8)]
+    want = sum(parts)
+    # sizes of what the gradients add up, and relative errors of tests/logits_ops.py (logarithms up to 20 here); bf16: a rounding of each
+    # part and of each sum on the way
+    p1, p2, (p3, l3, _) = cf._softmax_rows(flat)[0], cf._softmax_rows(1.25 * flat)[0], cf._softmax_rows(0.8 * flat)
+    at = (np.arange(V) == tf[:, None]) * 1.0
+    q = np.zeros_like(p1)
+    for r in range(B * N):
+        np.add.at(q[r], ids_np[r][ids_np[r] >= 0], np.exp(u_np[r][ids_np[r] >= 0]))
+    rest = np.where(q == 0, p2, 0.0)
+    size = p1 + at + 2 * p2 + q + rest / rest.sum(-1, keepdims=True) + np.abs(adv).reshape(-1, 1) * (at + p3 * (1 - l3 - (p3 * l3).sum(-1, keepdims=True)))
+    off = L.sum_error(V) + 2 * U * 100
+    bound = (8 * off + (4 * 2.0 ** -8 if dtype == BF16 else 0.0)) * size
+    # (loss: three logarithms, an entropy of up to log V with an error of 2 + 2 log V such, and terms of the ids)
+    b_value = off * (20 + np.abs(adv).reshape(-1) * (3 + 2 * np.log(V)))
+    value = (cf.cross_entropy(flat, tf) + cf.topk_distill(flat, ids_np, u_np, 1.25, tail=True)[0]
+             + sum(cf.token_logprobs(flat, tf, 0.8)[:2]) * adv.reshape(-1))
+    for _ in range(2):
+        rt.backward(loss)
+        L.assert_within(rt.backend.copy_to_host(x.grad), want.reshape(x_np.shape), bound.reshape(x_np.shape), "gradient")
+        L.assert_within(rt.backend.copy_to_host(loss).reshape(-1), value, b_value, "loss")
+    rt.release()
