@@ -728,10 +728,10 @@ bool ds_held_launch(hipStream_t s, const T* x, T* dx, const DsArgs& a, const DsO
     constexpr int WIDE = WideVec<T>::value;
     const uint32_t vectors = a.V / WIDE;
     const dim3 grid((uint32_t)rows);
-    // Held rows of two 512-thread workgroups a CU are faster than rows read twice (2048 x 50257 bf16 177 against 184 us, 4096 x 32768
-    // fp32 424 against 431).  Beyond them a CU holds 1024 threads at a time: fp32 still gains (512 x 70000 63 against 73 us, 4096 x
-    // 80000 516 against 570, though 4096 x 50257 378 against 365), bf16, with twice the arithmetic a byte and no second workgroup to
-    // fill its waits, loses (1024 x 110000 120 against 106 us, 8192 x 151936 1096 against 1071).
+    // Held rows of two 512-thread workgroups a CU are faster than rows read twice (2048 x 50257 bf16 82 against 95 us, 4096 x 20000 70
+    // against 94, 8192 x 32768 fp32 386 against 419).  Beyond them a CU holds 1024 threads at a time: fp32 still gains or is even (4096 x
+    // 80000 514 against 548 us, 4096 x 50257 346 against 351, 512 x 70000 65 in both), bf16, with twice the arithmetic a byte and no
+    // second workgroup to fill its waits, loses (1024 x 110000 120 against 102 us, 8192 x 151936 1130 against 1075).
 #define AGRAD_DS(N, BLOCK) \
     if (vectors <= (uint32_t)(N) * BLOCK) { hipLaunchKernelGGL((distill_held_kernel<T, WIDE, N, BLOCK, TAIL>), grid, dim3(BLOCK), 0, s, x, dx, a, o); return true; }
     // Short rows take the smallest workgroup that has four vectors a thread and a thread a slot, as the reductions of its waves are

@@ -213,8 +213,10 @@ __device__ __forceinline__ void top_by_steps(uint32_t n, uint32_t top, Candidate
 // 180 for top = 128, as the shares are interleaved).  With them known, the row is not read again but for the lines whose
 // largest logit reaches the bound -- or not at all, where the threads still hold their vectors (HELD; tops: their largest
 // logits).  (Reading the shares again instead of lines reads the whole row: eight threads have a part in each 128 bytes.
-// 8192 rows of 128256 bf16, top 64: 595 us.)  A row whose largest logits are equal in great number, or crowd into few
-// shares, can leave more than LDS holds and goes the slow way.
+// 8192 rows of 128256 bf16, top 64: 595 us.)  A row whose largest logits are equal in great number, share the upper half of their
+// bits, or crowd into few shares, can leave more than LDS holds and goes the slow way: all equal, those rows take 1830 us for 344;
+// fp32 rows about 1000, where an upper half is a step of 4, 750 for 131 (4096 of 50257, top 20); the worst found, such rows in
+// ascending order, 12000.
 template <typename T, int VEC, int BLOCK, bool HELD, int U>
 __device__ __forceinline__ void row_top(const T* base, const RowParts<T, VEC>& parts, const Stretch& part, uint32_t top, float best, float largest,
                                         const typename RawVec<T, VEC>::type (&held)[U], const float (&tops)[U],
@@ -514,7 +516,8 @@ __device__ __forceinline__ void lp_store(T* to, float (&d)[VEC], uint32_t accumu
 // A row whose lse is so large that fp32 holds little of the logarithm beside the offset (all classes at a mask's lowest value:
 // nothing of it, p would be 1 each; with a scale above 1 the lse is -inf like that of a row without classes).  The row's
 // first workgroup takes all of it and sums it up again about its largest logit; it has read the row before it writes, so dx
-// may be x here too.
+// may be x here too.  Reading twice costs many rows a factor of two (4096 of 128256 fp32 1423 us for 684, 2048 of 50257 bf16 141 for
+// 64), a workgroup a row a few long ones more (one row of 151936 bf16 52 us for 4, 256 rows 135 for 26).
 constexpr float kLargeLse = 256.0f;          // (an error of 2^-17 in log p)
 template <typename T, int VEC, int BLOCK>
 __device__ void lp_bwd_row(const T* base, T* out, const RowParts<T, VEC>& parts, LpRow r, uint32_t accumulate) {
