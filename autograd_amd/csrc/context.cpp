@@ -35,6 +35,7 @@ struct agrad_ctx {
     void* ce_scratch = nullptr;
     // what the workgroups that share a row of logits leave for each other (logprobs.hip, distill.hip)
     void* row_scratch = nullptr;
+    std::mutex row_pairs;                  // held while two launches that hand something over in it are enqueued
     uint32_t team_polls = 0;               // 0: the kernels' own bound on a team member's wait
 };
 
@@ -1185,6 +1186,7 @@ int agrad_topk_distill_fused(agrad_ctx* ctx, int dtype, const void* logits, cons
                              const float* teacher_values, float* loss, const float* row_scale, void* dlogits, uint64_t rows,
                              uint32_t V, uint64_t ld, uint32_t top, float scale, float teacher_scale, float grad_scale, int mode) {
     CTX_OR_FAIL(ctx)
+    std::lock_guard<std::mutex> lock(ctx->row_pairs);
     return launch_distill_fused(ctx->stream, dtype, logits, teacher_ids, teacher_values, loss, row_scale, dlogits, rows, V, ld, top,
                                 scale, teacher_scale, grad_scale, mode, ctx->err_flag, ctx->row_scratch);
 }

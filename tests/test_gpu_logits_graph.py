@@ -395,3 +395,32 @@ def test_logits_that_several_operators_read(order, dtype):
         L.assert_within(rt.backend.copy_to_host(x.grad), want.reshape(x_np.shape), bound.reshape(x_np.shape), "gradient")
         L.assert_within(rt.backend.copy_to_host(loss).reshape(-1), value, b_value, "loss")
     rt.release()
+
+
+def test_two_threads_of_one_context(ctx):
+    """the launches of one call follow one another on the stream, whichever thread enqueues in between: a few long rows take two, and the
+    second reads what the first left in the context's memory"""
+    with L.Device(ctx) as dev:
+        calls = [enqueue(ctx, dev, single_rows(ctx, s)) for s in (41, 42, 43)]
+        want = []
+        for launch, results in calls:
+            launch()
+            want.append(results())
+        errors = []
+
+        def work(launch):
+            try:
+                for _ in range(200):
+                    launch()
+            except Exception as e:      # noqa: BLE001
+                errors.append(e)
+
+        threads = [threading.Thread(target=work, args=(c[0],)) for c in calls]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not errors, errors
+        for (_, results), w in zip(calls, want):
+            for k, v in results().items():
+                np.testing.assert_array_equal(v, w[k], err_msg=k)
