@@ -424,3 +424,27 @@ def test_two_threads_of_one_context(ctx):
         for (_, results), w in zip(calls, want):
             for k, v in results().items():
                 np.testing.assert_array_equal(v, w[k], err_msg=k)
+
+
+@pytest.mark.parametrize("fuse", [True, False])
+@pytest.mark.parametrize("read", ["entropy", "logp"])
+def test_outputs_that_nothing_reads(read, fuse):
+    """an output with a gradient of its own that no loss comes from adds nothing, whatever its memory held"""
+    rng = np.random.default_rng(51)
+    B, N, V = 2, 5, 130
+    x_np, t_np = rng.standard_normal((B, N, V)).astype(np.float32), rng.integers(0, V, (B, N)).astype(np.int32)
+    a_np = rng.standard_normal((B, N)).astype(np.float32)
+    x, t, a = leaf("hip", x_np.shape, np.float32, True, x_np), leaf("hip", t_np.shape, np.int32, False, t_np), leaf("hip", a_np.shape, np.float32, False, a_np)
+    said = x.token_logprobs(t, entropy=True, top=4)
+    loss = getattr(said, read) * a
+    rt = compiled("hip", loss, fuse_grad_zeroing=fuse)
+    other = said.logp if read == "entropy" else said.entropy
+    if other.grad is not None:
+        rt.backend.copy_from_host(other.grad, np.full((B, N), 7.0, np.float32))
+    g = a_np.reshape(-1)
+    want = cf.token_logprobs_grad(x_np.reshape(-1, V), t_np.reshape(-1), g if read == "logp" else None, g if read == "entropy" else None)
+    for _ in range(2):
+        rt.backward(loss)
+        # (as above: p (|g| + |h| (|log p| + entropy)) <= 4, with 1e-5)
+        np.testing.assert_allclose(rt.backend.copy_to_host(x.grad).reshape(-1, V), want, rtol=1e-5, atol=1e-5)
+    rt.release()
