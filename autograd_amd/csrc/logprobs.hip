@@ -726,7 +726,8 @@ int logits_check(const char* what, int dtype, const void* x, const void* dx, uin
     if (ld < V || ld > 0xffffffffull) return set_error(AGRAD_EINVAL, "%s: row stride %llu for %u classes", what, (unsigned long long)ld, V);
     // (a launch has fewer than 2^32 threads; the largest workgroup here has 1024)
     if (rows >= 0x00400000ull) return set_error(AGRAD_EINVAL, "%s: at most %u rows a call", what, 0x003fffffu);
-    if (!(scale > 0.0f) || !std::isfinite(scale)) return set_error(AGRAD_EINVAL, "%s: the scale must be positive and finite", what);
+    // (above 2e38 the product with log2(e), by which the kernels take distances, is not finite: a distance of 0 would be NaN)
+    if (!(scale > 0.0f) || !(scale <= 2e38f)) return set_error(AGRAD_EINVAL, "%s: the scale must be positive and at most 2e38", what);
     const uintptr_t es = dtype_size(dtype);
     if (reinterpret_cast<uintptr_t>(x) % es || reinterpret_cast<uintptr_t>(dx) % es)
         return set_error(AGRAD_EINVAL, "%s: logits or gradient not aligned to their elements", what);

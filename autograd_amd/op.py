@@ -527,8 +527,8 @@ class CrossEntropyLossOp(Op):
 
 def _inverse_temperature(value, what):
     value = float(value)
-    if not (0.0 < value < float("inf")):
-        raise ValueError(f"{what} must be positive and finite, got {value}")
+    if not (1e-45 <= value <= 2e38):          # (what fp32 holds, and the kernels' product with log2(e))
+        raise ValueError(f"{what} must be positive, from 1e-45 to 2e38, got {value}")
     return value
 
 

@@ -495,7 +495,7 @@ int agrad_set_team_wait_polls(agrad_ctx* ctx, uint32_t polls);
 /* ---- what a model's logits say about given tokens, and learning from another model's -------------
  * Both operators take logits x[rows, V] with a row stride of ld >= V elements (a vocabulary padded to a
  * multiple of 64 has ld > V; the columns [V, ld) are neither read nor written), fp32 or bf16, and a
- * positive finite `scale`, the inverse temperature: z = scale * x, p = softmax(z).  At most 2^22 - 1 rows
+ * positive `scale` of at most 2e38, the inverse temperature: z = scale * x, p = softmax(z).  At most 2^22 - 1 rows
  * a call.  Neither has a counterpart in the reference. */
 
 /* Log probabilities of given tokens.  Per row, with lse = log sum_v exp(z[v]):

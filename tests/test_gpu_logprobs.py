@@ -456,3 +456,28 @@ def test_equal_logits_have_their_alternatives(ctx, dtype, V):
     got = L.forward(ctx, L.store(x, dtype), np.array([0, V - 1, -1], np.int32), 9)
     check_forward(got, x, np.array([0, V - 1, -1]), 1.0, 9)
     np.testing.assert_array_equal(got["top_ids"], np.tile(np.arange(9), (3, 1)))
+
+
+def test_scales_at_their_ends(ctx):
+    """the largest scale takes the largest logits for the whole distribution, the smallest none; beyond them a call is refused"""
+    x = np.array([[0.0, 1.0, 1.0, -np.inf, 0.5], [-3.0, -2.0, -2.0, -2.0, -np.inf]], np.float32)
+    t = np.array([1, 2], np.int32)
+    for scale, n in ((2e38, (2, 3)), (1e-45, (4, 4))):
+        got = L.forward(ctx, x, t, 2, scale)
+        for r in range(2):
+            assert abs(got["logp"][r] + np.log(n[r])) <= 16 * U and abs(got["entropy"][r] - np.log(n[r])) <= 16 * U
+            assert np.abs(got["top_logp"][r] + np.log(n[r])).max() <= 16 * U
+        loss, stats = L.distill_forward(ctx, x, np.array([[1, 2], [1, 2]], np.int32), np.zeros((2, 2), np.float32), scale=scale)
+        assert np.abs(loss - np.log(np.array(n) / 2.0)).max() <= 32 * U
+    with L.Device(ctx) as dev:
+        d, i, o = dev.up(x), dev.up(np.zeros(16, np.int32)), dev.up(np.zeros(16, np.float32))
+        for bad in (2.1e38, 3.4e38, 1e39):
+            for name, args in (("token_logprobs_forward", (L.p(i), L.p(o), None, None, None, None, 2, 5, 5, 0, bad)),
+                               ("token_logprobs_backward", (L.p(i), L.p(o), None, L.p(o), None, L.p(d), 2, 5, 5, bad, 0)),
+                               ("topk_distill_forward", (L.p(i), L.p(o), L.p(o), None, 2, 5, 5, 1, bad, 1.0, 0)),
+                               ("topk_distill_backward", (L.p(i), L.p(o), L.p(o), L.p(o), L.p(d), 2, 5, 5, 1, bad, 1.0, 0, 0)),
+                               ("topk_distill_fused", (L.p(i), L.p(o), L.p(o), None, L.p(d), 2, 5, 5, 1, bad, 1.0, 1.0, 0))):
+                with pytest.raises(capi.AgradError) as e:
+                    ctx.call("agrad_" + name, capi.F32, L.p(d), *args)
+                assert e.value.code == capi.EINVAL, name
+    ctx.synchronize()

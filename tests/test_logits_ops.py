@@ -181,3 +181,14 @@ def test_a_tail_takes_so_many_classes():
     assert x.distill_topk(ids, u, tail=True).shape == (1,) and long.distill_topk(ids, u).shape == (1,)
     with pytest.raises(ValueError):
         long.distill_topk(ids, u, tail=True)
+
+
+def test_ops_refuse_scales_that_a_call_would_refuse():
+    x, t = T((2, 9)), T((2,), np.int32, False)
+    ids, u = T((2, 4), np.int32, False), T((2, 4), np.float32, False)
+    for bad in (1e-46, 2.1e38, 1e39):
+        for make in (lambda: x.token_logprobs(t, scale=bad), lambda: x.distill_topk(ids, u, scale=bad), lambda: x.distill_topk(ids, u, teacher_scale=bad)):
+            with pytest.raises(ValueError):
+                make()
+    for good in (1e-45, 2e38):
+        x.token_logprobs(t, scale=good), x.distill_topk(ids, u, scale=good, teacher_scale=good)
