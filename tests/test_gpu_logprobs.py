@@ -436,7 +436,7 @@ def assert_order(ctx, dtype, V, rows):
 
 
 @pytest.mark.parametrize("dtype,V", [("f32", 4096), ("f32", 8192), ("f32", 15364), ("f32", 16384), ("f32", 16387),
-                                     ("bf16", 8192), ("bf16", 16384), ("bf16", 30728), ("bf16", 32000), ("bf16", 32768), ("bf16", 32775)])
+                                     ("bf16", 8192), ("bf16", 16384), ("bf16", 30736), ("bf16", 32000), ("bf16", 32768), ("bf16", 32775)])
 def test_alternatives_of_rows_that_fill_their_threads(ctx, dtype, V):
     """rows of 4, 8 and 16 vectors a thread, and next to that: up to all of a thread's vectors are candidates"""
     assert_order(ctx, dtype, V, 0)
